@@ -23,6 +23,12 @@ from .kernels import (  # noqa: F401
     linear_bias_gelu,
     token_pos_embedding,
 )
+from .paged import (  # noqa: F401
+    paged_attention,
+    paged_kv_append,
+    rotary_table,
+    shared_prefix_attention,
+)
 from .model import CutileGPT  # noqa: F401
 from .hf_loader import HFWeightLoader  # noqa: F401
 from . import api  # noqa: F401  (Tile API: cutilegpt_amd.api.tile, configure_tiles, ...)
@@ -43,4 +49,8 @@ __all__ = [
     "linear_bias_gelu",
     "attention_qkv",
     "token_pos_embedding",
+    "paged_kv_append",
+    "paged_attention",
+    "shared_prefix_attention",
+    "rotary_table",
 ]

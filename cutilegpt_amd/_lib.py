@@ -72,6 +72,10 @@ SIGNATURES = {
                            _I64, _I64, _I64, _I64, _I64, _I64, _I, _P]),
     "cgpt_forward": (_I, [_P, _I64, _P, _F, _F, _P, _P, _P]),
     "cgpt_argmax": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I64, _P, _P]),
+    "cgpt_paged_kv_append": (_I, [_P] * 10 + [_I64] * 26 + [_I, _I, _P, _P]),
+    "cgpt_paged_attention": (_I, [_P] * 7 + [_I64] * 19 + [_F, _P, _I64, _I, _P, _P]),
+    "cgpt_shared_prefix_attention": (_I, [_P] * 8 + [_I64] * 20 + [_F, _P, _I64, _I, _P, _P]),
+    "cgpt_paged_attention_workspace": (_I, [_I64] * 8 + [_I, _P]),
     "cgpt_partials_bias_act": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I64, _I, _I,
                                     _P]),
 }

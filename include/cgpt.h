@@ -421,6 +421,79 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
                   void* stream);
 
 /*
+ * The paged key-value cache.  Pools hold pages of page_size rows: element (page,
+ * head, slot, d) of k_cache at base + page*kc_sp + head*kc_sh + slot*kc_ss + d,
+ * of v_cache with the vc_ strides; rows separate and 16-byte aligned, strides
+ * multiples of 16 bytes.  Row b of block_table (max_pages int32, rows bt_stride
+ * apart) names sequence b's pages: its key t is in slot t % page_size of page
+ * block_table[b][t / page_size].  seq_lens[b] (device int32) counts its keys, those
+ * of the step's tokens, its last ones, included.  The tokens are packed rows: token b
+ * for sequence b (cu_q NULL, n_tokens == B), or cu_q[b] .. cu_q[b+1]-1 (B + 1 device
+ * int32); rows behind cu_q[B] are neither read nor written.  Element (token, head,
+ * d) of q, k, v and the outputs at base + token*st + head*sh + d, 16-byte
+ * aligned.  Hq is a multiple of Hkv; head_dim is 16, 32, 64 or 128; dtype fp32, bf16
+ * or fp16; n_pages * page strides may pass 32 bits; page_size * max_pages < 2^30.
+ *
+ * Device values that are out of range fault nothing and set *err_flag (a device int,
+ * may be NULL) to 1: a page id outside [0, n_pages) is not written, and read as
+ * page 0; a length past max_pages * page_size is cut there; a position past the
+ * rotation table takes its last row.  Positions below 0 (padding rows of length
+ * 0) are skipped and set nothing.
+ *
+ * cgpt_paged_kv_append: k and v (Hkv heads) into their pages; with rot_dim > 0 the
+ * first rot_dim values of every key, and of q (Hq heads, written to q_out, which may
+ * be q; both may be NULL), are turned by the token's position p: pairs (i,
+ * i + rot_dim/2), or (2i, 2i+1) when interleaved, (x, y) -> (x c - y s, y c + x s) with
+ * c = rotary[p][i], s = rotary[p][rot_dim/2 + i] (fp32, n_pos rows rot_stride apart), in
+ * fp32 and rounded once.  Two tokens of a call must not share a slot.
+ *
+ * cgpt_paged_attention: o = softmax(q K^T * scale) V of every token over the keys
+ * at positions up to its own; rows without a key give zeros.  Query head h reads
+ * key head h / (Hq/Hkv).  Statistics and sums are fp32; P is rounded to dtype
+ * before P V, as in cgpt_attention_fwd.  cgpt_shared_prefix_attention: the same,
+ * keys below prefix_len read from the pages prefix_pages (device int32) for every
+ * sequence, once for all.  workspace: 16-byte aligned device memory of at least the
+ * bytes that cgpt_paged_attention_workspace gives for the same sizes (prefix_len 0
+ * for cgpt_paged_attention), not shared by calls that may overlap; it needs no
+ * clearing.
+ *
+ * No counterpart in the reference, which keeps no cache and runs
+ * cutile_causal_attention over the whole prefix for every token
+ * (cutile_gpt/models/gpt.py:185-229, kernels/attention.py:24-175).
+ */
+int cgpt_paged_kv_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                         void* v_cache, const int* block_table, const int* seq_lens,
+                         const int* cu_q, const float* rotary, int64_t n_tokens, int64_t B,
+                         int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t page_size,
+                         int64_t n_pages, int64_t max_pages, int64_t bt_stride, int64_t q_st,
+                         int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                         int64_t qo_st, int64_t qo_sh, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
+                         int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, int64_t rot_dim,
+                         int64_t n_pos, int64_t rot_stride, int interleaved, int dtype,
+                         int* err_flag, void* stream);
+int cgpt_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
+                         const int* block_table, const int* seq_lens, const int* cu_q,
+                         int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
+                         int64_t page_size, int64_t n_pages, int64_t max_pages, int64_t bt_stride,
+                         int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh, int64_t kc_sp,
+                         int64_t kc_sh, int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss,
+                         float scale, void* workspace, int64_t workspace_bytes, int dtype,
+                         int* err_flag, void* stream);
+int cgpt_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
+                                 const int* block_table, const int* seq_lens, const int* cu_q,
+                                 const int* prefix_pages, int64_t prefix_len, int64_t n_tokens,
+                                 int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
+                                 int64_t page_size, int64_t n_pages, int64_t max_pages,
+                                 int64_t bt_stride, int64_t q_st, int64_t q_sh, int64_t o_st,
+                                 int64_t o_sh, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
+                                 int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, float scale,
+                                 void* workspace, int64_t workspace_bytes, int dtype,
+                                 int* err_flag, void* stream);
+int cgpt_paged_attention_workspace(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv,
+                                   int64_t head_dim, int64_t page_size, int64_t max_pages,
+                                   int64_t prefix_len, int dtype, int64_t* workspace_bytes);
+
+/*
  * Greedy token per row: ids[r] = argmax_c x[r * ld + c] (the first maximum;
  * NaN entries are skipped), also stored at hist[r * hist_ld + *step_dev] when
  * hist is not NULL (step_dev NULL: column 0).  Replaces the top_k = 1 case of
