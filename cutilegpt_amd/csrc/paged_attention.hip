@@ -3,9 +3,31 @@
 // o[i, h] = softmax(scale q[i, h] K^T) V over the keys 0 .. pos(i) of token i's
 // sequence, read from its pages; with a shared prefix the first prefix_len keys of
 // every sequence are read from one list of pages.
+#include <algorithm>
+
+#include "internal.h"
 #include "paged.h"
 
 namespace cgpt {
+
+// Chunk swizzle of V row `key` in LDS.  16-bit rows are read by transposing loads, eight
+// rows apart in the low bits; fp32 columns by four lane groups, four rows apart.
+template <typename T, int CPR> __device__ __forceinline__ int vswz(int key) {
+  if (sizeof(T) == 2) return key & ((CPR < 8 ? CPR : 8) - 1);
+  return ((key >> 2) << 2) & (CPR - 1);
+}
+
+// Half of a V^T operand: the 16-lane group's lane k points at 4 consecutive d of its
+// row and receives the 4 keys of column 16 dt + k.
+template <int KROW, int SWZ>
+__device__ __forceinline__ u32x2_t vt_read(const uint8_t* sv, int row, int dt, int frow) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  const int byte = dt * 32 + 8 * (frow & 3);
+  const uint8_t* p = sv + row * KROW + (((byte >> 4) ^ (row & SWZ)) << 4) + (byte & 15);
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)((__attribute__((address_space(3))) uint8_t*)(p)));
+  return __builtin_bit_cast(u32x2_t, r);
+}
 
 struct PagedAttnArgs {
   const void* q;
@@ -16,89 +38,713 @@ struct PagedAttnArgs {
   int prefix_len, prefix_cols;
   int64_t q_st, q_sh, o_st, o_sh;
   int Hq, Hkv;
+  FastDiv group;  // query heads a key head
   float scale_log2;
   int* err;
 };
 
-constexpr int kRowThreads = 256;
+// ------------------------------------------------------------------ work units
+//
+// The work is a list of items, each one tile of R query rows of one key head against
+// a run of keys:
+//   * (prefix only) rows are the packed tokens of all sequences, token-major, G
+//     heads each; keys are [0, prefix_len);
+//   * rows are one sequence's; keys are [prefix_len, length).
+// An item's keys are cut into units of UK.  The units of all items, in order (prefix:
+// head, row tile, unit; then sequence, head, row tile, unit), are dealt to the blocks in
+// equal contiguous runs, so a batch of any lengths keeps every CU busy to the end: the
+// lengths live on the device, and the host launches one grid for all of them.  A run
+// ends inside an item at most twice; those pieces leave (m, l, O) partials, which the
+// join kernel adds in key order.  Nothing depends on which block runs first.
 
-// One wave per (token, head): 64 keys at a time, a lane's key against the whole
-// query, then a running softmax and the values with a lane per column.
-template <typename T, int HD>
-__global__ __launch_bounds__(kRowThreads) void paged_rows_kernel(PagedAttnArgs a) {
-  constexpr int EPV = Elem<T>::kVec, DPL = (HD + 63) / 64;
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * (kRowThreads / 64) + (threadIdx.x >> 6);
-  if (row >= a.seq.n_tokens * a.Hq) return;
-  const int t = row / a.Hq, h = row % a.Hq, hk = h / (a.Hq / a.Hkv);
-  const int b = seq_of(a.seq, t);
-  if (b >= a.seq.B) return;
-  int first, count;
-  seq_tokens(a.seq, b, &first, &count);
-  const int len = a.seq.lens[b];
-  bool bad = len > a.seq.cap;
-  const int n = min(len - count + (t - first) + 1, a.seq.cap);  // keys this row sees
-  const T* q = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
-  const int* trow = a.seq.table + b * a.seq.stride;
-  float m = -INFINITY, l = 0.f, acc[DPL];
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-  for (int k0 = 0; k0 < n; k0 += 64) {
-    const int key = min(k0 + lane, n - 1);
-    const int col = a.seq.page.div(key), slot = key - col * static_cast<int>(a.seq.page.d);
-    const int page = page_of(key < a.prefix_len ? a.prefix : trow, col, a.seq.n_pages, &bad);
-    const int64_t kr = page * a.kc.sp + hk * a.kc.sh + slot * a.kc.ss;
-    const int64_t vr = page * a.vc.sp + hk * a.vc.sh + slot * a.vc.ss;
-    const T* kp = static_cast<const T*>(a.kc.base) + kr;
-    float s = 0.f;
-    for (int c = 0; c < HD; c += EPV) {
-      float kv[EPV], qv[EPV];
-      load_vec(kp + c, kv);
-      load_vec(q + c, qv);
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) s = fmaf(kv[e], qv[e], s);
-    }
-    s = k0 + lane < n ? s * a.scale_log2 : -INFINITY;
-    const float mn = fmaxf(m, wave_max(s));
-    const float shift = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - shift), p = __builtin_amdgcn_exp2f(s - shift);
-    m = mn;
-    l = l * alpha + wave_sum(p);
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[i] *= alpha;
-    const int live = min(64, n - k0);
-    for (int j = 0; j < live; ++j) {
-      const int64_t r = __shfl(vr, j, 64);
-      const float pj = __shfl(p, j, 64);
-      const T* vp = static_cast<const T*>(a.vc.base) + r;
-#pragma unroll
-      for (int i = 0; i < DPL; ++i)
-        if (lane + 64 * i < HD) acc[i] = fmaf(pj, Elem<T>::load(vp + lane + 64 * i), acc[i]);
-    }
-  }
-  if (bad && a.err != nullptr) *a.err = 1;
-  T* o = static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh;
-#pragma unroll
-  for (int i = 0; i < DPL; ++i)
-    if (lane + 64 * i < HD) Elem<T>::store(o + lane + 64 * i, l > 0.f ? acc[i] / l : 0.f);
+struct SeqUnits {
+  int first, count;  // tokens
+  int len, n;        // keys; keys the table can name (0 without a token)
+  int kb, base0;     // first own key, and the 16-key boundary at or below it
+  int rt, kt;        // row tiles, key units
+};
+
+template <int R, int UK>
+__device__ __forceinline__ SeqUnits seq_units(const PagedAttnArgs& a, int b) {
+  SeqUnits u;
+  seq_tokens(a.seq, b, &u.first, &u.count);
+  u.len = max(a.seq.lens[b], 0);
+  u.n = u.count > 0 ? min(u.len, a.seq.cap) : 0;
+  u.kb = a.prefix_len;
+  u.base0 = u.kb & ~15;
+  u.rt = (u.count * (a.Hq / a.Hkv) + R - 1) / R;
+  u.kt = u.n > u.kb ? (u.n - u.base0 + UK - 1) / UK : 0;
+  return u;
 }
 
-template <typename T, int HD>
-static int launch_rows(const PagedAttnArgs& a, hipStream_t s) {
-  const int64_t rows = static_cast<int64_t>(a.seq.n_tokens) * a.Hq;
-  hipLaunchKernelGGL((paged_rows_kernel<T, HD>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kRowThreads), 0, s, a);
+// Blocks that share U units, and the block that owns unit u when block i owns
+// [i U / g, (i + 1) U / g).
+__device__ __forceinline__ int active_blocks(int grid, int U) { return min(grid, max(U, 1)); }
+__device__ __forceinline__ int unit_start(int i, int U, int g) {
+  return static_cast<int>(static_cast<int64_t>(i) * U / g);
+}
+__device__ __forceinline__ int unit_owner(int u, int U, int g) {
+  return static_cast<int>(((static_cast<int64_t>(u) + 1) * g - 1) / U);
+}
+
+// The workspace: unit starts of the sequences; the two edge partials of every block
+// (2 x R rows each); with a prefix also one partial a row for the items that one block
+// holds whole.
+struct PagedWs {
+  int* starts;       // B + 1
+  float* edge_ml;    // grid x 2 x R x {m, l}
+  float* edge_o;     // grid x 2 x R x HD
+  float* whole_ml;   // {prefix, own} x n_tokens x Hq x {m, l}
+  float* whole_o;    // {prefix, own} x n_tokens x Hq x HD
+};
+
+template <typename T, int HD, int QTW>
+struct StreamShape {
+  static constexpr int ES = sizeof(T);
+  static constexpr int EPC = 16 / ES;              // elements of a 16-byte chunk
+  static constexpr int CPR = HD / EPC;             // chunks of a row
+  static constexpr int SWZ = (CPR < 8 ? CPR : 8) - 1;
+  static constexpr int KSTEP = 4 * EPC;            // head_dim of one k-slab
+  static constexpr int NKS = (HD + KSTEP - 1) / KSTEP;
+  static constexpr int ND = HD / 16;
+  static constexpr int NT = (ES == 2 ? 2 : 1) * (HD >= 64 ? 1 : 2);  // 16-key tiles a wave takes at once
+  static constexpr int KT = 16 * NT;
+  static constexpr int UK = 4 * KT;                // keys of a unit
+  static constexpr int QT = QTW, R = 16 * QTW;
+  static constexpr int KROW = HD * ES;
+  static constexpr int VBYTES = KT * KROW;         // a wave's V tile in LDS; holds 16 fp32 rows of O too
+  // Chunk of a row that lane group g takes in slab ks; rows of 16 16-bit values have but two.
+  __device__ static constexpr bool has(int ks, int g) { return CPR >= 4 * NKS || 4 * ks + g < CPR; }
+  __device__ static constexpr int chunk(int ks, int g) { return has(ks, g) ? 4 * ks + g : CPR - 1; }
+  static_assert(VBYTES >= 16 * HD * 4, "the join of the waves reuses the V tiles");
+};
+
+constexpr int kStreamThreads = 256;
+
+// Bit 31 (or, of a 16-bit type, 15) set where a value of the word is not finite: its
+// exponent field, all ones, carries into the sign.
+template <typename T> __device__ __forceinline__ uint32_t special_bits(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return ((w & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+  if constexpr (std::is_same<T, bf16_t>::value) return (w & 0x7f807f80u) + 0x00800080u;
+  return (w & 0x7c007c00u) + 0x04000400u;
+}
+// The word with 0 in the place of values that are not finite.
+template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return special_bits<T>(w) ? 0u : w;
+  const uint32_t bits = special_bits<T>(w);
+  return w & ~(((bits & 0x80000000u) ? 0xffff0000u : 0u) | ((bits & 0x8000u) ? 0xffffu : 0u));
+}
+
+// Each wave streams keys by itself: K and V rows go from their pages into registers,
+// one subtile of KT keys ahead of the one in use, in the layout of the matrix cores' A
+// operand (lane l: row l % 16, 16-byte chunk l / 16), so S^T = K Q^T needs no LDS at
+// all; V passes through the wave's own LDS tile for its transpose (O^T = V^T P^T).
+// The four waves of a block take the KT-key quarters of a unit and meet only at an
+// item's end.  P comes straight from the S^T accumulators, the key order inside a slab
+// permuted alike on both operands.
+//
+// A16: page_size is a multiple of 16, so 16 keys lie in one page and the page comes by a
+// scalar load; else every lane looks its own key up.
+template <typename T, int HD, int QTW, bool A16>
+__global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2) void paged_stream_kernel(
+    PagedAttnArgs a, PagedWs ws, int prefix_units) {
+  using C = StreamShape<T, HD, QTW>;
+  constexpr int QT = C::QT, NT = C::NT, NKS = C::NKS, ND = C::ND, KT = C::KT, UK = C::UK, R = C::R;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * C::VBYTES];
+  __shared__ float wave_m[4][R], wave_l[4][R];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int g = lane >> 4, frow = lane & 15;
+  const int G = a.Hq / a.Hkv, page_size = static_cast<int>(a.seq.page.d);
+  uint8_t* const sv = smem + wave * C::VBYTES;
+  bool bad = false;
+
+  // Units of the sequences, 64 at a time: lane l holds sequence c0 + l.
+  int c0 = 0, n_units = 0, incl = 0, before = prefix_units, total = 0;
+  auto load_chunk = [&](int c) __attribute__((always_inline)) {
+    c0 = c;
+    n_units = 0;
+    if (c + lane < a.seq.B) {
+      const SeqUnits u = seq_units<R, UK>(a, c + lane);
+      n_units = u.rt * u.kt * a.Hkv;
+    }
+    incl = n_units;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += v;
+    }
+    total = __builtin_amdgcn_readlane(incl, 63);
+  };
+  int U = prefix_units;
+  for (int c = 0; c < a.seq.B; c += 64) {
+    load_chunk(c);
+    if (blockIdx.x == 0 && wave == 0 && c + lane < a.seq.B) ws.starts[c + lane] = U + incl - n_units;
+    U += total;
+  }
+  if (blockIdx.x == 0 && tid == 0) ws.starts[a.seq.B] = U;
+  if (a.seq.B > 64) load_chunk(0);
+  const int gblocks = active_blocks(gridDim.x, U);
+  if (static_cast<int>(blockIdx.x) >= gblocks || U == 0) return;
+  int u = unit_start(blockIdx.x, U, gblocks);
+  const int u_end = unit_start(blockIdx.x + 1, U, gblocks);
+
+  while (u < u_end) {
+    // Addresses are made anew for every item: kept over the loop they cost registers that
+    // the loads in flight need.
+    asm volatile("" : "+v"(g), "+v"(frow));
+    // ---- the item that unit u lies in
+    const bool prefix = u < prefix_units;
+    int hk, rt, t0, kt_item, b = 0, n, kb, base0, rows, first = 0, pos0 = 0;
+    const int* trow;
+    if (prefix) {
+      kt_item = (a.prefix_len + UK - 1) / UK;
+      rows = a.seq.n_tokens * G;
+      const int rts = (rows + R - 1) / R;
+      const int item = u / kt_item;
+      t0 = u - item * kt_item;
+      hk = item / rts;
+      rt = item - hk * rts;
+      n = a.prefix_len;
+      kb = base0 = 0;
+      trow = a.prefix;
+    } else {
+      while (u >= before + total) {
+        before += total;
+        load_chunk(c0 + 64);
+      }
+      const int at = __popcll(__builtin_amdgcn_ballot_w64(before + incl <= u));
+      b = c0 + at;
+      const SeqUnits su = seq_units<R, UK>(a, b);
+      const int rel = u - before - __builtin_amdgcn_readlane(incl - n_units, at);
+      kt_item = su.kt;
+      const int item = rel / su.kt;
+      t0 = rel - item * su.kt;
+      hk = item / su.rt;
+      rt = item - hk * su.rt;
+      kb = su.kb;
+      base0 = su.base0;
+      rows = su.count * G;
+      first = su.first;
+      pos0 = su.len - su.count;
+      // Keys that the tile's last row sees.
+      const int last = a.group.div(min(rt * R + R, rows) - 1);
+      n = min(su.n, max(pos0 + last + 1, 0));
+      trow = a.seq.table + b * a.seq.stride;
+      bad |= su.len > a.seq.cap;
+    }
+    const int t1 = min(kt_item, t0 + (u_end - u));
+    u += t1 - t0;
+
+    // ---- its rows: lane (g, frow) works for rows rt R + 16 qt + frow
+    const int r0 = rt * R, nqt = min(QT, (rows - r0 + 15) >> 4);
+    int lim[QT];  // last key the row sees; rows that do not exist are never masked
+    u32x4_t qf[QT][NKS];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int r = r0 + 16 * qt + frow;
+      const bool live = r < rows;
+      const int i = a.group.div(live ? r : 0), h = hk * G + (live ? r : 0) - i * G;
+      const int t = first + i;
+      if (prefix) {
+        const int bb = seq_of(a.seq, t);
+        int f, c;
+        lim[qt] = -1;
+        if (bb < a.seq.B) {
+          seq_tokens(a.seq, bb, &f, &c);
+          lim[qt] = min(a.seq.lens[bb] - c + (t - f), a.prefix_len - 1);
+        }
+      } else {
+        lim[qt] = min(pos0 + i, n - 1);
+      }
+      if (!live) lim[qt] = 0x7fffffff;
+      const T* qp = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + C::chunk(ks, g) * C::EPC);
+        qf[qt][ks] = live && C::has(ks, g) ? v : u32x4_t{0, 0, 0, 0};
+      }
+    }
+    f32x4_t o[QT][ND];
+    float m_run[QT], l_run[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      m_run[qt] = -INFINITY;
+      l_run[qt] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) o[qt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- its keys
+    const T* const kh = static_cast<const T*>(a.kc.base) + hk * a.kc.sh;
+    const T* const vh = static_cast<const T*>(a.vc.base) + hk * a.vc.sh;
+    const int sub0 = base0 + t0 * UK + wave * KT;  // first subtile; the next is UK further
+    const int cnt = sub0 < n ? min(t1 - t0, (n - sub0 + UK - 1) / UK) : 0;
+    u32x4_t kf[NT][NKS], vf[NT][NKS];
+    // Pages of subtile i: one a 16-key tile, or one a lane's key.
+    auto fetch = [&](int i, int (&pg)[NT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt) {
+        const int tile = sub0 + i * UK + 16 * kt;
+        if (A16) {
+          const int col = a.seq.page.div(min(tile, (n - 1) & ~15));
+          pg[kt] = ((const __attribute__((address_space(4))) int*)trow)[__builtin_amdgcn_readfirstlane(col)];
+        } else {
+          pg[kt] = trow[a.seq.page.div(max(min(tile + frow, n - 1), kb))];
+        }
+      }
+    };
+    auto load = [&](int i, const int (&pg)[NT], u32x4_t (&kd)[NT][NKS], u32x4_t (&vd)[NT][NKS]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt) {
+        const int key = max(min(sub0 + i * UK + 16 * kt + frow, n - 1), kb);
+        const int slot = key - a.seq.page.div(key) * page_size;
+        int p = pg[kt];
+        if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) {
+          p = 0;
+          bad = true;
+        }
+        const T* kp = kh + p * a.kc.sp + slot * a.kc.ss;
+        const T* vp = vh + p * a.vc.sp + slot * a.vc.ss;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+          const int c = C::chunk(ks, g);
+          kd[kt][ks] = *reinterpret_cast<const u32x4_t*>(kp + c * C::EPC);
+          vd[kt][ks] = *reinterpret_cast<const u32x4_t*>(vp + c * C::EPC);
+          // Lanes past a short row's chunks: 0 x inf would be NaN.
+          if (!C::has(ks, g)) kd[kt][ks] = u32x4_t{0, 0, 0, 0};
+        }
+      }
+    };
+    auto v_slot = [&](int kt, int ks) __attribute__((always_inline)) {
+      const int key = 16 * kt + frow;
+      return sv + key * C::KROW + (((4 * ks + g) ^ vswz<T, C::CPR>(key)) << 4);
+    };
+    auto compute = [&](int base, const u32x4_t (&kd)[NT][NKS], const u32x4_t (&vd)[NT][NKS]) __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+          if (C::has(ks, g)) *reinterpret_cast<u32x4_t*>(v_slot(kt, ks)) = vd[kt][ks];
+      asm volatile("" ::: "memory");
+      f32x4_t s[QT][NT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) s[qt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+        if (qt < nqt)
+#pragma unroll
+          for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) Mfma<T>::run(kd[kt][ks], qf[qt][ks], s[qt][kt]);
+      bool masked = false;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+        if (qt < nqt) {
+          if (base < kb || __builtin_amdgcn_ballot_w64(lim[qt] < base + KT - 1) != 0) {
+            masked = true;
+            const int hi = lim[qt] - base - 4 * g, lo = kb - base - 4 * g;
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                s[qt][kt][r] = (16 * kt + r > hi || 16 * kt + r < lo) ? -INFINITY : s[qt][kt][r];
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[qt][kt][r]);
+          mx = column_max(mx) * a.scale_log2;
+          // The shift moves only when the maximum outgrows it by more than 8, so P <= 2^8
+          // and the accumulators are rescaled on few subtiles.
+          const bool grow = mx > m_run[qt] + 8.0f;
+          if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+            const float m_new = grow ? mx : m_run[qt];
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[qt] - m_new) : 1.0f;
+            m_run[qt] = m_new;
+            l_run[qt] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[qt][dt][r] *= alpha;
+          }
+          const float shift = m_run[qt] == -INFINITY ? 0.f : -m_run[qt];
+          float sum = 0.f;
+#pragma unroll
+          for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][kt][r], a.scale_log2, shift));
+              s[qt][kt][r] = p;
+              sum += p;
+            }
+          l_run[qt] += sum;
+        }
+      // A masked key's weight is 0, but 0 x NaN is NaN.  Where a masked subtile holds values
+      // that are not finite, those are added here, key by key, to the rows that see them,
+      // and the matrix cores get the finite ones.
+      if (masked) {
+        uint32_t odd[NT], any = 0;
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int ks = 0; ks < NKS; ++ks)
+            if (C::has(ks, g)) {
+              const u32x4_t v = *reinterpret_cast<const u32x4_t*>(v_slot(kt, ks));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) bits |= special_bits<T>(v[e]);
+            }
+          const uint64_t m = __builtin_amdgcn_ballot_w64((bits & 0x80008000u) != 0);
+          odd[kt] = static_cast<uint32_t>(m | m >> 16 | m >> 32 | m >> 48) & 0xffffu;
+          any |= odd[kt];
+        }
+        if (__builtin_expect(any != 0, 0)) {
+#pragma unroll 1
+          for (int j = 0; j < KT; ++j) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int kt = 0; kt < NT; ++kt) bits = kt == j >> 4 ? odd[kt] : bits;
+            if (!((bits >> (j & 15)) & 1)) continue;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              float p = 0.f;
+#pragma unroll
+              for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p = kt == j >> 4 && r == (j & 3) ? s[qt][kt][r] : p;
+              p = __shfl(p, (j & 12) * 4 + frow, 64);
+              const bool seen = base + j <= lim[qt] && base + j >= kb;
+#pragma unroll
+              for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int d = 16 * dt + 4 * g + e;
+                  const float v = Elem<T>::load(reinterpret_cast<const T*>(
+                      sv + j * C::KROW + (((d / C::EPC) ^ vswz<T, C::CPR>(j)) << 4)) + d % C::EPC);
+                  if (seen && !(fabsf(v) < INFINITY)) o[qt][dt][e] = fmaf(p, v, o[qt][dt][e]);
+                }
+            }
+          }
+#pragma unroll
+          for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks)
+              if (C::has(ks, g)) {
+                u32x4_t* const v = reinterpret_cast<u32x4_t*>(v_slot(kt, ks));
+                u32x4_t w = *v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = finite_part<T>(w[e]);
+                *v = w;
+              }
+          asm volatile("" ::: "memory");
+        }
+      }
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int c = 0; c < NT / 2; ++c) {
+          u32x4_t pf[QT];
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            pf[qt] = u32x4_t{pack2<T>(s[qt][2 * c][0], s[qt][2 * c][1]), pack2<T>(s[qt][2 * c][2], s[qt][2 * c][3]),
+                             pack2<T>(s[qt][2 * c + 1][0], s[qt][2 * c + 1][1]),
+                             pack2<T>(s[qt][2 * c + 1][2], s[qt][2 * c + 1][3])};
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            const u32x2_t lo = vt_read<C::KROW, C::SWZ>(sv, 32 * c + 4 * g + (frow >> 2), dt, frow);
+            const u32x2_t hi = vt_read<C::KROW, C::SWZ>(sv, 32 * c + 16 + 4 * g + (frow >> 2), dt, frow);
+            const u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              if (qt < nqt) Mfma<T>::run(w, pf[qt], o[qt][dt]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            u32x4_t w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int key = 16 * kt + 4 * g + j, d = 16 * dt + frow;
+              w[j] = *reinterpret_cast<const uint32_t*>(sv + key * C::KROW + (((d >> 2) ^ vswz<T, C::CPR>(key)) << 4) +
+                                                        4 * (d & 3));
+            }
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              if (qt < nqt) {
+                const u32x4_t pf = {__float_as_uint(s[qt][kt][0]), __float_as_uint(s[qt][kt][1]),
+                                    __float_as_uint(s[qt][kt][2]), __float_as_uint(s[qt][kt][3])};
+                Mfma<T>::run(w, pf, o[qt][dt]);
+              }
+          }
+      }
+      asm volatile("" ::: "memory");
+    };
+    if (cnt > 0) {
+      int pg[NT];
+      fetch(0, pg);
+      load(0, pg, kf, vf);
+      fetch(1, pg);
+#pragma unroll 1
+      for (int i = 0; i < cnt; ++i) {
+        u32x4_t kn[NT][NKS], vn[NT][NKS];
+        if (i + 1 < cnt) {
+          int pn[NT];
+          fetch(i + 2, pn);
+          load(i + 1, pg, kn, vn);
+#pragma unroll
+          for (int kt = 0; kt < NT; ++kt) pg[kt] = pn[kt];
+        }
+        compute(sub0 + i * UK, kf, vf);
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+          for (int ks = 0; ks < NKS; ++ks) {
+            kf[kt][ks] = kn[kt][ks];
+            vf[kt][ks] = vn[kt][ks];
+          }
+      }
+    }
+
+    // ---- the four waves' parts joined
+    const bool whole = t0 == 0 && t1 == kt_item;
+    const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      if (qt >= nqt) break;
+      const float l = column_sum(l_run[qt]);
+      if (g == 0) {
+        wave_m[wave][16 * qt + frow] = m_run[qt];
+        wave_l[wave][16 * qt + frow] = l;
+      }
+    }
+    for (int qt = 0; qt < nqt; ++qt) {
+      __syncthreads();  // the maxima are there, the V tiles (or the rows before) are done with
+      const int row = 16 * qt + frow;
+      const float m = fmaxf(fmaxf(wave_m[0][row], wave_m[1][row]), fmaxf(wave_m[2][row], wave_m[3][row]));
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wave_m[wave][row] - m);
+      float* os = reinterpret_cast<float*>(sv);
+#pragma unroll
+      for (int q2 = 0; q2 < QT; ++q2)
+        if (q2 == qt)
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            const f32x4_t v = {o[q2][dt][0] * f, o[q2][dt][1] * f, o[q2][dt][2] * f, o[q2][dt][3] * f};
+            *reinterpret_cast<f32x4_t*>(os + frow * HD + ((((4 * dt + g) ^ frow) & (HD / 4 - 1)) << 2)) = v;
+          }
+      __syncthreads();
+      for (int i = tid; i < 16 * (HD / 4); i += kStreamThreads) {
+        const int rr = i / (HD / 4), c = i % (HD / 4), r = r0 + 16 * qt + rr;
+        if (r >= rows) continue;
+        const int wr = 16 * qt + rr;
+        const float mm = fmaxf(fmaxf(wave_m[0][wr], wave_m[1][wr]), fmaxf(wave_m[2][wr], wave_m[3][wr]));
+        float l = 0.f;
+        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float* ow = reinterpret_cast<const float*>(smem + w * C::VBYTES);
+          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(ow + rr * HD + (((c ^ rr) & (HD / 4 - 1)) << 2));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += x[e];
+          l += mm == -INFINITY ? 0.f : wave_l[w][wr] * __builtin_amdgcn_exp2f(wave_m[w][wr] - mm);
+        }
+        const int tok = a.group.div(r), h = hk * G + r - tok * G, t = first + tok;
+        if (whole && a.prefix_len == 0) {
+          const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key, or a NaN that stays one
+          const float out[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+          store4_out(static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh + 4 * c, out);
+        } else {
+          float *ml, *ov;
+          if (whole) {
+            const int64_t at = (prefix ? 0 : static_cast<int64_t>(a.seq.n_tokens) * a.Hq) + static_cast<int64_t>(t) * a.Hq + h;
+            ml = ws.whole_ml + 2 * at;
+            ov = ws.whole_o + HD * at;
+          } else {
+            const int64_t at = static_cast<int64_t>(slot) * R + wr;
+            ml = ws.edge_ml + 2 * at;
+            ov = ws.edge_o + HD * at;
+          }
+          *reinterpret_cast<f32x4_t*>(ov + 4 * c) = v;
+          if (c == 0) {
+            ml[0] = mm;
+            ml[1] = l;
+          }
+        }
+      }
+    }
+    __syncthreads();  // wave_m, wave_l and the tiles are free again
+  }
+  if (bad && a.err != nullptr) *a.err = 1;
+}
+
+// One block a (token, head) row: its partials, each read by HD / 4 lanes, added group
+// by group and then across the groups, always in the same order.  Rows that one block
+// has written whole are left; rows without a key become zeros.
+template <typename T, int HD, int R, int UK>
+__global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units,
+                                                                    int grid) {
+  constexpr int LP = HD / 4, NG = kStreamThreads / LP;
+  __shared__ float gm[NG], gl[NG];
+  __shared__ __attribute__((aligned(16))) float go[NG][HD];
+  const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq;
+  const int G = a.Hq / a.Hkv, hk = h / G;
+  const int b = seq_of(a.seq, t);
+  if (b >= a.seq.B) return;
+  const SeqUnits su = seq_units<R, UK>(a, b);
+  const int U = ws.starts[a.seq.B], g = active_blocks(grid, U);
+  // Runs of partials: blocks [i0, i1] of an item, or one whole row.
+  int i0[2] = {0, 0}, n_part[2] = {0, 0}, wr[2] = {0, 0};
+  const int64_t row = static_cast<int64_t>(t) * a.Hq + h;
+  auto run = [&](int k, int start, int units, int r) {
+    i0[k] = unit_owner(start, U, g);
+    n_part[k] = unit_owner(start + units - 1, U, g) - i0[k] + 1;
+    wr[k] = r;
+  };
+  if (prefix_units > 0) {
+    const int rows = a.seq.n_tokens * G, rts = (rows + R - 1) / R, kt = (a.prefix_len + UK - 1) / UK;
+    const int r = t * G + h - hk * G;
+    run(0, (hk * rts + r / R) * kt, kt, r % R);
+  }
+  if (su.kt > 0) {
+    const int r = (t - su.first) * G + h - hk * G;
+    run(1, ws.starts[b] + (hk * su.rt + r / R) * su.kt, su.kt, r % R);
+  }
+  if (a.prefix_len == 0 && n_part[1] == 1) return;
+  const int lg = threadIdx.x / LP, c = threadIdx.x % LP;
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  const int np = n_part[0] + n_part[1];
+#pragma unroll 4
+  for (int j = lg; j < np; j += NG) {
+    const int k = j < n_part[0] ? 0 : 1, i = j - (k ? n_part[0] : 0);
+    const float *ml, *ov;
+    if (n_part[k] == 1) {
+      const int64_t at = (k ? static_cast<int64_t>(a.seq.n_tokens) * a.Hq : 0) + row;
+      ml = ws.whole_ml + 2 * at;
+      ov = ws.whole_o + HD * at;
+    } else {
+      const int64_t at = static_cast<int64_t>(2 * (i0[k] + i) + (i == 0 ? 1 : 0)) * R + wr[k];
+      ml = ws.edge_ml + 2 * at;
+      ov = ws.edge_o + HD * at;
+    }
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(ov + 4 * c);
+    const float mi = ml[0], li = ml[1], mn = fmaxf(m, mi);
+    const float fo = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    const float fi = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - mn);
+    m = mn;
+    l = l * fo + li * fi;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * fo + x[e] * fi;
+  }
+  if (c == 0) {
+    gm[lg] = m;
+    gl[lg] = l;
+  }
+  *reinterpret_cast<f32x4_t*>(&go[lg][4 * c]) = o;
+  __syncthreads();
+  if (lg != 0) return;
+  const int used = min(NG, np);
+  float mm = -INFINITY;
+  for (int k = 0; k < used; ++k) mm = fmaxf(mm, gm[k]);
+  float lt = 0.f, out[4] = {0.f, 0.f, 0.f, 0.f};
+  if (mm != -INFINITY)
+    for (int k = 0; k < used; ++k) {
+      const float f = __builtin_amdgcn_exp2f(gm[k] - mm);
+      lt += gl[k] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = fmaf(go[k][4 * c + e], f, out[e]);
+    }
+  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] *= inv;
+  store4_out(static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh + 4 * c, out);
+}
+
+// ------------------------------------------------------------------------- host
+
+struct StreamPlan {
+  int grid, prefix_units;
+  int64_t o_starts, o_eml, o_eo, o_wml, o_wo, bytes;
+};
+
+// Grid and workspace of a call: as many blocks as the CUs hold, or one for every unit
+// there can be where that is fewer.
+template <typename T, int HD, int QTW>
+static int plan_stream(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t cap, int64_t prefix_len,
+                       StreamPlan* p) {
+  using C = StreamShape<T, HD, QTW>;
+  const int64_t G = Hq / Hkv, rows = n_tokens * G;
+  const int64_t pu = prefix_len > 0 ? Hkv * ((rows + C::R - 1) / C::R) * ((prefix_len + C::UK - 1) / C::UK) : 0;
+  const int64_t own = Hkv * (rows / C::R + B) * ((cap - (prefix_len & ~int64_t{15}) + C::UK - 1) / C::UK);
+  if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
+  const int64_t per_cu = HD * QTW <= 64 && QTW == 1 ? 4 : 2;
+  p->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pu + own, per_cu * num_cus())));
+  p->prefix_units = static_cast<int>(pu);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += (bytes + 63) / 64 * 64;
+    return o;
+  };
+  p->o_starts = take((B + 1) * 4);
+  p->o_eml = take(int64_t{p->grid} * 2 * C::R * 8);
+  p->o_eo = take(int64_t{p->grid} * 2 * C::R * HD * 4);
+  p->o_wml = take(prefix_len > 0 ? 2 * n_tokens * Hq * 8 : 0);
+  p->o_wo = take(prefix_len > 0 ? 2 * n_tokens * Hq * HD * 4 : 0);
+  p->bytes = at;
+  return CGPT_OK;
+}
+
+template <typename T, int HD, int QTW>
+static int launch_stream(const PagedAttnArgs& a, void* workspace, int64_t ws_bytes, hipStream_t s) {
+  using C = StreamShape<T, HD, QTW>;
+  StreamPlan p;
+  const int rc = plan_stream<T, HD, QTW>(a.seq.n_tokens, a.seq.B, a.Hq, a.Hkv, a.seq.cap, a.prefix_len, &p);
+  if (rc != CGPT_OK) return rc;
+  if (ws_bytes < p.bytes || workspace == nullptr) return CGPT_ESCRATCH;
+  char* w = static_cast<char*>(workspace);
+  const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), reinterpret_cast<float*>(w + p.o_eml),
+                   reinterpret_cast<float*>(w + p.o_eo), reinterpret_cast<float*>(w + p.o_wml),
+                   reinterpret_cast<float*>(w + p.o_wo)};
+  if (a.seq.page.d % 16 == 0)
+    hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, true>), dim3(p.grid), dim3(kStreamThreads), 0, s, a, ws,
+                       p.prefix_units);
+  else
+    hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, false>), dim3(p.grid), dim3(kStreamThreads), 0, s, a, ws,
+                       p.prefix_units);
+  hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK>), dim3(static_cast<unsigned>(a.seq.n_tokens * a.Hq)),
+                     dim3(kStreamThreads), 0, s, a, ws, p.prefix_units, p.grid);
   return hip_status(hipGetLastError());
 }
 
-template <typename T>
-static int launch_paged(int hd, const PagedAttnArgs& a, hipStream_t s) {
-  switch (hd) {
-    case 16: return launch_rows<T, 16>(a, s);
-    case 32: return launch_rows<T, 32>(a, s);
-    case 64: return launch_rows<T, 64>(a, s);
-    case 128: return launch_rows<T, 128>(a, s);
-    default: return CGPT_ESHAPE;
+// Query rows of a tile: 64 where a sequence (or, against a prefix, the batch) has more
+// than 16 rows a key head, 32 at head_dim 128, whose accumulators are twice as wide.
+template <int HD>
+static bool wide_rows(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t prefix_len) {
+  const int64_t rows = n_tokens * (Hq / Hkv);
+  return prefix_len > 0 ? rows > 16 : rows > 16 * B;
+}
+
+template <typename F>
+static int with_stream(int dtype, int hd, F&& f) {
+#define CGPT_PAGED_HD(T)                                                \
+  switch (hd) {                                                         \
+    case 16: return f(T{}, std::integral_constant<int, 16>{});          \
+    case 32: return f(T{}, std::integral_constant<int, 32>{});          \
+    case 64: return f(T{}, std::integral_constant<int, 64>{});          \
+    case 128: return f(T{}, std::integral_constant<int, 128>{});        \
+    default: return CGPT_ESHAPE;                                        \
   }
+  if (dtype == CGPT_BF16) CGPT_PAGED_HD(bf16_t)
+  if (dtype == CGPT_F16) CGPT_PAGED_HD(f16_t)
+  CGPT_PAGED_HD(float)
+#undef CGPT_PAGED_HD
 }
 
 }  // namespace cgpt
@@ -146,13 +792,17 @@ extern "C" int cgpt_shared_prefix_attention(const void* q, const void* k_cache, 
   a.o_sh = o_sh;
   a.Hq = static_cast<int>(Hq);
   a.Hkv = static_cast<int>(Hkv);
+  a.group = FastDiv(Hq / Hkv);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err_flag;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int hd = static_cast<int>(head_dim);
-  if (dtype == CGPT_BF16) return launch_paged<bf16_t>(hd, a, s);
-  if (dtype == CGPT_F16) return launch_paged<f16_t>(hd, a, s);
-  return launch_paged<float>(hd, a, s);
+  return with_stream(dtype, static_cast<int>(head_dim), [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    if (wide_rows<HD>(n_tokens, B, Hq, Hkv, prefix_len))
+      return launch_stream<T, HD, (HD == 128 ? 2 : 4)>(a, workspace, workspace_bytes, s);
+    return launch_stream<T, HD, 1>(a, workspace, workspace_bytes, s);
+  });
 }
 
 extern "C" int cgpt_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -172,7 +822,22 @@ extern "C" int cgpt_paged_attention(const void* q, const void* k_cache, const vo
 extern "C" int cgpt_paged_attention_workspace(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv,
                                               int64_t head_dim, int64_t page_size, int64_t max_pages,
                                               int64_t prefix_len, int dtype, int64_t* workspace_bytes) {
+  using namespace cgpt;
   if (workspace_bytes == nullptr) return CGPT_EINVAL;
   *workspace_bytes = 0;
-  return CGPT_OK;
+  if (n_tokens < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || page_size <= 0 || max_pages < 0 ||
+      prefix_len < 0 || prefix_len > page_size * max_pages)
+    return CGPT_EINVAL;
+  if (dtype != CGPT_F32 && dtype != CGPT_BF16 && dtype != CGPT_F16) return CGPT_EDTYPE;
+  if (n_tokens == 0 || B == 0) return CGPT_OK;
+  return with_stream(dtype, static_cast<int>(head_dim), [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    StreamPlan p;
+    const int rc = wide_rows<HD>(n_tokens, B, Hq, Hkv, prefix_len)
+                       ? plan_stream<T, HD, (HD == 128 ? 2 : 4)>(n_tokens, B, Hq, Hkv, page_size * max_pages, prefix_len, &p)
+                       : plan_stream<T, HD, 1>(n_tokens, B, Hq, Hkv, page_size * max_pages, prefix_len, &p);
+    if (rc == CGPT_OK) *workspace_bytes = p.bytes;
+    return rc;
+  });
 }
