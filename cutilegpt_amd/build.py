@@ -43,6 +43,8 @@ def hipcc() -> str:
 FILE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

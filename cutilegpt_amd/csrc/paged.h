@@ -43,6 +43,29 @@ struct PagedBatch {
   FastDiv page;
 };
 
+struct PagedAttnArgs {
+  const void* q;
+  void* o;
+  PagePool kc, vc;
+  PagedBatch seq;
+  const int* prefix;  // pages of the shared prefix
+  int prefix_len, prefix_cols;
+  int64_t q_st, q_sh, o_st, o_sh;
+  int Hq, Hkv;
+  FastDiv group;  // query heads a key head
+  float scale_log2;
+  int* err;
+};
+
+// Attention of the query tiles of long steps (paged_tile.hip), 16-bit types of head_dim
+// 64 and 128.  flat: rows are all packed tokens, keys the shared prefix; else rows are a
+// sequence's and keys all of its own, those below prefix_len read from the prefix's
+// pages.  qt: 16-row sub-tiles of a wave (1 or 2; 4 waves).  n_split > 1 or flat: every
+// split leaves (m, l, O) of each (token, head) row in part_ml / part_o, else o is written.
+bool paged_tile_ok(int dtype, int head_dim);
+int launch_paged_tile(int dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split,
+                      float* part_ml, float* part_o, hipStream_t s);
+
 // The checks that the entry points share.
 inline int check_paged(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
                        int64_t page_size, int64_t n_pages, int64_t cols, int64_t stride,
@@ -105,6 +128,32 @@ __device__ __forceinline__ int page_of(const int* row, int col, int n_pages, boo
     return 0;
   }
   return p;
+}
+
+// Bit 31 (or, of a 16-bit type, 15) set where a value of the word is not finite: its
+// exponent field, all ones, carries into the sign.
+template <typename T> __device__ __forceinline__ uint32_t special_bits(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return ((w & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+  if constexpr (std::is_same<T, bf16_t>::value) return (w & 0x7f807f80u) + 0x00800080u;
+  return (w & 0x7c007c00u) + 0x04000400u;
+}
+// The word with 0 in the place of values that are not finite.
+template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return special_bits<T>(w) ? 0u : w;
+  const uint32_t bits = special_bits<T>(w);
+  return w & ~(((bits & 0x80000000u) ? 0xffff0000u : 0u) | ((bits & 0x8000u) ? 0xffffu : 0u));
+}
+
+// Half of a V^T operand: the 16-lane group's lane k points at 4 consecutive d of its
+// row and receives the 4 keys of column 16 dt + k.
+template <int KROW, int SWZ>
+__device__ __forceinline__ u32x2_t vt_read(const uint8_t* sv, int row, int dt, int frow) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  const int byte = dt * 32 + 8 * (frow & 3);
+  const uint8_t* p = sv + row * KROW + (((byte >> 4) ^ (row & SWZ)) << 4) + (byte & 15);
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)((__attribute__((address_space(3))) uint8_t*)(p)));
+  return __builtin_bit_cast(u32x2_t, r);
 }
 
 #endif

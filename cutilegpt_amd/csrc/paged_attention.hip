@@ -17,32 +17,6 @@ template <typename T, int CPR> __device__ __forceinline__ int vswz(int key) {
   return ((key >> 2) << 2) & (CPR - 1);
 }
 
-// Half of a V^T operand: the 16-lane group's lane k points at 4 consecutive d of its
-// row and receives the 4 keys of column 16 dt + k.
-template <int KROW, int SWZ>
-__device__ __forceinline__ u32x2_t vt_read(const uint8_t* sv, int row, int dt, int frow) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  const int byte = dt * 32 + 8 * (frow & 3);
-  const uint8_t* p = sv + row * KROW + (((byte >> 4) ^ (row & SWZ)) << 4) + (byte & 15);
-  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) s16x4*)((__attribute__((address_space(3))) uint8_t*)(p)));
-  return __builtin_bit_cast(u32x2_t, r);
-}
-
-struct PagedAttnArgs {
-  const void* q;
-  void* o;
-  PagePool kc, vc;
-  PagedBatch seq;
-  const int* prefix;  // pages of the shared prefix
-  int prefix_len, prefix_cols;
-  int64_t q_st, q_sh, o_st, o_sh;
-  int Hq, Hkv;
-  FastDiv group;  // query heads a key head
-  float scale_log2;
-  int* err;
-};
-
 // ------------------------------------------------------------------ work units
 //
 // The work is a list of items, each one tile of R query rows of one key head against
@@ -96,6 +70,8 @@ struct PagedWs {
   float* edge_o;     // grid x 2 x R x HD
   float* whole_ml;   // {prefix, own} x n_tokens x Hq x {m, l}
   float* whole_o;    // {prefix, own} x n_tokens x Hq x HD
+  float* tile_ml;    // the tile kernel's splits x n_tokens x Hq x {m, l}
+  float* tile_o;     // splits x n_tokens x Hq x HD
 };
 
 template <typename T, int HD, int QTW>
@@ -120,20 +96,6 @@ struct StreamShape {
 };
 
 constexpr int kStreamThreads = 256;
-
-// Bit 31 (or, of a 16-bit type, 15) set where a value of the word is not finite: its
-// exponent field, all ones, carries into the sign.
-template <typename T> __device__ __forceinline__ uint32_t special_bits(uint32_t w) {
-  if constexpr (sizeof(T) == 4) return ((w & 0x7f800000u) + 0x00800000u) & 0x80000000u;
-  if constexpr (std::is_same<T, bf16_t>::value) return (w & 0x7f807f80u) + 0x00800080u;
-  return (w & 0x7c007c00u) + 0x04000400u;
-}
-// The word with 0 in the place of values that are not finite.
-template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
-  if constexpr (sizeof(T) == 4) return special_bits<T>(w) ? 0u : w;
-  const uint32_t bits = special_bits<T>(w);
-  return w & ~(((bits & 0x80000000u) ? 0xffff0000u : 0u) | ((bits & 0x8000u) ? 0xffffu : 0u));
-}
 
 // Each wave streams keys by itself: K and V rows go from their pages into registers,
 // one subtile of KT keys ahead of the one in use, in the layout of the matrix cores' A
@@ -588,7 +550,7 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
 // has written whole are left; rows without a key become zeros.
 template <typename T, int HD, int R, int UK>
 __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units,
-                                                                    int grid) {
+                                                                    int grid, int n_tile) {
   constexpr int LP = HD / 4, NG = kStreamThreads / LP;
   __shared__ float gm[NG], gl[NG];
   __shared__ __attribute__((aligned(16))) float go[NG][HD];
@@ -597,9 +559,10 @@ __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArg
   const int b = seq_of(a.seq, t);
   if (b >= a.seq.B) return;
   const SeqUnits su = seq_units<R, UK>(a, b);
-  const int U = ws.starts[a.seq.B], g = active_blocks(grid, U);
-  // Runs of partials: blocks [i0, i1] of an item, or one whole row.
-  int i0[2] = {0, 0}, n_part[2] = {0, 0}, wr[2] = {0, 0};
+  const int U = grid > 0 ? ws.starts[a.seq.B] : 0, g = active_blocks(grid, U);
+  // Runs of partials: the splits of the tile kernel, or blocks [i0, i1] of an item, or one
+  // whole row.
+  int i0[2] = {0, 0}, n_part[2] = {n_tile, 0}, wr[2] = {0, 0};
   const int64_t row = static_cast<int64_t>(t) * a.Hq + h;
   auto run = [&](int k, int start, int units, int r) {
     i0[k] = unit_owner(start, U, g);
@@ -611,7 +574,7 @@ __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArg
     const int r = t * G + h - hk * G;
     run(0, (hk * rts + r / R) * kt, kt, r % R);
   }
-  if (su.kt > 0) {
+  if (grid > 0 && su.kt > 0) {
     const int r = (t - su.first) * G + h - hk * G;
     run(1, ws.starts[b] + (hk * su.rt + r / R) * su.kt, su.kt, r % R);
   }
@@ -624,7 +587,11 @@ __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArg
   for (int j = lg; j < np; j += NG) {
     const int k = j < n_part[0] ? 0 : 1, i = j - (k ? n_part[0] : 0);
     const float *ml, *ov;
-    if (n_part[k] == 1) {
+    if (k == 0 && n_tile > 0) {
+      const int64_t at = static_cast<int64_t>(i) * a.seq.n_tokens * a.Hq + row;
+      ml = ws.tile_ml + 2 * at;
+      ov = ws.tile_o + HD * at;
+    } else if (n_part[k] == 1) {
       const int64_t at = (k ? static_cast<int64_t>(a.seq.n_tokens) * a.Hq : 0) + row;
       ml = ws.whole_ml + 2 * at;
       ov = ws.whole_o + HD * at;
@@ -660,7 +627,7 @@ __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArg
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[e] = fmaf(go[k][4 * c + e], f, out[e]);
     }
-  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // no key, or a NaN that stays one
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] *= inv;
   store4_out(static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh + 4 * c, out);
@@ -668,67 +635,103 @@ __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArg
 
 // ------------------------------------------------------------------------- host
 
-struct StreamPlan {
-  int grid, prefix_units;
-  int64_t o_starts, o_eml, o_eo, o_wml, o_wo, bytes;
+// What a call runs: the tile kernel on the sequences' rows or on all rows against the
+// prefix, the stream kernel, and the join.  Workspace offsets in bytes.
+struct PagedPlan {
+  bool tile = false, flat = false;  // tile kernel; its rows are the whole batch's
+  int tile_qt = 1, n_split = 1;
+  int stream_qt = 0, grid = 0, prefix_units = 0;  // stream kernel (stream_qt 0: none)
+  int64_t o_starts = 0, o_eml = 0, o_eo = 0, o_wml = 0, o_wo = 0, o_tml = 0, o_to = 0, bytes = 0;
 };
 
-// Grid and workspace of a call: as many blocks as the CUs hold, or one for every unit
-// there can be where that is fewer.
-template <typename T, int HD, int QTW>
-static int plan_stream(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t cap, int64_t prefix_len,
-                       StreamPlan* p) {
-  using C = StreamShape<T, HD, QTW>;
-  const int64_t G = Hq / Hkv, rows = n_tokens * G;
-  const int64_t pu = prefix_len > 0 ? Hkv * ((rows + C::R - 1) / C::R) * ((prefix_len + C::UK - 1) / C::UK) : 0;
-  const int64_t own = Hkv * (rows / C::R + B) * ((cap - (prefix_len & ~int64_t{15}) + C::UK - 1) / C::UK);
-  if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
-  const int64_t per_cu = HD * QTW <= 64 && QTW == 1 ? 4 : 2;
-  p->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pu + own, per_cu * num_cus())));
-  p->prefix_units = static_cast<int>(pu);
-  int64_t at = 0;
+template <typename T, int HD>
+static int make_plan(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t cap, int64_t prefix_len, int dtype,
+                     PagedPlan* p) {
+  const int64_t G = Hq / Hkv, rows = n_tokens * G, cus = num_cus();
   auto take = [&](int64_t bytes) {
-    const int64_t o = at;
-    at += (bytes + 63) / 64 * 64;
+    const int64_t o = p->bytes;
+    p->bytes += (bytes + 63) / 64 * 64;
     return o;
   };
-  p->o_starts = take((B + 1) * 4);
-  p->o_eml = take(int64_t{p->grid} * 2 * C::R * 8);
-  p->o_eo = take(int64_t{p->grid} * 2 * C::R * HD * 4);
-  p->o_wml = take(prefix_len > 0 ? 2 * n_tokens * Hq * 8 : 0);
-  p->o_wo = take(prefix_len > 0 ? 2 * n_tokens * Hq * HD * 4 : 0);
-  p->bytes = at;
+  const bool tile_ok = paged_tile_ok(dtype, HD);
+  p->flat = tile_ok && prefix_len > 0 && rows > 64 && rows <= 16 * B;
+  p->tile = p->flat || (tile_ok && rows > 16 * B);
+  if (p->tile) {
+    // 128-row tiles where they fill the card, else 64; then the keys split until the card
+    // is full, 256 keys a split at least.
+    const int64_t keys = p->flat ? prefix_len : cap;
+    auto blocks = [&](int64_t bq) { return Hkv * (p->flat ? (rows + bq - 1) / bq : rows / bq + B); };
+    p->tile_qt = blocks(128) >= 4 * cus || (p->flat && rows > 64) ? 2 : 1;
+    const int64_t n = blocks(64 * p->tile_qt);
+    p->n_split = static_cast<int>(std::max<int64_t>(1, std::min((3 * cus + n - 1) / n, keys / 256)));
+    if (!p->flat && n >= 2 * cus) p->n_split = 1;
+    if (n * p->n_split > 0x7fffffff) return CGPT_ESHAPE;
+    const bool parts = p->flat || p->n_split > 1;
+    p->o_tml = take(parts ? p->n_split * n_tokens * Hq * 8 : 0);
+    p->o_to = take(parts ? p->n_split * n_tokens * Hq * HD * 4 : 0);
+  }
+  if (!p->tile || p->flat) {
+    // 64-row tiles (32 at head_dim 128, whose accumulators are twice as wide) where a
+    // sequence, or the batch against its prefix, has more than 16 rows a key head.
+    const bool wide = !p->flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
+    p->stream_qt = wide ? (HD == 128 ? 2 : 4) : 1;
+    const int64_t R = 16 * p->stream_qt, UK = StreamShape<T, HD, 1>::UK;
+    const int64_t pu = prefix_len > 0 && !p->flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + UK - 1) / UK) : 0;
+    const int64_t own = Hkv * (rows / R + B) * ((cap - (prefix_len & ~int64_t{15}) + UK - 1) / UK);
+    if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
+    const int64_t per_cu = HD <= 64 && p->stream_qt == 1 ? 4 : 2;
+    p->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pu + own, per_cu * cus)));
+    p->prefix_units = static_cast<int>(pu);
+    p->o_starts = take((B + 1) * 4);
+    p->o_eml = take(int64_t{p->grid} * 2 * R * 8);
+    p->o_eo = take(int64_t{p->grid} * 2 * R * HD * 4);
+    p->o_wml = take(prefix_len > 0 ? 2 * n_tokens * Hq * 8 : 0);
+    p->o_wo = take(prefix_len > 0 ? 2 * n_tokens * Hq * HD * 4 : 0);
+  }
   return CGPT_OK;
 }
 
 template <typename T, int HD, int QTW>
-static int launch_stream(const PagedAttnArgs& a, void* workspace, int64_t ws_bytes, hipStream_t s) {
-  using C = StreamShape<T, HD, QTW>;
-  StreamPlan p;
-  const int rc = plan_stream<T, HD, QTW>(a.seq.n_tokens, a.seq.B, a.Hq, a.Hkv, a.seq.cap, a.prefix_len, &p);
-  if (rc != CGPT_OK) return rc;
-  if (ws_bytes < p.bytes || workspace == nullptr) return CGPT_ESCRATCH;
-  char* w = static_cast<char*>(workspace);
-  const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), reinterpret_cast<float*>(w + p.o_eml),
-                   reinterpret_cast<float*>(w + p.o_eo), reinterpret_cast<float*>(w + p.o_wml),
-                   reinterpret_cast<float*>(w + p.o_wo)};
+static void launch_stream(const PagedAttnArgs& a, const PagedWs& ws, const PagedPlan& p, hipStream_t s) {
   if (a.seq.page.d % 16 == 0)
     hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, true>), dim3(p.grid), dim3(kStreamThreads), 0, s, a, ws,
                        p.prefix_units);
   else
     hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, false>), dim3(p.grid), dim3(kStreamThreads), 0, s, a, ws,
                        p.prefix_units);
-  hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK>), dim3(static_cast<unsigned>(a.seq.n_tokens * a.Hq)),
-                     dim3(kStreamThreads), 0, s, a, ws, p.prefix_units, p.grid);
-  return hip_status(hipGetLastError());
 }
 
-// Query rows of a tile: 64 where a sequence (or, against a prefix, the batch) has more
-// than 16 rows a key head, 32 at head_dim 128, whose accumulators are twice as wide.
-template <int HD>
-static bool wide_rows(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t prefix_len) {
-  const int64_t rows = n_tokens * (Hq / Hkv);
-  return prefix_len > 0 ? rows > 16 : rows > 16 * B;
+template <typename T, int HD, int QTW>
+static void launch_join(const PagedAttnArgs& a, const PagedWs& ws, const PagedPlan& p, hipStream_t s) {
+  using C = StreamShape<T, HD, QTW>;
+  hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK>), dim3(static_cast<unsigned>(a.seq.n_tokens * a.Hq)),
+                     dim3(kStreamThreads), 0, s, a, ws, p.prefix_units, p.grid,
+                     p.flat || p.n_split > 1 ? p.n_split : 0);
+}
+
+template <typename T, int HD>
+static int run_plan(const PagedAttnArgs& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t s) {
+  PagedPlan p;
+  int rc = make_plan<T, HD>(a.seq.n_tokens, a.seq.B, a.Hq, a.Hkv, a.seq.cap, a.prefix_len, dtype, &p);
+  if (rc != CGPT_OK) return rc;
+  if (p.bytes > 0 && (ws_bytes < p.bytes || workspace == nullptr)) return CGPT_ESCRATCH;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return CGPT_EINVAL;
+  char* w = static_cast<char*>(workspace);
+  auto f32 = [&](int64_t o) { return reinterpret_cast<float*>(w + o); };
+  const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), f32(p.o_eml), f32(p.o_eo), f32(p.o_wml), f32(p.o_wo),
+                   f32(p.o_tml), f32(p.o_to)};
+  constexpr int WIDE = HD == 128 ? 2 : 4;
+  if (p.tile) {
+    rc = launch_paged_tile(dtype, HD, a, p.flat, p.tile_qt, p.n_split, ws.tile_ml, ws.tile_o, s);
+    if (rc != CGPT_OK) return rc;
+  }
+  if (p.stream_qt == 1) launch_stream<T, HD, 1>(a, ws, p, s);
+  if (p.stream_qt > 1) launch_stream<T, HD, WIDE>(a, ws, p, s);
+  if (p.stream_qt > 1)
+    launch_join<T, HD, WIDE>(a, ws, p, s);
+  else if (p.stream_qt == 1 || p.n_split > 1)
+    launch_join<T, HD, 1>(a, ws, p, s);
+  return hip_status(hipGetLastError());
 }
 
 template <typename F>
@@ -799,9 +802,7 @@ extern "C" int cgpt_shared_prefix_attention(const void* q, const void* k_cache, 
   return with_stream(dtype, static_cast<int>(head_dim), [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    if (wide_rows<HD>(n_tokens, B, Hq, Hkv, prefix_len))
-      return launch_stream<T, HD, (HD == 128 ? 2 : 4)>(a, workspace, workspace_bytes, s);
-    return launch_stream<T, HD, 1>(a, workspace, workspace_bytes, s);
+    return run_plan<T, HD>(a, dtype, workspace, workspace_bytes, s);
   });
 }
 
@@ -833,10 +834,8 @@ extern "C" int cgpt_paged_attention_workspace(int64_t n_tokens, int64_t B, int64
   return with_stream(dtype, static_cast<int>(head_dim), [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    StreamPlan p;
-    const int rc = wide_rows<HD>(n_tokens, B, Hq, Hkv, prefix_len)
-                       ? plan_stream<T, HD, (HD == 128 ? 2 : 4)>(n_tokens, B, Hq, Hkv, page_size * max_pages, prefix_len, &p)
-                       : plan_stream<T, HD, 1>(n_tokens, B, Hq, Hkv, page_size * max_pages, prefix_len, &p);
+    PagedPlan p;
+    const int rc = make_plan<T, HD>(n_tokens, B, Hq, Hkv, page_size * max_pages, prefix_len, dtype, &p);
     if (rc == CGPT_OK) *workspace_bytes = p.bytes;
     return rc;
   });

@@ -1,0 +1,395 @@
+// Attention over the paged cache for tiles of many query rows: prompts taken in
+// chunks, and all sequences of a batch against their shared prefix.
+//
+// A block is 4 waves of QT x 16 query rows of one key head (with grouped heads the
+// rows are token-major, the group's heads side by side, so a key row is read once for
+// all of them); keys come 64 at a time, K and V straight from their pages into LDS by
+// direct-to-LDS loads with an address a lane, the next 64 in flight while these are
+// used.  The page ids are read one block of keys ahead of the loads that need them.
+// S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs as in cgpt_attention_fwd's kernel: a
+// lane owns one query row, P goes from the accumulators straight into the second
+// product, V is transposed by the LDS read.
+#include "internal.h"
+#include "paged.h"
+
+namespace cgpt {
+
+constexpr int kTileThreads = 256, kTileKeys = 64;
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// 16 bytes a lane from its own address to LDS: lane l's land at M0 + 16 l.  Not counted
+// by the compiler (see dma_lds16).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma_lds16_at(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+#endif
+
+template <typename T, int HD, int QTW, bool FLAT>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, 4))) void
+paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, int n_tiles) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  static_assert(sizeof(T) == 2 && (HD == 64 || HD == 128), "16-bit types, head_dim 64 or 128");
+  constexpr int QT = QTW, BQ = 64 * QTW, BKV = kTileKeys, NWAVE = 4;
+  constexpr int KROW = HD * 2, CPR = KROW / 16, RPI = 64 / CPR;  // bytes, chunks of a row; rows of a 1 KiB load
+  constexpr int XB = BKV * KROW, STAGE = 2 * XB;
+  constexpr int INS = XB / 1024 / NWAVE;                         // loads a wave makes of K (and of V) a block
+  constexpr int NKS = HD / 32, ND = HD / 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, frow = lane & 15;
+  const int G = a.Hq / a.Hkv, page_size = static_cast<int>(a.seq.page.d);
+
+  // Key heads are the fastest index (blocks of one head on one XCD where their number
+  // allows), the last row tiles, which see most keys, start first.
+  int idx = blockIdx.x;
+  const int hk = idx % a.Hkv;
+  idx /= a.Hkv;
+  const int split = idx % n_split, tile = n_tiles - 1 - idx / n_split;
+
+  // ---- rows
+  int r0, rows, first = 0, pos0 = 0, n;
+  const int* trow = nullptr;
+  bool bad = false;
+  if (FLAT) {
+    r0 = tile * BQ;
+    rows = a.seq.n_tokens * G;
+    n = a.prefix_len;
+  } else {
+    // Sequence b has the tiles from start(b) = cu[b] G / BQ + b on, at least as many as its
+    // rows fill.
+    int b = 0;
+    for (int c = 0; c < a.seq.B; c += 64) {
+      const int bb = c + lane + 1;
+      int at = bb;
+      if (a.seq.cu != nullptr && bb <= a.seq.B) at = min(max(a.seq.cu[bb], 0), a.seq.n_tokens);
+      const bool below = bb <= a.seq.B && at * G / BQ + bb <= tile;
+      const int k = __popcll(__builtin_amdgcn_ballot_w64(below));
+      b += k;
+      if (k < 64) break;
+    }
+    if (b >= a.seq.B) return;
+    int count;
+    seq_tokens(a.seq, b, &first, &count);
+    rows = count * G;
+    r0 = (tile - (first * G / BQ + b)) * BQ;
+    if (r0 < 0 || r0 >= rows) return;
+    const int len = max(a.seq.lens[b], 0);
+    bad = len > a.seq.cap;
+    pos0 = len - count;
+    n = min(min(len, a.seq.cap), max(pos0 + a.group.div(min(r0 + BQ, rows) - 1) + 1, 0));
+    trow = a.seq.table + b * a.seq.stride;
+  }
+  const int wr0 = r0 + wave * 16 * QT;
+  const bool wave_live = wr0 < rows;
+
+  // ---- keys of this split, in blocks of 64
+  const int n_kv = (n + BKV - 1) / BKV, per = (n_kv + n_split - 1) / n_split;
+  const int j0 = split * per, j1 = min(j0 + per, n_kv);
+
+  const int lrow = lane / CPR, slot16 = lane % CPR;
+  const uint8_t* const kh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.kc.base) + hk * a.kc.sh);
+  const uint8_t* const vh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.vc.base) + hk * a.vc.sh);
+  int pg[INS];
+  auto key_of = [&](int j, int ii) __attribute__((always_inline)) {
+    return min(j * BKV + (ii * NWAVE + wave) * RPI + lrow, n - 1);
+  };
+  auto fetch = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ii = 0; ii < INS; ++ii) {
+      const int key = key_of(j, ii);
+      pg[ii] = (FLAT || key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
+    }
+  };
+  auto issue = [&](int j, uint8_t* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ii = 0; ii < INS; ++ii) {
+      const int row = (ii * NWAVE + wave) * RPI + lrow, key = key_of(j, ii);
+      const int slot = key - a.seq.page.div(key) * page_size;
+      int p = pg[ii];
+      if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) {
+        p = 0;
+        bad = true;
+      }
+      const int chunk = (slot16 ^ (row & 7)) << 4;
+      const uint32_t lds = (ii * NWAVE + wave) * 1024;
+      dma_lds16_at(kh + 2 * (p * a.kc.sp + slot * a.kc.ss) + chunk, lds_addr(buf + lds));
+      dma_lds16_at(vh + 2 * (p * a.vc.sp + slot * a.vc.ss) + chunk, lds_addr(buf + XB + lds));
+    }
+  };
+
+  if (j0 < j1) {
+    fetch(j0);
+    issue(j0, smem);
+    fetch(min(j0 + 1, j1 - 1));
+  }
+
+  u32x4_t qf[QT][NKS];
+  int lim[QT];  // last key the row sees; rows that do not exist are never masked
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int r = wr0 + 16 * qt + frow;
+    const bool live = r < rows;
+    const int i = a.group.div(live ? r : 0), h = hk * G + (live ? r : 0) - i * G, t = first + i;
+    if (FLAT) {
+      const int b = seq_of(a.seq, t);
+      lim[qt] = -1;
+      if (b < a.seq.B) {
+        int f, c;
+        seq_tokens(a.seq, b, &f, &c);
+        lim[qt] = min(a.seq.lens[b] - c + (t - f), n - 1);
+      }
+    } else {
+      lim[qt] = min(pos0 + i, n - 1);
+    }
+    if (!live) lim[qt] = 0x7fffffff;
+    const T* qp = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + (4 * ks + g) * 8);
+      qf[qt][ks] = live ? v : u32x4_t{0, 0, 0, 0};
+    }
+  }
+  // nm = minus the running maximum of a row's scaled scores, +inf while it has none.
+  f32x4_t o[QT][ND];
+  float nm[QT], l_run[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    nm[qt] = INFINITY;
+    l_run[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) o[qt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // The last key that any row of the wave sees.
+  int wave_last;
+  if (FLAT) {
+    wave_last = n - 1;
+  } else {
+    wave_last = pos0 + a.group.div(min(wr0 + 16 * QT, rows) - 1);
+  }
+  wait_vmcnt<0>();
+
+  const int tr_row = 4 * g + (frow >> 2);
+  for (int j = j0; j < j1; ++j) {
+    raw_barrier();
+    const uint8_t* sk = smem + ((j - j0) & 1) * STAGE;
+    const uint8_t* sv = sk + XB;
+    if (j + 1 < j1) {
+      issue(j + 1, smem + ((j - j0 + 1) & 1) * STAGE);
+      fetch(min(j + 2, j1 - 1));
+    }
+    const int base = j * BKV;
+    if (wave_live && base <= wave_last) {
+      f32x4_t s[QT][4];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) s[qt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const int key = kt * 16 + frow, c = 4 * ks + g;
+          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ (key & 7)) << 4));
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(kf, qf[qt][ks], s[qt][kt]);
+        }
+      bool masked = false;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+        if (__builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0) {
+          masked = true;
+          const int hi = lim[qt] - base - 4 * g;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[qt][kt][r] = 16 * kt + r > hi ? -INFINITY : s[qt][kt][r];
+        }
+      // P against the running maximum as it stands.  A lane whose 16 values sum to at most
+      // 2^7 has none above it, so its maximum need not move; only when some lane fails that
+      // (a NaN sum fails it, and a row without a maximum) is the block's maximum taken and,
+      // where it outgrows the running one by more than 8, the row rescaled and its P
+      // made again.
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        float p[4][4], sum = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][kt][r], a.scale_log2, nm[qt]));
+            sum += p[kt][r];
+          }
+        if (__builtin_amdgcn_ballot_w64(sum <= 128.0f) != __builtin_amdgcn_read_exec()) {
+          const float m_old = -nm[qt];
+          float mx = -INFINITY;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[qt][kt][r]);
+          mx = column_max(mx) * a.scale_log2;
+          const bool grow = mx > m_old + 8.0f;
+          const float m_new = grow ? mx : m_old;
+          const float alpha = grow ? __builtin_amdgcn_exp2f(m_old - m_new) : 1.0f;
+          nm[qt] = m_new == -INFINITY ? INFINITY : -m_new;
+          l_run[qt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[qt][dt][r] *= alpha;
+          // A row that has seen no key yet: its scores are all -inf and its P 0.
+          const float shift = m_new == -INFINITY ? 0.f : -m_new;
+          sum = 0.f;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              p[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][kt][r], a.scale_log2, shift));
+              sum += p[kt][r];
+            }
+        }
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[qt][kt][r] = p[kt][r];
+        l_run[qt] += sum;
+      }
+      // Values that are not finite at keys some row does not see (0 x NaN is NaN): added
+      // here, key by key, to the rows that see them, and taken out of the operand below.
+      bool odd = false;
+      if (masked) {
+        uint64_t keys = 0;
+#pragma unroll 1
+        for (int k8 = 0; k8 < BKV; k8 += RPI) {
+          const u32x4_t v = *reinterpret_cast<const u32x4_t*>(sv + (k8 + lrow) * KROW + (slot16 << 4));
+          const uint32_t bits = special_bits<T>(v[0]) | special_bits<T>(v[1]) | special_bits<T>(v[2]) | special_bits<T>(v[3]);
+          const uint64_t m = __builtin_amdgcn_ballot_w64((bits & 0x80008000u) != 0);
+          for (int k = 0; k < RPI; ++k)
+            if ((m >> (k * CPR)) & ((uint64_t{1} << CPR) - 1)) keys |= uint64_t{1} << (k8 + k);
+        }
+        odd = keys != 0;
+        if (__builtin_expect(odd, 0)) {
+#pragma unroll 1
+          for (int k = 0; k < BKV; ++k) {
+            if (!((keys >> k) & 1)) continue;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              float p = 0.f;
+#pragma unroll
+              for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p = kt == k >> 4 && r == (k & 3) ? s[qt][kt][r] : p;
+              p = __shfl(p, (k & 12) * 4 + frow, 64);
+              const bool seen = base + k <= lim[qt];
+#pragma unroll
+              for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int d = 16 * dt + 4 * g + e;
+                  const float v = Elem<T>::load(
+                      reinterpret_cast<const T*>(sv + k * KROW + (((d >> 3) ^ (k & 7)) << 4)) + (d & 7));
+                  if (seen && !(fabsf(v) < INFINITY)) o[qt][dt][e] = fmaf(p, v, o[qt][dt][e]);
+                }
+            }
+          }
+        }
+      }
+      auto pv = [&](auto clean) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          u32x4_t pf[QT];
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            pf[qt] = u32x4_t{pack2<T>(s[qt][2 * c][0], s[qt][2 * c][1]), pack2<T>(s[qt][2 * c][2], s[qt][2 * c][3]),
+                             pack2<T>(s[qt][2 * c + 1][0], s[qt][2 * c + 1][1]),
+                             pack2<T>(s[qt][2 * c + 1][2], s[qt][2 * c + 1][3])};
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            const u32x2_t lo = vt_read<KROW, 7>(sv, 32 * c + tr_row, dt, frow);
+            const u32x2_t hi = vt_read<KROW, 7>(sv, 32 * c + 16 + tr_row, dt, frow);
+            u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
+            if constexpr (decltype(clean)::value)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = finite_part<T>(w[e]);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(w, pf[qt], o[qt][dt]);
+          }
+        }
+      };
+      if (__builtin_expect(odd, 0))
+        pv(std::true_type{});
+      else
+        pv(std::false_type{});
+    }
+    if (j + 1 < j1) wait_vmcnt<0>();
+  }
+
+  // ---- out: lane holds O[row][16 dt + 4 g .. +3]
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float l = column_sum(l_run[qt]);
+    const int r = wr0 + 16 * qt + frow;
+    if (r >= rows) continue;
+    const int i = a.group.div(r), h = hk * G + r - i * G, t = first + i;
+    if (!FLAT && n_split == 1) {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key, or a NaN that stays one
+      T* orow = static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+        const float v[4] = {o[qt][dt][0] * inv, o[qt][dt][1] * inv, o[qt][dt][2] * inv, o[qt][dt][3] * inv};
+        store4_out(orow + 16 * dt + 4 * g, v);
+      }
+    } else {
+      const int64_t at = (static_cast<int64_t>(split) * a.seq.n_tokens + t) * a.Hq + h;
+      if (g == 0) {
+        part_ml[2 * at] = -nm[qt];
+        part_ml[2 * at + 1] = l;
+      }
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * HD + 16 * dt + 4 * g) = o[qt][dt];
+    }
+  }
+  if (bad && a.err != nullptr) *a.err = 1;
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
+bool paged_tile_ok(int dtype, int head_dim) {
+  return dtype != CGPT_F32 && (head_dim == 64 || head_dim == 128);
+}
+
+template <typename T, int HD, int QTW>
+static int launch_tile(const PagedAttnArgs& a, bool flat, int n_split, float* part_ml, float* part_o, hipStream_t s) {
+  constexpr int BQ = 64 * QTW;
+  const int64_t rows = static_cast<int64_t>(a.seq.n_tokens) * (a.Hq / a.Hkv);
+  const int64_t tiles = flat ? (rows + BQ - 1) / BQ : rows / BQ + a.seq.B;
+  const int64_t blocks = tiles * n_split * a.Hkv;
+  if (blocks > 0x7fffffff) return CGPT_ESHAPE;
+  if (flat)
+    hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, true>), dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0,
+                       s, a, part_ml, part_o, n_split, static_cast<int>(tiles));
+  else
+    hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, false>), dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0,
+                       s, a, part_ml, part_o, n_split, static_cast<int>(tiles));
+  return hip_status(hipGetLastError());
+}
+
+template <typename T, int HD>
+static int launch_tile_qt(const PagedAttnArgs& a, bool flat, int qt, int n_split, float* part_ml, float* part_o,
+                          hipStream_t s) {
+  return qt == 2 ? launch_tile<T, HD, 2>(a, flat, n_split, part_ml, part_o, s)
+                 : launch_tile<T, HD, 1>(a, flat, n_split, part_ml, part_o, s);
+}
+
+int launch_paged_tile(int dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split, float* part_ml,
+                      float* part_o, hipStream_t s) {
+  if (dtype == CGPT_BF16 && head_dim == 64) return launch_tile_qt<bf16_t, 64>(a, flat, qt, n_split, part_ml, part_o, s);
+  if (dtype == CGPT_BF16 && head_dim == 128) return launch_tile_qt<bf16_t, 128>(a, flat, qt, n_split, part_ml, part_o, s);
+  if (dtype == CGPT_F16 && head_dim == 64) return launch_tile_qt<f16_t, 64>(a, flat, qt, n_split, part_ml, part_o, s);
+  if (dtype == CGPT_F16 && head_dim == 128) return launch_tile_qt<f16_t, 128>(a, flat, qt, n_split, part_ml, part_o, s);
+  return CGPT_EDTYPE;
+}
+
+}  // namespace cgpt
