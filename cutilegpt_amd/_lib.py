@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch  # noqa: F401  (must be loaded first, see module docstring)
@@ -72,13 +73,21 @@ SIGNATURES = {
                            _I64, _I64, _I64, _I64, _I64, _I64, _I, _P]),
     "cgpt_forward": (_I, [_P, _I64, _P, _F, _F, _P, _P, _P]),
     "cgpt_argmax": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I64, _P, _P]),
-    "cgpt_paged_kv_append": (_I, [_P] * 10 + [_I64] * 26 + [_I, _I, _P, _P]),
-    "cgpt_paged_attention": (_I, [_P] * 7 + [_I64] * 19 + [_F, _P, _I64, _I, _P, _P]),
-    "cgpt_shared_prefix_attention": (_I, [_P] * 8 + [_I64] * 20 + [_F, _P, _I64, _I, _P, _P]),
-    "cgpt_paged_attention_workspace": (_I, [_I64] * 8 + [_I, _P]),
+    "cgpt_paged_kv_append": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_paged_attention": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_paged_attention_workspace": (_I, [ctypes.c_char_p, _P]),
     "cgpt_partials_bias_act": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I64, _I, _I,
                                     _P]),
 }
+
+# cgpt_paged_args, field by field (eight bytes each): struct.pack gives the bytes that
+# the paged entry points take, at a tenth of what converting as many arguments costs.
+PAGED_FIELDS = ("q", "k", "v", "out", "k_cache", "v_cache", "block_table", "seq_lens", "cu_q", "prefix_pages",
+                "rotary", "workspace", "err_flag", "workspace_bytes", "n_tokens", "B", "Hq", "Hkv", "head_dim",
+                "n_pages", "page_size", "max_pages", "bt_stride", "prefix_len", "q_st", "q_sh", "k_st", "k_sh",
+                "v_st", "v_sh", "out_st", "out_sh", "kc_sp", "kc_sh", "kc_ss", "vc_sp", "vc_sh", "vc_ss", "rot_dim",
+                "n_pos", "rot_stride", "interleaved", "dtype", "scale")
+paged_args = struct.Struct(f"{len(PAGED_FIELDS) - 1}qd").pack
 
 ABI_VERSION = 1
 

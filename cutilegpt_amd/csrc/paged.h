@@ -38,7 +38,7 @@ struct PagedBatch {
   const int* lens;
   const int* cu;
   int64_t stride;
-  int n_tokens, B, n_pages, cols;
+  int n_tokens, B, n_pages;
   int cap;  // keys a table row can name
   FastDiv page;
 };
@@ -49,7 +49,7 @@ struct PagedAttnArgs {
   PagePool kc, vc;
   PagedBatch seq;
   const int* prefix;  // pages of the shared prefix
-  int prefix_len, prefix_cols;
+  int prefix_len;
   int64_t q_st, q_sh, o_st, o_sh;
   int Hq, Hkv;
   FastDiv group;  // query heads a key head
@@ -62,33 +62,50 @@ struct PagedAttnArgs {
 // sequence's and keys all of its own, those below prefix_len read from the prefix's
 // pages.  qt: 16-row sub-tiles of a wave (1 or 2; 4 waves).  n_split > 1 or flat: every
 // split leaves (m, l, O) of each (token, head) row in part_ml / part_o, else o is written.
-bool paged_tile_ok(int dtype, int head_dim);
-int launch_paged_tile(int dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split,
+bool paged_tile_ok(int64_t dtype, int head_dim);
+int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split,
                       float* part_ml, float* part_o, hipStream_t s);
 
-// The checks that the entry points share.
-inline int check_paged(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
-                       int64_t page_size, int64_t n_pages, int64_t cols, int64_t stride,
-                       const PagePool& k, const PagePool& v, int dtype) {
-  if (n_tokens < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || page_size <= 0 || n_pages <= 0 || cols < 0)
+// The checks that the entry points share: the sizes, then (with tokens to work on) the
+// pointers.  CGPT_OK with *empty when there is nothing to launch.
+inline int check_paged(const cgpt_paged_args* p, bool* empty) {
+  if (p == nullptr) return CGPT_EINVAL;
+  const cgpt_paged_args& a = *p;
+  if (a.n_tokens < 0 || a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.page_size <= 0 || a.n_pages <= 0 || a.max_pages < 0)
     return CGPT_EINVAL;
-  if (Hq % Hkv != 0 || (cols > 0 && B > 1 && stride < 0)) return CGPT_EINVAL;
-  if (dtype != CGPT_F32 && dtype != CGPT_BF16 && dtype != CGPT_F16) return CGPT_EDTYPE;
-  if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128) return CGPT_ESHAPE;
-  if (n_tokens > 0x3fffffff || B > 0x3fffffff || Hq > 0x7fff || page_size > 0x3fffffff ||
-      n_pages > 0x7fffffff || cols > 0x3fffffff || n_tokens * Hq > 0x7fffffff)
+  if (a.Hq % a.Hkv != 0 || a.bt_stride < 0) return CGPT_EINVAL;
+  if (a.dtype != CGPT_F32 && a.dtype != CGPT_BF16 && a.dtype != CGPT_F16) return CGPT_EDTYPE;
+  if (a.head_dim != 16 && a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 128) return CGPT_ESHAPE;
+  if (a.n_tokens > 0x3fffffff || a.B > 0x3fffffff || a.Hq > 0x7fff || a.page_size > 0x3fffffff ||
+      a.n_pages > 0x7fffffff || a.max_pages > 0x3fffffff || a.n_tokens * a.Hq > 0x7fffffff ||
+      a.page_size * a.max_pages > 0x3fffffff)
     return CGPT_ESHAPE;
-  if (page_size * cols > 0x3fffffff) return CGPT_ESHAPE;
-  const int64_t epv = dtype == CGPT_F32 ? 4 : 8;
-  for (const PagePool* p : {&k, &v}) {
-    if (p->base == nullptr || (reinterpret_cast<uintptr_t>(p->base) & 15)) return CGPT_EINVAL;
-    // Rows are read and written as 16-byte vectors; no two may overlap.
-    if (p->sp % epv != 0 || p->sh % epv != 0 || p->ss % epv != 0) return CGPT_EINVAL;
-    if ((n_pages > 1 && p->sp < head_dim) || (Hkv > 1 && p->sh < head_dim) ||
-        (page_size > 1 && p->ss < head_dim))
-      return CGPT_EINVAL;
+  // Rows are read and written as 16-byte vectors; no two of a pool may overlap.
+  const int64_t epv = a.dtype == CGPT_F32 ? 4 : 8;
+  const int64_t pools[2][3] = {{a.kc_sp, a.kc_sh, a.kc_ss}, {a.vc_sp, a.vc_sh, a.vc_ss}};
+  const void* bases[2] = {a.k_cache, a.v_cache};
+  for (int i = 0; i < 2; ++i) {
+    const int64_t *s = pools[i], hd = a.head_dim;
+    if (bases[i] == nullptr || (reinterpret_cast<uintptr_t>(bases[i]) & 15)) return CGPT_EINVAL;
+    if (s[0] % epv != 0 || s[1] % epv != 0 || s[2] % epv != 0) return CGPT_EINVAL;
+    if ((a.n_pages > 1 && s[0] < hd) || (a.Hkv > 1 && s[1] < hd) || (a.page_size > 1 && s[2] < hd)) return CGPT_EINVAL;
   }
+  *empty = a.n_tokens == 0 || a.B == 0;
+  if (*empty) return CGPT_OK;
+  if (a.seq_lens == nullptr || (a.max_pages > 0 && a.block_table == nullptr)) return CGPT_EINVAL;
+  if (a.cu_q == nullptr && a.n_tokens != a.B) return CGPT_EINVAL;
+  for (int64_t st : {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh, a.out_st, a.out_sh})
+    if (st < 0 || st % epv != 0) return CGPT_EINVAL;
+  for (const void* r : {a.q, a.k, a.v, static_cast<const void*>(a.out)})
+    if (reinterpret_cast<uintptr_t>(r) & 15) return CGPT_EINVAL;
+  if (a.out != nullptr && ((a.Hq > 1 && a.out_sh < a.head_dim) || (a.n_tokens > 1 && a.out_st < a.head_dim)))
+    return CGPT_EINVAL;
   return CGPT_OK;
+}
+
+inline PagedBatch paged_batch(const cgpt_paged_args& a) {
+  return PagedBatch{a.block_table, a.seq_lens, a.cu_q, a.bt_stride, static_cast<int>(a.n_tokens), static_cast<int>(a.B),
+                    static_cast<int>(a.n_pages), static_cast<int>(a.page_size * a.max_pages), FastDiv(a.page_size)};
 }
 
 #if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
@@ -118,6 +135,29 @@ __device__ __forceinline__ int seq_of(const PagedBatch& s, int t) {
       lo = mid + 1;
   }
   return lo;
+}
+
+// Row tiles of R rows over sequences of any numbers of tokens: sequence b has the slots
+// from start(b) = cu[b] G / R + b on, at least as many as its rows fill.  The sequence
+// of slot *slot, which becomes its tile within the sequence (possibly behind its rows);
+// B when there is none.
+template <int R>
+__device__ __forceinline__ int slot_seq(const PagedBatch& s, int G, int lane, int* slot) {
+  if (s.cu == nullptr && G <= R) {  // one tile each
+    const int b = *slot;
+    *slot = 0;
+    return b;
+  }
+  int b = 0;
+  for (int c = 0; c < s.B; c += 64) {
+    const int bb = c + lane + 1;
+    const int at = s.cu == nullptr || bb > s.B ? bb : min(max(s.cu[bb], 0), s.n_tokens);
+    const int k = __popcll(__builtin_amdgcn_ballot_w64(bb <= s.B && at * G / R + bb <= *slot));
+    b += k;
+    if (k < 64) break;
+  }
+  if (b < s.B) *slot -= (s.cu == nullptr ? b : min(max(s.cu[b], 0), s.n_tokens)) * G / R + b;
+  return b;
 }
 
 // Page of key t of the table row, clamped into the pool; *bad when it was not.

@@ -89,62 +89,26 @@ static int launch_append(const AppendArgs& a, hipStream_t s) {
 
 }  // namespace cgpt
 
-extern "C" int cgpt_paged_kv_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
-                                    void* v_cache, const int* block_table, const int* seq_lens,
-                                    const int* cu_q, const float* rotary, int64_t n_tokens, int64_t B,
-                                    int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t page_size,
-                                    int64_t n_pages, int64_t max_pages, int64_t bt_stride, int64_t q_st,
-                                    int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
-                                    int64_t qo_st, int64_t qo_sh, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
-                                    int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, int64_t rot_dim,
-                                    int64_t n_pos, int64_t rot_stride, int interleaved, int dtype,
-                                    int* err_flag, void* stream) {
+extern "C" int cgpt_paged_kv_append(const cgpt_paged_args* args, void* stream) {
   using namespace cgpt;
-  const PagePool kc{k_cache, kc_sp, kc_sh, kc_ss}, vc{v_cache, vc_sp, vc_sh, vc_ss};
-  const int rc = check_paged(n_tokens, B, Hq, Hkv, head_dim, page_size, n_pages, max_pages, bt_stride, kc, vc, dtype);
+  bool empty;
+  const int rc = check_paged(args, &empty);
   if (rc != CGPT_OK) return rc;
-  if (k_cache == v_cache) return CGPT_EINVAL;
-  if ((q == nullptr) != (q_out == nullptr)) return CGPT_EINVAL;
-  if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2 != 0) return CGPT_ESHAPE;
-  if (rot_dim > 0 && (rotary == nullptr || n_pos <= 0 || rot_stride < rot_dim || n_pos > 0x7fffffff)) return CGPT_EINVAL;
-  if (n_tokens == 0 || B == 0) return CGPT_OK;
-  if (k == nullptr || v == nullptr || seq_lens == nullptr || (max_pages > 0 && block_table == nullptr)) return CGPT_EINVAL;
-  if (cu_q == nullptr && n_tokens != B) return CGPT_EINVAL;
-  const int64_t epv = dtype == CGPT_F32 ? 4 : 8;
-  for (int64_t st : {q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh})
-    if (st < 0 || st % epv != 0) return CGPT_EINVAL;
-  for (const void* p : {q, k, v, static_cast<const void*>(q_out)})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return CGPT_EINVAL;
-  if (reinterpret_cast<uintptr_t>(rotary) & 3) return CGPT_EINVAL;
-  AppendArgs a;
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.q_out = q_out;
-  a.kc = kc;
-  a.vc = vc;
-  a.seq = PagedBatch{block_table, seq_lens, cu_q, bt_stride, static_cast<int>(n_tokens), static_cast<int>(B),
-                     static_cast<int>(n_pages), static_cast<int>(max_pages),
-                     static_cast<int>(page_size * max_pages), FastDiv(page_size)};
-  a.rot = rotary;
-  a.q_st = q_st;
-  a.q_sh = q_sh;
-  a.k_st = k_st;
-  a.k_sh = k_sh;
-  a.v_st = v_st;
-  a.v_sh = v_sh;
-  a.qo_st = qo_st;
-  a.qo_sh = qo_sh;
-  a.rot_stride = rot_stride;
-  a.Hq = static_cast<int>(Hq);
-  a.Hkv = static_cast<int>(Hkv);
-  a.head_dim = static_cast<int>(head_dim);
-  a.rot_dim = static_cast<int>(rot_dim);
-  a.n_pos = static_cast<int>(n_pos);
-  a.interleaved = interleaved;
-  a.err = err_flag;
+  const cgpt_paged_args& p = *args;
+  if (p.k_cache == p.v_cache || (p.q == nullptr) != (p.out == nullptr)) return CGPT_EINVAL;
+  if (p.rot_dim < 0 || p.rot_dim > p.head_dim || p.rot_dim % 2 != 0) return CGPT_ESHAPE;
+  if (p.rot_dim > 0 && (p.rotary == nullptr || (reinterpret_cast<uintptr_t>(p.rotary) & 3) || p.n_pos <= 0 ||
+                        p.n_pos > 0x7fffffff || p.rot_stride < p.rot_dim))
+    return CGPT_EINVAL;
+  if (empty) return CGPT_OK;
+  if (p.k == nullptr || p.v == nullptr) return CGPT_EINVAL;
+  const AppendArgs a{p.q, p.k, p.v, p.out, PagePool{p.k_cache, p.kc_sp, p.kc_sh, p.kc_ss},
+                     PagePool{p.v_cache, p.vc_sp, p.vc_sh, p.vc_ss}, paged_batch(p), p.rotary, p.q_st, p.q_sh, p.k_st,
+                     p.k_sh, p.v_st, p.v_sh, p.out_st, p.out_sh, p.rot_stride, static_cast<int>(p.Hq),
+                     static_cast<int>(p.Hkv), static_cast<int>(p.head_dim), static_cast<int>(p.rot_dim),
+                     static_cast<int>(p.n_pos), static_cast<int>(p.interleaved), p.err_flag};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == CGPT_BF16) return launch_append<bf16_t>(a, s);
-  if (dtype == CGPT_F16) return launch_append<f16_t>(a, s);
+  if (p.dtype == CGPT_BF16) return launch_append<bf16_t>(a, s);
+  if (p.dtype == CGPT_F16) return launch_append<f16_t>(a, s);
   return launch_append<float>(a, s);
 }

@@ -74,7 +74,7 @@ struct PagedWs {
   float* tile_o;     // splits x n_tokens x Hq x HD
 };
 
-template <typename T, int HD, int QTW>
+template <typename T, int HD, int QTW, int NW = 4>
 struct StreamShape {
   static constexpr int ES = sizeof(T);
   static constexpr int EPC = 16 / ES;              // elements of a 16-byte chunk
@@ -85,7 +85,7 @@ struct StreamShape {
   static constexpr int ND = HD / 16;
   static constexpr int NT = (ES == 2 ? 2 : 1) * (HD >= 64 ? 1 : 2);  // 16-key tiles a wave takes at once
   static constexpr int KT = 16 * NT;
-  static constexpr int UK = 4 * KT;                // keys of a unit
+  static constexpr int UK = NW * KT;               // keys of a unit, KT a wave
   static constexpr int QT = QTW, R = 16 * QTW;
   static constexpr int KROW = HD * ES;
   static constexpr int VBYTES = KT * KROW;         // a wave's V tile in LDS; holds 16 fp32 rows of O too
@@ -95,25 +95,27 @@ struct StreamShape {
   static_assert(VBYTES >= 16 * HD * 4, "the join of the waves reuses the V tiles");
 };
 
-constexpr int kStreamThreads = 256;
+constexpr int kStreamThreads = 256, kStreamWaves = 4;
 
 // Each wave streams keys by itself: K and V rows go from their pages into registers,
 // one subtile of KT keys ahead of the one in use, in the layout of the matrix cores' A
 // operand (lane l: row l % 16, 16-byte chunk l / 16), so S^T = K Q^T needs no LDS at
 // all; V passes through the wave's own LDS tile for its transpose (O^T = V^T P^T).
-// The four waves of a block take the KT-key quarters of a unit and meet only at an
-// item's end.  P comes straight from the S^T accumulators, the key order inside a slab
-// permuted alike on both operands.
+// The NW waves of a block take a unit's KT-key parts and meet only at an item's end.
+// P comes straight from the S^T accumulators, the key order inside a slab permuted alike
+// on both operands.
 //
-// A16: page_size is a multiple of 16, so 16 keys lie in one page and the page comes by a
-// scalar load; else every lane looks its own key up.
-template <typename T, int HD, int QTW, bool A16>
-__global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2) void paged_stream_kernel(
-    PagedAttnArgs a, PagedWs ws, int prefix_units) {
-  using C = StreamShape<T, HD, QTW>;
+// WHOLE: a block is one item with all its keys, the prefix's among them, and writes its
+// rows' results; no workspace, no join.
+// A16: 16 keys from a multiple of 16 on lie in one page (and on one side of the prefix's
+// end), whose id comes by a scalar load; else every lane looks its own key up.
+template <typename T, int HD, int QTW, bool A16, int NW, bool WHOLE>
+__global__ __launch_bounds__(64 * NW, NW == 4 && HD * QTW <= 64 && QTW == 1 ? 4 : NW == 16 ? 4 : 2) void
+paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
+  using C = StreamShape<T, HD, QTW, NW>;
   constexpr int QT = C::QT, NT = C::NT, NKS = C::NKS, ND = C::ND, KT = C::KT, UK = C::UK, R = C::R;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * C::VBYTES];
-  __shared__ float wave_m[4][R], wave_l[4][R];
+  __shared__ __attribute__((aligned(16))) uint8_t smem[NW * C::VBYTES];
+  __shared__ float wave_m[NW][R], wave_l[NW][R];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int g = lane >> 4, frow = lane & 15;
@@ -123,12 +125,13 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
 
   // Units of the sequences, 64 at a time: lane l holds sequence c0 + l.
   int c0 = 0, n_units = 0, incl = 0, before = prefix_units, total = 0;
+  SeqUnits mine{};
   auto load_chunk = [&](int c) __attribute__((always_inline)) {
     c0 = c;
     n_units = 0;
     if (c + lane < a.seq.B) {
-      const SeqUnits u = seq_units<R, UK>(a, c + lane);
-      n_units = u.rt * u.kt * a.Hkv;
+      mine = seq_units<R, UK>(a, c + lane);
+      n_units = mine.rt * mine.kt * a.Hkv;
     }
     incl = n_units;
 #pragma unroll
@@ -138,26 +141,29 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
     }
     total = __builtin_amdgcn_readlane(incl, 63);
   };
-  int U = prefix_units;
-  for (int c = 0; c < a.seq.B; c += 64) {
-    load_chunk(c);
-    if (blockIdx.x == 0 && wave == 0 && c + lane < a.seq.B) ws.starts[c + lane] = U + incl - n_units;
-    U += total;
+  int u = 0, u_end = 1;
+  if constexpr (!WHOLE) {
+    int U = prefix_units;
+    for (int c = 0; c < a.seq.B; c += 64) {
+      load_chunk(c);
+      if (blockIdx.x == 0 && wave == 0 && c + lane < a.seq.B) ws.starts[c + lane] = U + incl - n_units;
+      U += total;
+    }
+    if (blockIdx.x == 0 && tid == 0) ws.starts[a.seq.B] = U;
+    if (a.seq.B > 64) load_chunk(0);
+    const int gblocks = active_blocks(gridDim.x, U);
+    if (static_cast<int>(blockIdx.x) >= gblocks || U == 0) return;
+    u = unit_start(blockIdx.x, U, gblocks);
+    u_end = unit_start(blockIdx.x + 1, U, gblocks);
   }
-  if (blockIdx.x == 0 && tid == 0) ws.starts[a.seq.B] = U;
-  if (a.seq.B > 64) load_chunk(0);
-  const int gblocks = active_blocks(gridDim.x, U);
-  if (static_cast<int>(blockIdx.x) >= gblocks || U == 0) return;
-  int u = unit_start(blockIdx.x, U, gblocks);
-  const int u_end = unit_start(blockIdx.x + 1, U, gblocks);
 
   while (u < u_end) {
     // Addresses are made anew for every item: kept over the loop they cost registers that
     // the loads in flight need.
     asm volatile("" : "+v"(g), "+v"(frow));
     // ---- the item that unit u lies in
-    const bool prefix = u < prefix_units;
-    int hk, rt, t0, kt_item, b = 0, n, kb, base0, rows, first = 0, pos0 = 0;
+    const bool prefix = !WHOLE && u < prefix_units;
+    int hk, rt, t0 = 0, kt_item, n, kb = 0, base0 = 0, rows, first = 0, pos0 = 0;
     const int* trow;
     if (prefix) {
       kt_item = (a.prefix_len + UK - 1) / UK;
@@ -168,35 +174,53 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
       hk = item / rts;
       rt = item - hk * rts;
       n = a.prefix_len;
-      kb = base0 = 0;
       trow = a.prefix;
     } else {
-      while (u >= before + total) {
-        before += total;
-        load_chunk(c0 + 64);
+      int b, len, count, n_all;
+      if constexpr (WHOLE) {
+        const int tile = static_cast<int>(blockIdx.x) / a.Hkv;
+        hk = static_cast<int>(blockIdx.x) - tile * a.Hkv;
+        rt = tile;
+        b = slot_seq<R>(a.seq, G, lane, &rt);
+        if (b >= a.seq.B) return;
+        seq_tokens(a.seq, b, &first, &count);
+        len = max(a.seq.lens[b], 0);
+        n_all = min(len, a.seq.cap);
+        rows = count * G;
+        if (rt < 0 || rt * R >= rows) return;
+      } else {
+        while (u >= before + total) {
+          if (c0 + 64 >= a.seq.B) return;  // the lengths changed under the call
+          before += total;
+          load_chunk(c0 + 64);
+        }
+        const int at = __popcll(__builtin_amdgcn_ballot_w64(before + incl <= u));
+        auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
+        b = c0 + at;
+        const int rts = of(mine.rt);
+        const int rel = u - before - of(incl - n_units);
+        first = of(mine.first);
+        count = of(mine.count);
+        len = of(mine.len);
+        n_all = of(mine.n);
+        kt_item = of(mine.kt);
+        const int item = rel / kt_item;
+        t0 = rel - item * kt_item;
+        hk = item / rts;
+        rt = item - hk * rts;
+        kb = a.prefix_len;
+        base0 = kb & ~15;
+        rows = count * G;
       }
-      const int at = __popcll(__builtin_amdgcn_ballot_w64(before + incl <= u));
-      b = c0 + at;
-      const SeqUnits su = seq_units<R, UK>(a, b);
-      const int rel = u - before - __builtin_amdgcn_readlane(incl - n_units, at);
-      kt_item = su.kt;
-      const int item = rel / su.kt;
-      t0 = rel - item * su.kt;
-      hk = item / su.rt;
-      rt = item - hk * su.rt;
-      kb = su.kb;
-      base0 = su.base0;
-      rows = su.count * G;
-      first = su.first;
-      pos0 = su.len - su.count;
+      pos0 = len - count;
       // Keys that the tile's last row sees.
-      const int last = a.group.div(min(rt * R + R, rows) - 1);
-      n = min(su.n, max(pos0 + last + 1, 0));
+      n = min(n_all, max(pos0 + a.group.div(min(rt * R + R, rows) - 1) + 1, 0));
+      if constexpr (WHOLE) kt_item = (n + UK - 1) / UK;
       trow = a.seq.table + b * a.seq.stride;
-      bad |= su.len > a.seq.cap;
+      bad |= len > a.seq.cap;
     }
-    const int t1 = min(kt_item, t0 + (u_end - u));
-    u += t1 - t0;
+    const int t1 = WHOLE ? kt_item : min(kt_item, t0 + (u_end - u));
+    u += WHOLE ? 1 : t1 - t0;
 
     // ---- its rows: lane (g, frow) works for rows rt R + 16 qt + frow
     const int r0 = rt * R, nqt = min(QT, (rows - r0 + 15) >> 4);
@@ -249,10 +273,12 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
       for (int kt = 0; kt < NT; ++kt) {
         const int tile = sub0 + i * UK + 16 * kt;
         if (A16) {
-          const int col = a.seq.page.div(min(tile, (n - 1) & ~15));
-          pg[kt] = ((const __attribute__((address_space(4))) int*)trow)[__builtin_amdgcn_readfirstlane(col)];
+          const int key = min(tile, (n - 1) & ~15), col = a.seq.page.div(key);
+          const int* const row = WHOLE && key < a.prefix_len ? a.prefix : trow;
+          pg[kt] = ((const __attribute__((address_space(4))) int*)row)[__builtin_amdgcn_readfirstlane(col)];
         } else {
-          pg[kt] = trow[a.seq.page.div(max(min(tile + frow, n - 1), kb))];
+          const int key = max(min(tile + frow, n - 1), kb);
+          pg[kt] = (WHOLE && key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
         }
       }
     };
@@ -474,7 +500,7 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
       }
     }
 
-    // ---- the four waves' parts joined
+    // ---- the waves' parts joined
     const bool whole = t0 == 0 && t1 == kt_item;
     const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
 #pragma unroll
@@ -489,7 +515,9 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
     for (int qt = 0; qt < nqt; ++qt) {
       __syncthreads();  // the maxima are there, the V tiles (or the rows before) are done with
       const int row = 16 * qt + frow;
-      const float m = fmaxf(fmaxf(wave_m[0][row], wave_m[1][row]), fmaxf(wave_m[2][row], wave_m[3][row]));
+      float m = wave_m[0][row];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) m = fmaxf(m, wave_m[w][row]);
       const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wave_m[wave][row] - m);
       float* os = reinterpret_cast<float*>(sv);
 #pragma unroll
@@ -501,15 +529,17 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
             *reinterpret_cast<f32x4_t*>(os + frow * HD + ((((4 * dt + g) ^ frow) & (HD / 4 - 1)) << 2)) = v;
           }
       __syncthreads();
-      for (int i = tid; i < 16 * (HD / 4); i += kStreamThreads) {
+      for (int i = tid; i < 16 * (HD / 4); i += 64 * NW) {
         const int rr = i / (HD / 4), c = i % (HD / 4), r = r0 + 16 * qt + rr;
         if (r >= rows) continue;
         const int wr = 16 * qt + rr;
-        const float mm = fmaxf(fmaxf(wave_m[0][wr], wave_m[1][wr]), fmaxf(wave_m[2][wr], wave_m[3][wr]));
+        float mm = wave_m[0][wr];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) mm = fmaxf(mm, wave_m[w][wr]);
         float l = 0.f;
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
           const float* ow = reinterpret_cast<const float*>(smem + w * C::VBYTES);
           const f32x4_t x = *reinterpret_cast<const f32x4_t*>(ow + rr * HD + (((c ^ rr) & (HD / 4 - 1)) << 2));
 #pragma unroll
@@ -517,7 +547,7 @@ __global__ __launch_bounds__(kStreamThreads, HD * QTW <= 64 && QTW == 1 ? 4 : 2)
           l += mm == -INFINITY ? 0.f : wave_l[w][wr] * __builtin_amdgcn_exp2f(wave_m[w][wr] - mm);
         }
         const int tok = a.group.div(r), h = hk * G + r - tok * G, t = first + tok;
-        if (whole && a.prefix_len == 0) {
+        if (WHOLE || (whole && a.prefix_len == 0)) {
           const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key, or a NaN that stays one
           const float out[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
           store4_out(static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh + 4 * c, out);
@@ -638,22 +668,36 @@ __global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArg
 // What a call runs: the tile kernel on the sequences' rows or on all rows against the
 // prefix, the stream kernel, and the join.  Workspace offsets in bytes.
 struct PagedPlan {
+  bool whole = false;               // stream kernel, a block an item
   bool tile = false, flat = false;  // tile kernel; its rows are the whole batch's
   int tile_qt = 1, n_split = 1;
   int stream_qt = 0, grid = 0, prefix_units = 0;  // stream kernel (stream_qt 0: none)
   int64_t o_starts = 0, o_eml = 0, o_eo = 0, o_wml = 0, o_wo = 0, o_tml = 0, o_to = 0, bytes = 0;
 };
 
+// Waves of a block that takes a whole item: as many as the registers allow.
+constexpr int whole_waves(int hd) { return hd == 128 ? 8 : 16; }
+constexpr int64_t kWholeKeys = 2048, kWholeAgain = int64_t{16} << 20;
+
 template <typename T, int HD>
-static int make_plan(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t cap, int64_t prefix_len, int dtype,
-                     PagedPlan* p) {
-  const int64_t G = Hq / Hkv, rows = n_tokens * G, cus = num_cus();
+static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
+  const int64_t n_tokens = call.n_tokens, B = call.B, Hq = call.Hq, Hkv = call.Hkv, prefix_len = call.prefix_len;
+  const int64_t cap = call.page_size * call.max_pages, rows = n_tokens * (Hq / Hkv), cus = num_cus();
   auto take = [&](int64_t bytes) {
     const int64_t o = p->bytes;
     p->bytes += (bytes + 63) / 64 * 64;
     return o;
   };
-  const bool tile_ok = paged_tile_ok(dtype, HD);
+  // Short sequences: one launch.
+  const int64_t again = prefix_len * Hkv * HD * static_cast<int64_t>(sizeof(T)) * 2 * (B - 1);
+  if (rows <= 16 * B && cap <= kWholeKeys && again <= kWholeAgain) {
+    p->whole = true;
+    const int64_t blocks = Hkv * (call.cu_q == nullptr && Hq / Hkv <= 16 ? B : rows / 16 + B);
+    if (blocks > 0x7fffffff) return CGPT_ESHAPE;
+    p->grid = static_cast<int>(blocks);
+    return CGPT_OK;
+  }
+  const bool tile_ok = paged_tile_ok(call.dtype, HD);
   p->flat = tile_ok && prefix_len > 0 && rows > 64 && rows <= 16 * B;
   p->tile = p->flat || (tile_ok && rows > 16 * B);
   if (p->tile) {
@@ -691,13 +735,14 @@ static int make_plan(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64
   return CGPT_OK;
 }
 
-template <typename T, int HD, int QTW>
+template <typename T, int HD, int QTW, int NW, bool WHOLE>
 static void launch_stream(const PagedAttnArgs& a, const PagedWs& ws, const PagedPlan& p, hipStream_t s) {
-  if (a.seq.page.d % 16 == 0)
-    hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, true>), dim3(p.grid), dim3(kStreamThreads), 0, s, a, ws,
+  const bool a16 = a.seq.page.d % 16 == 0 && (!WHOLE || a.prefix_len % 16 == 0);
+  if (a16)
+    hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, true, NW, WHOLE>), dim3(p.grid), dim3(64 * NW), 0, s, a, ws,
                        p.prefix_units);
   else
-    hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, false>), dim3(p.grid), dim3(kStreamThreads), 0, s, a, ws,
+    hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, false, NW, WHOLE>), dim3(p.grid), dim3(64 * NW), 0, s, a, ws,
                        p.prefix_units);
 }
 
@@ -710,23 +755,27 @@ static void launch_join(const PagedAttnArgs& a, const PagedWs& ws, const PagedPl
 }
 
 template <typename T, int HD>
-static int run_plan(const PagedAttnArgs& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t s) {
+static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStream_t s) {
   PagedPlan p;
-  int rc = make_plan<T, HD>(a.seq.n_tokens, a.seq.B, a.Hq, a.Hkv, a.seq.cap, a.prefix_len, dtype, &p);
+  int rc = make_plan<T, HD>(call, &p);
   if (rc != CGPT_OK) return rc;
-  if (p.bytes > 0 && (ws_bytes < p.bytes || workspace == nullptr)) return CGPT_ESCRATCH;
-  if (reinterpret_cast<uintptr_t>(workspace) & 15) return CGPT_EINVAL;
-  char* w = static_cast<char*>(workspace);
+  char* w = static_cast<char*>(call.workspace);
+  if (p.bytes > 0 && (call.workspace_bytes < p.bytes || w == nullptr)) return CGPT_ESCRATCH;
+  if (reinterpret_cast<uintptr_t>(w) & 15) return CGPT_EINVAL;
   auto f32 = [&](int64_t o) { return reinterpret_cast<float*>(w + o); };
   const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), f32(p.o_eml), f32(p.o_eo), f32(p.o_wml), f32(p.o_wo),
                    f32(p.o_tml), f32(p.o_to)};
   constexpr int WIDE = HD == 128 ? 2 : 4;
   if (p.tile) {
-    rc = launch_paged_tile(dtype, HD, a, p.flat, p.tile_qt, p.n_split, ws.tile_ml, ws.tile_o, s);
+    rc = launch_paged_tile(call.dtype, HD, a, p.flat, p.tile_qt, p.n_split, ws.tile_ml, ws.tile_o, s);
     if (rc != CGPT_OK) return rc;
   }
-  if (p.stream_qt == 1) launch_stream<T, HD, 1>(a, ws, p, s);
-  if (p.stream_qt > 1) launch_stream<T, HD, WIDE>(a, ws, p, s);
+  if (p.whole) {
+    launch_stream<T, HD, 1, whole_waves(HD), true>(a, ws, p, s);
+    return hip_status(hipGetLastError());
+  }
+  if (p.stream_qt == 1) launch_stream<T, HD, 1, kStreamWaves, false>(a, ws, p, s);
+  if (p.stream_qt > 1) launch_stream<T, HD, WIDE, kStreamWaves, false>(a, ws, p, s);
   if (p.stream_qt > 1)
     launch_join<T, HD, WIDE>(a, ws, p, s);
   else if (p.stream_qt == 1 || p.n_split > 1)
@@ -735,108 +784,58 @@ static int run_plan(const PagedAttnArgs& a, int dtype, void* workspace, int64_t 
 }
 
 template <typename F>
-static int with_stream(int dtype, int hd, F&& f) {
+static int with_type(const cgpt_paged_args& p, F&& f) {
 #define CGPT_PAGED_HD(T)                                                \
-  switch (hd) {                                                         \
+  switch (p.head_dim) {                                                 \
     case 16: return f(T{}, std::integral_constant<int, 16>{});          \
     case 32: return f(T{}, std::integral_constant<int, 32>{});          \
     case 64: return f(T{}, std::integral_constant<int, 64>{});          \
     case 128: return f(T{}, std::integral_constant<int, 128>{});        \
     default: return CGPT_ESHAPE;                                        \
   }
-  if (dtype == CGPT_BF16) CGPT_PAGED_HD(bf16_t)
-  if (dtype == CGPT_F16) CGPT_PAGED_HD(f16_t)
+  if (p.dtype == CGPT_BF16) CGPT_PAGED_HD(bf16_t)
+  if (p.dtype == CGPT_F16) CGPT_PAGED_HD(f16_t)
   CGPT_PAGED_HD(float)
 #undef CGPT_PAGED_HD
 }
 
 }  // namespace cgpt
 
-extern "C" int cgpt_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
-                                            const int* block_table, const int* seq_lens, const int* cu_q,
-                                            const int* prefix_pages, int64_t prefix_len, int64_t n_tokens,
-                                            int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
-                                            int64_t page_size, int64_t n_pages, int64_t max_pages,
-                                            int64_t bt_stride, int64_t q_st, int64_t q_sh, int64_t o_st,
-                                            int64_t o_sh, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
-                                            int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, float scale,
-                                            void* workspace, int64_t workspace_bytes, int dtype,
-                                            int* err_flag, void* stream) {
+extern "C" int cgpt_paged_attention(const cgpt_paged_args* args, void* stream) {
   using namespace cgpt;
-  const PagePool kc{const_cast<void*>(k_cache), kc_sp, kc_sh, kc_ss}, vc{const_cast<void*>(v_cache), vc_sp, vc_sh, vc_ss};
-  const int rc = check_paged(n_tokens, B, Hq, Hkv, head_dim, page_size, n_pages, max_pages, bt_stride, kc, vc, dtype);
+  bool empty;
+  const int rc = check_paged(args, &empty);
   if (rc != CGPT_OK) return rc;
-  if (prefix_len < 0 || prefix_len > page_size * max_pages) return CGPT_EINVAL;
-  if (!(scale > 0.f)) return CGPT_EINVAL;
-  if (n_tokens == 0 || B == 0) return CGPT_OK;
-  if (q == nullptr || o == nullptr || seq_lens == nullptr || (max_pages > 0 && block_table == nullptr) ||
-      (prefix_len > 0 && prefix_pages == nullptr))
+  const cgpt_paged_args& p = *args;
+  const float scale = static_cast<float>(p.scale);
+  if (p.prefix_len < 0 || p.prefix_len > p.page_size * p.max_pages || !(scale > 0.f) || !(scale < INFINITY))
     return CGPT_EINVAL;
-  if (cu_q == nullptr && n_tokens != B) return CGPT_EINVAL;
-  const int64_t epv = dtype == CGPT_F32 ? 4 : 8;
-  for (int64_t st : {q_st, q_sh, o_st, o_sh})
-    if (st < 0 || st % epv != 0) return CGPT_EINVAL;
-  for (const void* p : {q, static_cast<const void*>(o)})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return CGPT_EINVAL;
-  PagedAttnArgs a;
-  a.q = q;
-  a.o = o;
-  a.kc = kc;
-  a.vc = vc;
-  a.seq = PagedBatch{block_table, seq_lens, cu_q, bt_stride, static_cast<int>(n_tokens), static_cast<int>(B),
-                     static_cast<int>(n_pages), static_cast<int>(max_pages),
-                     static_cast<int>(page_size * max_pages), FastDiv(page_size)};
-  a.prefix = prefix_pages;
-  a.prefix_len = static_cast<int>(prefix_len);
-  a.prefix_cols = static_cast<int>((prefix_len + page_size - 1) / page_size);
-  a.q_st = q_st;
-  a.q_sh = q_sh;
-  a.o_st = o_st;
-  a.o_sh = o_sh;
-  a.Hq = static_cast<int>(Hq);
-  a.Hkv = static_cast<int>(Hkv);
-  a.group = FastDiv(Hq / Hkv);
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.err = err_flag;
+  if (empty) return CGPT_OK;
+  if (p.q == nullptr || p.out == nullptr || (p.prefix_len > 0 && p.prefix_pages == nullptr)) return CGPT_EINVAL;
+  const PagedAttnArgs a{p.q, p.out, PagePool{p.k_cache, p.kc_sp, p.kc_sh, p.kc_ss},
+                        PagePool{p.v_cache, p.vc_sp, p.vc_sh, p.vc_ss}, paged_batch(p), p.prefix_pages,
+                        static_cast<int>(p.prefix_len), p.q_st, p.q_sh, p.out_st, p.out_sh, static_cast<int>(p.Hq),
+                        static_cast<int>(p.Hkv), FastDiv(p.Hq / p.Hkv), scale * 1.4426950408889634f, p.err_flag};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return with_stream(dtype, static_cast<int>(head_dim), [&](auto t, auto hd) {
-    using T = decltype(t);
-    constexpr int HD = decltype(hd)::value;
-    return run_plan<T, HD>(a, dtype, workspace, workspace_bytes, s);
+  return with_type(p, [&](auto t, auto hd) {
+    return run_plan<decltype(t), decltype(hd)::value>(a, p, s);
   });
 }
 
-extern "C" int cgpt_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
-                                    const int* block_table, const int* seq_lens, const int* cu_q,
-                                    int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
-                                    int64_t page_size, int64_t n_pages, int64_t max_pages, int64_t bt_stride,
-                                    int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh, int64_t kc_sp,
-                                    int64_t kc_sh, int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss,
-                                    float scale, void* workspace, int64_t workspace_bytes, int dtype,
-                                    int* err_flag, void* stream) {
-  return cgpt_shared_prefix_attention(q, k_cache, v_cache, o, block_table, seq_lens, cu_q, nullptr, 0, n_tokens, B,
-                                      Hq, Hkv, head_dim, page_size, n_pages, max_pages, bt_stride, q_st, q_sh, o_st,
-                                      o_sh, kc_sp, kc_sh, kc_ss, vc_sp, vc_sh, vc_ss, scale, workspace,
-                                      workspace_bytes, dtype, err_flag, stream);
-}
-
-extern "C" int cgpt_paged_attention_workspace(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv,
-                                              int64_t head_dim, int64_t page_size, int64_t max_pages,
-                                              int64_t prefix_len, int dtype, int64_t* workspace_bytes) {
+extern "C" int cgpt_paged_attention_workspace(const cgpt_paged_args* args, int64_t* workspace_bytes) {
   using namespace cgpt;
-  if (workspace_bytes == nullptr) return CGPT_EINVAL;
+  if (args == nullptr || workspace_bytes == nullptr) return CGPT_EINVAL;
   *workspace_bytes = 0;
-  if (n_tokens < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || page_size <= 0 || max_pages < 0 ||
-      prefix_len < 0 || prefix_len > page_size * max_pages)
+  const cgpt_paged_args& p = *args;
+  if (p.n_tokens < 0 || p.B < 0 || p.Hq <= 0 || p.Hkv <= 0 || p.Hq % p.Hkv != 0 || p.page_size <= 0 ||
+      p.max_pages < 0 || p.prefix_len < 0 || p.prefix_len > p.page_size * p.max_pages)
     return CGPT_EINVAL;
-  if (dtype != CGPT_F32 && dtype != CGPT_BF16 && dtype != CGPT_F16) return CGPT_EDTYPE;
-  if (n_tokens == 0 || B == 0) return CGPT_OK;
-  return with_stream(dtype, static_cast<int>(head_dim), [&](auto t, auto hd) {
-    using T = decltype(t);
-    constexpr int HD = decltype(hd)::value;
-    PagedPlan p;
-    const int rc = make_plan<T, HD>(n_tokens, B, Hq, Hkv, page_size * max_pages, prefix_len, dtype, &p);
-    if (rc == CGPT_OK) *workspace_bytes = p.bytes;
+  if (p.dtype != CGPT_F32 && p.dtype != CGPT_BF16 && p.dtype != CGPT_F16) return CGPT_EDTYPE;
+  if (p.n_tokens == 0 || p.B == 0) return CGPT_OK;
+  return with_type(p, [&](auto t, auto hd) {
+    PagedPlan plan;
+    const int rc = make_plan<decltype(t), decltype(hd)::value>(p, &plan);
+    if (rc == CGPT_OK) *workspace_bytes = plan.bytes;
     return rc;
   });
 }

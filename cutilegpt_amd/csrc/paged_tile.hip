@@ -59,23 +59,12 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
     rows = a.seq.n_tokens * G;
     n = a.prefix_len;
   } else {
-    // Sequence b has the tiles from start(b) = cu[b] G / BQ + b on, at least as many as its
-    // rows fill.
-    int b = 0;
-    for (int c = 0; c < a.seq.B; c += 64) {
-      const int bb = c + lane + 1;
-      int at = bb;
-      if (a.seq.cu != nullptr && bb <= a.seq.B) at = min(max(a.seq.cu[bb], 0), a.seq.n_tokens);
-      const bool below = bb <= a.seq.B && at * G / BQ + bb <= tile;
-      const int k = __popcll(__builtin_amdgcn_ballot_w64(below));
-      b += k;
-      if (k < 64) break;
-    }
+    int rt = tile, count;
+    const int b = slot_seq<BQ>(a.seq, G, lane, &rt);
     if (b >= a.seq.B) return;
-    int count;
     seq_tokens(a.seq, b, &first, &count);
     rows = count * G;
-    r0 = (tile - (first * G / BQ + b)) * BQ;
+    r0 = rt * BQ;
     if (r0 < 0 || r0 >= rows) return;
     const int len = max(a.seq.lens[b], 0);
     bad = len > a.seq.cap;
@@ -356,7 +345,7 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
-bool paged_tile_ok(int dtype, int head_dim) {
+bool paged_tile_ok(int64_t dtype, int head_dim) {
   return dtype != CGPT_F32 && (head_dim == 64 || head_dim == 128);
 }
 
@@ -364,7 +353,8 @@ template <typename T, int HD, int QTW>
 static int launch_tile(const PagedAttnArgs& a, bool flat, int n_split, float* part_ml, float* part_o, hipStream_t s) {
   constexpr int BQ = 64 * QTW;
   const int64_t rows = static_cast<int64_t>(a.seq.n_tokens) * (a.Hq / a.Hkv);
-  const int64_t tiles = flat ? (rows + BQ - 1) / BQ : rows / BQ + a.seq.B;
+  const int64_t tiles = flat ? (rows + BQ - 1) / BQ
+                        : a.seq.cu == nullptr && a.Hq / a.Hkv <= BQ ? a.seq.B : rows / BQ + a.seq.B;
   const int64_t blocks = tiles * n_split * a.Hkv;
   if (blocks > 0x7fffffff) return CGPT_ESHAPE;
   if (flat)
@@ -383,7 +373,7 @@ static int launch_tile_qt(const PagedAttnArgs& a, bool flat, int qt, int n_split
                  : launch_tile<T, HD, 1>(a, flat, n_split, part_ml, part_o, s);
 }
 
-int launch_paged_tile(int dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split, float* part_ml,
+int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split, float* part_ml,
                       float* part_o, hipStream_t s) {
   if (dtype == CGPT_BF16 && head_dim == 64) return launch_tile_qt<bf16_t, 64>(a, flat, qt, n_split, part_ml, part_o, s);
   if (dtype == CGPT_BF16 && head_dim == 128) return launch_tile_qt<bf16_t, 128>(a, flat, qt, n_split, part_ml, part_o, s);

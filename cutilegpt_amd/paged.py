@@ -35,6 +35,7 @@ of one call must not name the same slot.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import Optional
@@ -42,7 +43,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .kernels import _dtype_code, _require_gpu, _stream
+from .kernels import _require_gpu
 
 __all__ = ["rotary_table", "paged_kv_append", "paged_attention", "shared_prefix_attention"]
 
@@ -61,22 +62,27 @@ def rotary_table(n_pos: int, rot_dim: int, base: float = 10000.0, device="cuda")
     return torch.cat([w.cos(), w.sin()], 1).float()
 
 
-def _rows(t: torch.Tensor, vec: int) -> torch.Tensor:
-    """(n, heads, hd) rows that 16-byte loads can read: the view itself or a copy."""
+_CODE = {torch.float32: _lib.CGPT_F32, torch.bfloat16: _lib.CGPT_BF16, torch.float16: _lib.CGPT_F16}
+
+
+def _rows(t: torch.Tensor, vec: int):
+    """(n, heads, hd) rows that 16-byte loads can read, the view itself or a copy, and
+    their strides."""
     s0, s1, s2 = t.stride()
     if s2 != 1 or s0 % vec or s1 % vec or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
+        s0, s1, _ = t.stride()
+    return t, s0, s1
 
 
 def _check_out(name: str, out: torch.Tensor, like: torch.Tensor, vec: int) -> None:
-    _require_gpu(name, out)
-    s0, s1, s2 = out.stride()
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+    if (not isinstance(out, torch.Tensor) or out.shape != like.shape or out.dtype != like.dtype
+            or out.device != like.device):
         raise ValueError(f"{name}: the output must be a {like.dtype} tensor of shape {tuple(like.shape)} "
-                         f"on {like.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+                         f"on {like.device}")
+    s0, s1, s2 = out.stride()
     n, h, hd = out.shape
     if s2 != 1 or s0 % vec or s1 % vec or out.data_ptr() % 16 or (h > 1 and s1 < hd) or (n > 1 and s0 < hd):
         raise ValueError(f"{name}: the output's rows must be separate, contiguous and 16-byte aligned")
@@ -84,40 +90,47 @@ def _check_out(name: str, out: torch.Tensor, like: torch.Tensor, vec: int) -> No
 
 def _check_cache(name: str, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  block_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: Optional[torch.Tensor],
-                 err_flag: Optional[torch.Tensor]) -> int:
-    """Checks what every entry point takes; returns the elements in 16 bytes."""
+                 err_flag: Optional[torch.Tensor]):
+    """Checks what every entry point takes; returns the rows' device index, the dtype's
+    code, the elements in 16 bytes, the caches' sizes and strides and the table's sizes."""
     _require_gpu(name, x, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
-    dev, dt = x.device, x.dtype
-    _dtype_code(x, name)
-    for t in (k_cache, v_cache, block_table, seq_lens, cu_q, err_flag):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: every tensor must be on {dev}, got one on {t.device}")
-    if x.dim() != 3:
-        raise ValueError(f"{name}: the step's rows must be (n_tokens, heads, head_dim), got {tuple(x.shape)}")
+    dev, dt = x.get_device(), x.dtype
+    if (k_cache.get_device() != dev or v_cache.get_device() != dev or block_table.get_device() != dev
+            or seq_lens.get_device() != dev or (cu_q is not None and cu_q.get_device() != dev)
+            or (err_flag is not None and err_flag.get_device() != dev)):
+        raise ValueError(f"{name}: every tensor must be on {x.device}")
+    code = _CODE.get(dt)
+    if code is None:
+        raise ValueError(f"{name}: unsupported dtype {dt} (float32, bfloat16 or float16)")
     if k_cache.dtype != dt or v_cache.dtype != dt:
         raise ValueError(f"{name}: the caches hold {k_cache.dtype} and {v_cache.dtype}, the rows {dt}")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or 0 in k_cache.shape:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or 0 in shape:
         raise ValueError(f"{name}: k_cache and v_cache must share a shape (n_pages, n_kv_head, page_size, "
-                         f"head_dim), got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    n_pages, heads, page, hd = k_cache.shape
-    if hd not in _HEAD_DIMS or x.shape[2] != hd:
-        raise ValueError(f"{name}: head_dim must be one of {_HEAD_DIMS} and the caches', got "
-                         f"{x.shape[2]} and {hd}")
-    vec = 4 if dt is torch.float32 else 8
-    for c in (k_cache, v_cache):
-        sp, sh, ss, sd = c.stride()
-        if (sd != 1 or sp % vec or sh % vec or ss % vec or c.data_ptr() % 16 or (n_pages > 1 and sp < hd)
-                or (heads > 1 and sh < hd) or (page > 1 and ss < hd)):
-            raise ValueError(f"{name}: cache rows must be separate, contiguous and 16-byte aligned")
-    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0]:
+                         f"head_dim), got {tuple(shape)} and {tuple(v_cache.shape)}")
+    n_pages, heads, page, hd = shape
+    if x.dim() != 3 or x.shape[2] != hd or hd not in _HEAD_DIMS:
+        raise ValueError(f"{name}: the step's rows must be (n_tokens, heads, head_dim), head_dim one of "
+                         f"{_HEAD_DIMS} and the caches' {hd}, got {tuple(x.shape)}")
+    vec = 4 if code == 0 else 8
+    kp, kh, ks, kd = k_cache.stride()
+    vp, vh, vs, vd = v_cache.stride()
+    if (kd != 1 or vd != 1 or (kp | kh | ks | vp | vh | vs) % vec
+            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or (n_pages > 1 and min(kp, vp) < hd)
+            or (heads > 1 and min(kh, vh) < hd) or (page > 1 and min(ks, vs) < hd)):
+        raise ValueError(f"{name}: cache rows must be separate, contiguous and 16-byte aligned")
+    if block_table.dim() != 2 or seq_lens.dim() != 1:
         raise ValueError(f"{name}: block_table must be (B, pages) and seq_lens (B,), got "
                          f"{tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
+    B, cols = block_table.shape
+    ts, t1 = block_table.stride()
+    if seq_lens.shape[0] != B:
+        raise ValueError(f"{name}: block_table has {B} rows for {seq_lens.shape[0]} seq_lens")
     if (block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32
             or (cu_q is not None and cu_q.dtype != torch.int32)):
         raise ValueError(f"{name}: block_table, seq_lens and cu_q must be int32")
-    if (block_table.stride(1) != 1 and block_table.shape[1] > 1) or not seq_lens.is_contiguous():
+    if (t1 != 1 and cols > 1) or not seq_lens.is_contiguous():
         raise ValueError(f"{name}: block_table rows and seq_lens must be contiguous")
-    B = seq_lens.shape[0]
     if cu_q is None:
         if x.shape[0] != B:
             raise ValueError(f"{name}: {x.shape[0]} rows for {B} sequences need cu_q")
@@ -125,11 +138,22 @@ def _check_cache(name: str, x: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise ValueError(f"{name}: cu_q must be {B + 1} contiguous offsets, got {tuple(cu_q.shape)}")
     if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() != 1):
         raise ValueError(f"{name}: err_flag must be one int32")
-    return vec
+    return dev, code, vec, n_pages, heads, page, hd, (kp, kh, ks, vp, vh, vs), B, cols, ts
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(fn, args: bytes, dev: int, name: str) -> None:
+    """One native call on the rows' device, on its current stream."""
+    if dev == torch.cuda.current_device():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -146,56 +170,59 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     ``interleaved``, in float32, rounded once.  Returns the turned queries (in
     ``q_out`` when given, which may be ``q``), None without ``q``."""
     name = "paged_kv_append"
-    vec = _check_cache(name, k, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
+    dev, code, vec, n_pages, hkv, page, hd, cs, B, cols, ts = _check_cache(
+        name, k, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
     _require_gpu(name, v, q, rotary)
-    n, hkv, hd = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or hkv != k_cache.shape[1]:
-        raise ValueError(f"{name}: k and v must be {k.dtype} (n_tokens, {k_cache.shape[1]}, {hd}) rows, got "
+    n = k.shape[0]
+    if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != dev or k.shape[1] != hkv:
+        raise ValueError(f"{name}: k and v must be {k.dtype} (n_tokens, {hkv}, {hd}) rows, got "
                          f"{tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
     if k_cache.data_ptr() == v_cache.data_ptr():
         raise ValueError(f"{name}: k_cache and v_cache are the same memory")
-    rot = 0
+    rot = n_pos = rs = 0
     if rotary is not None:
-        if (rotary.dim() != 2 or rotary.dtype != torch.float32 or rotary.device != k.device
-                or rotary.shape[0] < 1 or rotary.stride(1) != 1 or rotary.stride(0) < rotary.shape[1]):
+        if rotary.dim() != 2 or rotary.dtype != torch.float32 or rotary.get_device() != dev:
             raise ValueError(f"{name}: rotary must be a float32 table (n_pos, rot_dim) on {k.device}")
-        rot = rotary.shape[1]
-        if rot < 2 or rot % 2 or rot > hd:
-            raise ValueError(f"{name}: rot_dim must be even and at most head_dim {hd}, got {rot}")
-    hq, qr = hkv, None
+        n_pos, rot = rotary.shape
+        rs, r1 = rotary.stride()
+        if n_pos < 1 or rot < 2 or rot % 2 or rot > hd or r1 != 1 or rs < rot:
+            raise ValueError(f"{name}: rotary must have rows of an even rot_dim of at most {hd} values, got "
+                             f"{tuple(rotary.shape)} with strides {rotary.stride()}")
+    hq, qr, qs, qh, os_, oh = hkv, None, 0, 0, 0, 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != hd or q.dtype != k.dtype or q.device != k.device:
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != hd or q.dtype != k.dtype or q.get_device() != dev:
             raise ValueError(f"{name}: q must be {k.dtype} rows ({n}, n_head, {hd}), got {q.dtype} {tuple(q.shape)}")
         hq = q.shape[1]
         if hq == 0 or hq % hkv:
             raise ValueError(f"{name}: n_head {hq} is not a multiple of n_kv_head {hkv}")
         if q_out is None:
-            q_out = torch.empty((n, hq, hd), dtype=q.dtype, device=q.device)
+            q_out = q.new_empty((n, hq, hd))
         else:
             _check_out(name, q_out, q, vec)
-        qr = _rows(q, vec)
+        qr, qs, qh = _rows(q, vec)
+        os_, oh, _ = q_out.stride()
     elif q_out is not None:
         raise ValueError(f"{name}: q_out without q")
-    kr, vr = _rows(k, vec), _rows(v, vec)
-    lib = _lib.load()
-    with torch.cuda.device(k.device):
-        _lib.check(lib.cgpt_paged_kv_append(
-            _ptr(qr), kr.data_ptr(), vr.data_ptr(), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(),
-            block_table.data_ptr(), seq_lens.data_ptr(), _ptr(cu_q), _ptr(rotary), n, seq_lens.shape[0], hq, hkv,
-            hd, k_cache.shape[2], k_cache.shape[0], block_table.shape[1], block_table.stride(0),
-            *((0, 0) if qr is None else qr.stride()[:2]), *kr.stride()[:2], *vr.stride()[:2],
-            *((0, 0) if q_out is None else q_out.stride()[:2]), *k_cache.stride()[:3], *v_cache.stride()[:3],
-            rot, 0 if rotary is None else rotary.shape[0], 0 if rotary is None else rotary.stride(0),
-            int(interleaved), _dtype_code(k, name), _ptr(err_flag), _stream()), name)
+    kr, ks, kh = _rows(k, vec)
+    vr, vs, vh = _rows(v, vec)
+    _launch(_lib.load().cgpt_paged_kv_append, _lib.paged_args(
+        _ptr(qr), kr.data_ptr(), vr.data_ptr(), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(), _ptr(cu_q), 0, _ptr(rotary), 0, _ptr(err_flag), 0,
+        n, B, hq, hkv, hd, n_pages, page, cols, ts, 0, qs, qh, ks, kh, vs, vh, os_, oh, *cs,
+        rot, n_pos, rs, bool(interleaved), code, 0.0), dev, name)
     return q_out
 
 
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(n: int, B: int, hq: int, hkv: int, hd: int, page: int, cols: int, prefix: int,
                      code: int, device: int) -> int:
-    out = _lib.ctypes.c_int64()
-    _lib.check(_lib.load().cgpt_paged_attention_workspace(n, B, hq, hkv, hd, page, cols, prefix, code,
-                                                          _lib.ctypes.byref(out)), "paged_attention_workspace")
+    """The C ABI's answer for these sizes (it goes by the device's CU count too)."""
+    out = ctypes.c_int64()
+    size = dict(n_tokens=n, B=B, Hq=hq, Hkv=hkv, head_dim=hd, page_size=page, max_pages=cols, prefix_len=prefix,
+                dtype=code)
+    args = _lib.paged_args(*(size.get(f, 0) for f in _lib.PAGED_FIELDS))
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().cgpt_paged_attention_workspace(args, ctypes.byref(out)), "paged_attention_workspace")
     return out.value
 
 
@@ -203,33 +230,29 @@ def _attend(name: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
             seq_lens: torch.Tensor, prefix_len: int, prefix_pages: Optional[torch.Tensor],
             cu_q: Optional[torch.Tensor], scale: Optional[float], out: Optional[torch.Tensor],
             err_flag: Optional[torch.Tensor]) -> torch.Tensor:
-    vec = _check_cache(name, q, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
-    n, hq, hd = q.shape
-    n_pages, hkv, page, _ = k_cache.shape
+    dev, code, vec, n_pages, hkv, page, hd, cs, B, cols, ts = _check_cache(
+        name, q, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
+    n, hq, _ = q.shape
     if hq == 0 or hq % hkv:
         raise ValueError(f"{name}: n_head {hq} is not a multiple of n_kv_head {hkv}")
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
     elif not 0.0 < scale < math.inf:
         raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
-    B, cols = block_table.shape
-    if prefix_len and prefix_pages is None:
-        prefix_pages = block_table[0]
     if out is None:
-        out = torch.empty((n, hq, hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, hq, hd))
     else:
         _check_out(name, out, q, vec)
-    qr = _rows(q, vec)
-    code = _dtype_code(q, name)
-    lib = _lib.load()
-    with torch.cuda.device(q.device):
-        size = _workspace_bytes(n, B, hq, hkv, hd, page, cols, prefix_len, code, q.device.index)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _lib.check(lib.cgpt_shared_prefix_attention(
-            qr.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(),
-            seq_lens.data_ptr(), _ptr(cu_q), _ptr(prefix_pages), prefix_len, n, B, hq, hkv, hd, page, n_pages, cols,
-            block_table.stride(0), *qr.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3],
-            *v_cache.stride()[:3], float(scale), _ptr(ws), size, code, _ptr(err_flag), _stream()), name)
+    qr, qs, qh = _rows(q, vec)
+    os_, oh, _ = out.stride()
+    size = _workspace_bytes(n, B, hq, hkv, hd, page, cols, prefix_len, code, dev)
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    pages = 0 if not prefix_len else (block_table if prefix_pages is None else prefix_pages).data_ptr()
+    _launch(_lib.load().cgpt_paged_attention, _lib.paged_args(
+        qr.data_ptr(), 0, 0, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), _ptr(cu_q), pages, 0, _ptr(ws), _ptr(err_flag), size,
+        n, B, hq, hkv, hd, n_pages, page, cols, ts, prefix_len, qs, qh, 0, 0, 0, 0, os_, oh, *cs,
+        0, 0, 0, 0, code, scale), dev, name)
     return out
 
 

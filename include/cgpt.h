@@ -429,10 +429,11 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
  * block_table[b][t / page_size].  seq_lens[b] (device int32) counts its keys, those
  * of the step's tokens, its last ones, included.  The tokens are packed rows: token b
  * for sequence b (cu_q NULL, n_tokens == B), or cu_q[b] .. cu_q[b+1]-1 (B + 1 device
- * int32); rows behind cu_q[B] are neither read nor written.  Element (token, head,
- * d) of q, k, v and the outputs at base + token*st + head*sh + d, 16-byte
- * aligned.  Hq is a multiple of Hkv; head_dim is 16, 32, 64 or 128; dtype fp32, bf16
- * or fp16; n_pages * page strides may pass 32 bits; page_size * max_pages < 2^30.
+ * int32); rows behind cu_q[B] are padding, their output rows are left as they were.
+ * Element (token, head, d) of q, k, v and out at base + token*st + head*sh + d,
+ * 16-byte aligned.  Hq is a multiple of Hkv; head_dim is 16, 32, 64 or 128; dtype
+ * fp32, bf16 or fp16; offsets into the pools may pass 32 bits; page_size * max_pages
+ * < 2^30.
  *
  * Device values that are out of range fault nothing and set *err_flag (a device int,
  * may be NULL) to 1: a page id outside [0, n_pages) is not written, and read as
@@ -441,57 +442,45 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
  * 0) are skipped and set nothing.
  *
  * cgpt_paged_kv_append: k and v (Hkv heads) into their pages; with rot_dim > 0 the
- * first rot_dim values of every key, and of q (Hq heads, written to q_out, which may
+ * first rot_dim values of every key, and of q (Hq heads, written to out, which may
  * be q; both may be NULL), are turned by the token's position p: pairs (i,
  * i + rot_dim/2), or (2i, 2i+1) when interleaved, (x, y) -> (x c - y s, y c + x s) with
  * c = rotary[p][i], s = rotary[p][rot_dim/2 + i] (fp32, n_pos rows rot_stride apart), in
  * fp32 and rounded once.  Two tokens of a call must not share a slot.
  *
- * cgpt_paged_attention: o = softmax(q K^T * scale) V of every token over the keys
+ * cgpt_paged_attention: out = softmax(q K^T * scale) V of every token over the keys
  * at positions up to its own; rows without a key give zeros.  Query head h reads
  * key head h / (Hq/Hkv).  Statistics and sums are fp32; P is rounded to dtype
- * before P V, as in cgpt_attention_fwd.  cgpt_shared_prefix_attention: the same,
- * keys below prefix_len read from the pages prefix_pages (device int32) for every
- * sequence, once for all.  workspace: 16-byte aligned device memory of at least the
- * bytes that cgpt_paged_attention_workspace gives for the same sizes (prefix_len 0
- * for cgpt_paged_attention), not shared by calls that may overlap; it needs no
+ * before P V, as in cgpt_attention_fwd.  With prefix_len > 0 the keys below it are
+ * the same for all sequences and come from the pages prefix_pages (device int32); the
+ * rows' own entries for whole pages of it are not read.  workspace: 16-byte aligned
+ * device memory of at least the bytes that cgpt_paged_attention_workspace gives for
+ * the same sizes (0: none needed), not shared by calls that may overlap; it needs no
  * clearing.
  *
  * No counterpart in the reference, which keeps no cache and runs
  * cutile_causal_attention over the whole prefix for every token
  * (cutile_gpt/models/gpt.py:185-229, kernels/attention.py:24-175).
  */
-int cgpt_paged_kv_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
-                         void* v_cache, const int* block_table, const int* seq_lens,
-                         const int* cu_q, const float* rotary, int64_t n_tokens, int64_t B,
-                         int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t page_size,
-                         int64_t n_pages, int64_t max_pages, int64_t bt_stride, int64_t q_st,
-                         int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
-                         int64_t qo_st, int64_t qo_sh, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
-                         int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, int64_t rot_dim,
-                         int64_t n_pos, int64_t rot_stride, int interleaved, int dtype,
-                         int* err_flag, void* stream);
-int cgpt_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
-                         const int* block_table, const int* seq_lens, const int* cu_q,
-                         int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
-                         int64_t page_size, int64_t n_pages, int64_t max_pages, int64_t bt_stride,
-                         int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh, int64_t kc_sp,
-                         int64_t kc_sh, int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss,
-                         float scale, void* workspace, int64_t workspace_bytes, int dtype,
-                         int* err_flag, void* stream);
-int cgpt_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
-                                 const int* block_table, const int* seq_lens, const int* cu_q,
-                                 const int* prefix_pages, int64_t prefix_len, int64_t n_tokens,
-                                 int64_t B, int64_t Hq, int64_t Hkv, int64_t head_dim,
-                                 int64_t page_size, int64_t n_pages, int64_t max_pages,
-                                 int64_t bt_stride, int64_t q_st, int64_t q_sh, int64_t o_st,
-                                 int64_t o_sh, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
-                                 int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, float scale,
-                                 void* workspace, int64_t workspace_bytes, int dtype,
-                                 int* err_flag, void* stream);
-int cgpt_paged_attention_workspace(int64_t n_tokens, int64_t B, int64_t Hq, int64_t Hkv,
-                                   int64_t head_dim, int64_t page_size, int64_t max_pages,
-                                   int64_t prefix_len, int dtype, int64_t* workspace_bytes);
+typedef struct cgpt_paged_args {
+  const void *q, *k, *v;
+  void *out, *k_cache, *v_cache;
+  const int *block_table, *seq_lens, *cu_q, *prefix_pages;
+  const float* rotary;
+  void* workspace;
+  int* err_flag;
+  int64_t workspace_bytes;
+  int64_t n_tokens, B, Hq, Hkv, head_dim;
+  int64_t n_pages, page_size, max_pages, bt_stride, prefix_len;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, out_st, out_sh;
+  int64_t kc_sp, kc_sh, kc_ss, vc_sp, vc_sh, vc_ss;
+  int64_t rot_dim, n_pos, rot_stride, interleaved;
+  int64_t dtype;
+  double scale;
+} cgpt_paged_args;
+int cgpt_paged_kv_append(const cgpt_paged_args* args, void* stream);
+int cgpt_paged_attention(const cgpt_paged_args* args, void* stream);
+int cgpt_paged_attention_workspace(const cgpt_paged_args* args, int64_t* workspace_bytes);
 
 /*
  * Greedy token per row: ids[r] = argmax_c x[r * ld + c] (the first maximum;

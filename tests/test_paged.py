@@ -16,62 +16,78 @@ P = 1 << 20  # a pointer that is never followed
 
 def call(fn, **change):
     """fn of libcgpt.so on well-formed sizes with no token (nothing to launch), changed."""
-    a = dict(q=P, k=P, v=P, q_out=P, k_cache=P, v_cache=2 * P, o=P, table=P, lens=P, cu=P, rotary=P, prefix=P, prefix_len=16,
-             n=0, B=2, Hq=4, Hkv=2, hd=64, page=16, n_pages=8, cols=4, stride=4, st=256, sh=64, sp=2048, ch=1024, ss=64,
-             rot=64, n_pos=64, rs=64, scale=0.125, dtype=_lib.CGPT_BF16)
+    a = dict(q=P, k=P, v=P, out=P, k_cache=P, v_cache=2 * P, block_table=P, seq_lens=P, cu_q=P, prefix_pages=P, rotary=P,
+             workspace=0, err_flag=0, workspace_bytes=0, n_tokens=0, B=2, Hq=4, Hkv=2, head_dim=64, n_pages=8, page_size=16,
+             max_pages=4, bt_stride=4, prefix_len=16, kc_sp=2048, kc_sh=1024, kc_ss=64, vc_sp=2048, vc_sh=1024, vc_ss=64,
+             rot_dim=64, n_pos=64, rot_stride=64, interleaved=0, dtype=_lib.CGPT_BF16, scale=0.125)
+    a.update({f"{x}_{s}": n for x in ("q", "k", "v", "out") for s, n in (("st", 256), ("sh", 64))})
+    assert set(change) <= set(a) and set(a) == set(_lib.PAGED_FIELDS)
     a.update(change)
-    g = lambda *names: [a[n] for n in names]
-    sizes = g("n", "B", "Hq", "Hkv", "hd", "page", "n_pages", "cols", "stride")
-    pools = g("sp", "ch", "ss", "sp", "ch", "ss")
-    lib = _lib.load()
-    if fn == "append":
-        return lib.cgpt_paged_kv_append(*g("q", "k", "v", "q_out", "k_cache", "v_cache", "table", "lens", "cu", "rotary"), *sizes,
-                                        *g("st", "sh") * 4, *pools, *g("rot", "n_pos", "rs"), 0, a["dtype"], None, None)
-    tail = [*sizes, *g("st", "sh", "st", "sh"), *pools, a["scale"], None, 0, a["dtype"], None, None]
-    if fn == "paged":
-        return lib.cgpt_paged_attention(*g("q", "k_cache", "v_cache", "o", "table", "lens", "cu"), *tail)
-    return lib.cgpt_shared_prefix_attention(*g("q", "k_cache", "v_cache", "o", "table", "lens", "cu", "prefix", "prefix_len"), *tail)
+    args = _lib.paged_args(*(a[f] for f in _lib.PAGED_FIELDS))
+    return getattr(_lib.load(), fn)(args, None)
 
 
-EINVAL, EDTYPE, ESHAPE = -1, -2, -3
-SHARED = [(dict(n=-1), EINVAL), (dict(B=-1), EINVAL), (dict(Hq=3), EINVAL), (dict(Hkv=0), EINVAL), (dict(page=0), EINVAL),
-          (dict(n_pages=0), EINVAL), (dict(cols=-1), EINVAL), (dict(k_cache=None), EINVAL), (dict(k_cache=P + 8), EINVAL),
-          (dict(sp=2047), EINVAL), (dict(ss=32), EINVAL), (dict(ss=0), EINVAL), (dict(sp=0), EINVAL), (dict(ch=0), EINVAL),
-          (dict(dtype=7), EDTYPE), (dict(hd=48), ESHAPE), (dict(hd=256), ESHAPE), (dict(page=1 << 20, cols=1 << 11), ESHAPE),
-          (dict(n=1 << 30), ESHAPE), (dict(n_pages=1 << 31), ESHAPE)]
+EINVAL, EDTYPE, ESHAPE, ESCRATCH = -1, -2, -3, -4
+SIZES = [(dict(n_tokens=-1), EINVAL), (dict(B=-1), EINVAL), (dict(Hq=3), EINVAL), (dict(Hkv=0), EINVAL),
+         (dict(page_size=0), EINVAL), (dict(n_pages=0), EINVAL), (dict(max_pages=-1), EINVAL), (dict(bt_stride=-1), EINVAL),
+         (dict(k_cache=0), EINVAL), (dict(v_cache=P + 8), EINVAL), (dict(kc_sp=2047), EINVAL), (dict(vc_ss=32), EINVAL),
+         (dict(kc_ss=0), EINVAL), (dict(vc_sp=0), EINVAL), (dict(kc_sh=0), EINVAL), (dict(dtype=7), EDTYPE),
+         (dict(head_dim=48), ESHAPE), (dict(head_dim=256), ESHAPE), (dict(page_size=1 << 20, max_pages=1 << 11), ESHAPE),
+         (dict(n_tokens=1 << 30), ESHAPE), (dict(n_pages=1 << 31), ESHAPE)]
+FNS = ["cgpt_paged_kv_append", "cgpt_paged_attention"]
 
 
-@pytest.mark.parametrize("fn", ["append", "paged", "shared"])
+@pytest.mark.parametrize("fn", FNS)
 def test_c_entry_points_refuse(fn):
     assert call(fn) == 0
-    for change, status in SHARED:
+    assert getattr(_lib.load(), fn)(None, None) == EINVAL
+    for change, status in SIZES:
         assert call(fn, **change) == status, change
     # With a token the pointers and strides of the rows count too.
-    for change in (dict(lens=None), dict(table=None), dict(st=255), dict(cu=None)):
-        assert call(fn, n=3, **change) == EINVAL, change
+    for change in (dict(seq_lens=0), dict(block_table=0), dict(q_st=255), dict(out_sh=4), dict(out_st=8), dict(cu_q=0),
+                   dict(q=P + 8), dict(out=P + 2), dict(k_st=-8)):
+        assert call(fn, n_tokens=3, **change) == EINVAL, change
 
 
 def test_c_append_refuses():
-    for change, status in ((dict(q=None), EINVAL), (dict(v_cache=P), EINVAL), (dict(rot=3), ESHAPE), (dict(rot=66), ESHAPE),
-                           (dict(rot=-2), ESHAPE), (dict(n_pos=0), EINVAL), (dict(rs=62), EINVAL), (dict(rotary=None), EINVAL)):
-        assert call("append", **change) == status, change
-    for change in (dict(k=None), dict(v=P + 2)):
-        assert call("append", n=3, **change) == EINVAL, change
-    assert call("append", rot=0, rotary=None, q=None, q_out=None) == 0
+    fn = FNS[0]
+    for change, status in ((dict(q=0), EINVAL), (dict(v_cache=P), EINVAL), (dict(rot_dim=3), ESHAPE), (dict(rot_dim=66), ESHAPE),
+                           (dict(rot_dim=-2), ESHAPE), (dict(n_pos=0), EINVAL), (dict(rot_stride=62), EINVAL),
+                           (dict(rotary=0), EINVAL), (dict(rotary=P + 1), EINVAL)):
+        assert call(fn, **change) == status, change
+    for change in (dict(k=0), dict(v=P + 2)):
+        assert call(fn, n_tokens=3, **change) == EINVAL, change
+    assert call(fn, rot_dim=0, rotary=0, q=0, out=0) == 0
 
 
 def test_c_attention_refuses():
-    for change in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan)):
-        assert call("paged", **change) == EINVAL, change
-    for change in (dict(prefix_len=-1), dict(prefix_len=65)):
-        assert call("shared", **change) == EINVAL, change
-    assert call("shared", n=3, prefix=None) == EINVAL
-    assert call("paged", n=3, q=None) == EINVAL
-    n = ctypes.c_int64(-1)
-    lib = _lib.load()
-    assert lib.cgpt_paged_attention_workspace(4, 4, 4, 2, 64, 16, 64, 0, _lib.CGPT_BF16, ctypes.byref(n)) == 0
-    assert n.value >= 0
-    assert lib.cgpt_paged_attention_workspace(4, 4, 4, 2, 64, 16, 64, 0, _lib.CGPT_BF16, None) == EINVAL
+    fn = FNS[1]
+    for change in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e-60),
+                   dict(scale=1e60), dict(prefix_len=-1), dict(prefix_len=65)):
+        assert call(fn, **change) == EINVAL, change
+    for change in (dict(prefix_pages=0), dict(q=0), dict(out=0)):
+        assert call(fn, n_tokens=3, **change) == EINVAL, change
+    # A workspace that is missing, too small or unaligned is refused before any launch.
+    long = dict(n_tokens=2, cu_q=0, prefix_len=0, max_pages=4096, bt_stride=4096)
+    assert call(fn, **long) == ESCRATCH
+    assert call(fn, **long, workspace=P, workspace_bytes=64) == ESCRATCH
+    assert call(fn, **long, workspace=P + 8, workspace_bytes=1 << 40) == EINVAL
+
+
+def test_workspace_size():
+    lib, n = _lib.load(), ctypes.c_int64(-1)
+    size = dict(n_tokens=4, B=4, Hq=4, Hkv=2, head_dim=64, page_size=16, max_pages=4096, dtype=_lib.CGPT_BF16)
+
+    def ask(**change):
+        args = _lib.paged_args(*({**size, **change}.get(f, 0) for f in _lib.PAGED_FIELDS))
+        return lib.cgpt_paged_attention_workspace(args, ctypes.byref(n))
+
+    assert ask() == 0 and n.value > 0
+    assert ask(n_tokens=0) == 0 and n.value == 0
+    for change, status in ((dict(B=-1), EINVAL), (dict(Hq=3), EINVAL), (dict(prefix_len=-1), EINVAL), (dict(dtype=9), EDTYPE),
+                           (dict(head_dim=80), ESHAPE)):
+        assert ask(**change) == status, change
+    assert lib.cgpt_paged_attention_workspace(None, ctypes.byref(n)) == EINVAL
 
 
 def test_wrappers_refuse_host_tensors():

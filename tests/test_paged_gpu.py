@@ -133,24 +133,38 @@ def test_append_bad_device_values(gpu):
 
 # --------------------------------------------------------------------------- attention
 
+# Tables as short as the sequences, and tables for far longer ones: the kernels are
+# chosen by what the lengths may be.
+WIDE = pytest.mark.parametrize("room", [0, 5000])
+
+
+def cols(room, page):
+    return 1 + room // page
+
+
 LENS = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 300]
 
 
+@WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("hd", [16, 32, 64, 128])
-@pytest.mark.parametrize("Hq,Hkv,page", [(3, 3, 16), (8, 2, 10), (16, 1, 64)])
-def test_single_tokens(gpu, dtype, hd, Hq, Hkv, page):
+@pytest.mark.parametrize("Hq,Hkv,page", [(3, 3, 16), (8, 2, 10), (16, 1, 64), (18, 1, 16)])
+def test_single_tokens(gpu, dtype, hd, Hq, Hkv, page, room):
     """One token a sequence, every length around the tiles, an odd page and one as long as
-    a tile, one key head to one, four and sixteen query heads."""
-    check_attention(Problem(dtype, hd, page, Hq, Hkv, [n - 1 for n in LENS], [1] * len(LENS), seed=hd + Hq), gpu)
+    a tile, one key head to one, four, sixteen and eighteen query heads."""
+    check_attention(Problem(dtype, hd, page, Hq, Hkv, [n - 1 for n in LENS], [1] * len(LENS), seed=hd + Hq,
+                            spare_cols=cols(room, page)), gpu)
 
 
+@WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("hd,Hq,Hkv,page", [(16, 2, 2, 1), (32, 6, 2, 24), (64, 4, 4, 16), (128, 8, 1, 128)])
-def test_ragged_tokens(gpu, dtype, hd, Hq, Hkv, page):
+@pytest.mark.parametrize("hd,Hq,Hkv,page", [(16, 2, 2, 1), (32, 6, 2, 24), (64, 4, 4, 16), (128, 8, 1, 128), (64, 6, 2, 10)])
+@pytest.mark.parametrize("new", [[1, 150, 5, 0, 1, 70], [3, 0, 5, 1, 1, 8], [0, 0, 0, 0, 0, 200]])
+def test_ragged_tokens(gpu, dtype, hd, Hq, Hkv, page, new, room):
     """Sequences with no token, one, a few and a long prompt; rows behind the last one are
     left as they were."""
-    p = Problem(dtype, hd, page, Hq, Hkv, ctx=[10, 0, 130, 7, 0, 64], new=[1, 150, 5, 0, 1, 70], seed=hd, pad_rows=3)
+    p = Problem(dtype, hd, page, Hq, Hkv, ctx=[10, 0, 130, 7, 0, 64], new=new, seed=hd, pad_rows=3,
+                spare_cols=cols(room, page))
     out = torch.full(p.q.shape, 7.0, dtype=dtype, device=gpu)
     check_attention(p, gpu, out=out)
     assert (out[int(p.cu[-1]):] == 7.0).all()
@@ -166,32 +180,41 @@ def test_one_long_sequence(gpu, dtype, new):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("hd,Hq,Hkv,page", [(16, 4, 2, 8), (32, 3, 3, 16), (64, 5, 5, 16), (128, 8, 2, 64)])
 @pytest.mark.parametrize("prefix", [16, 129, 700])
-def test_shared_prefix(gpu, dtype, hd, Hq, Hkv, page, prefix):
+@WIDE
+def test_shared_prefix(gpu, dtype, hd, Hq, Hkv, page, prefix, room):
     prefix = -(-prefix // page) * page
     ctx = [prefix + c for c in (0, 1, 30, 64, 200)]
-    check_attention(Problem(dtype, hd, page, Hq, Hkv, ctx, [1] * 5, prefix=prefix, seed=prefix), gpu)
+    check_attention(Problem(dtype, hd, page, Hq, Hkv, ctx, [1] * 5, prefix=prefix, seed=prefix,
+                            spare_cols=cols(room, page)), gpu)
 
 
+@WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("B", [1, 33, 70])
-def test_shared_prefix_batches(gpu, dtype, B):
+@pytest.mark.parametrize("B", [1, 9, 33, 70])
+@pytest.mark.parametrize("hd,Hkv", [(64, 2), (128, 1), (32, 4)])
+def test_shared_prefix_batches(gpu, dtype, B, hd, Hkv, room):
     """More rows than a tile of the prefix holds; one sequence alone."""
-    ctx = [128 + (37 * b) % 50 for b in range(B)]
-    check_attention(Problem(dtype, 64, 32, 4, 2, ctx, [1] * B, prefix=128, seed=B), gpu)
+    ctx = [640 + (37 * b) % 50 for b in range(B)]
+    check_attention(Problem(dtype, hd, 32, 4, Hkv, ctx, [1] * B, prefix=640, seed=B, spare_cols=cols(room, 32)), gpu)
 
 
+@WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("hd", [32, 64, 128])
-def test_shared_prefix_ragged_tokens(gpu, dtype, hd):
-    p = Problem(dtype, hd, 16, 4, 4, ctx=[160, 165, 160, 200], new=[20, 1, 0, 64], prefix=160, seed=9, pad_rows=1)
+@pytest.mark.parametrize("new", [[20, 1, 0, 64], [5, 1, 0, 2], [3, 3, 3, 3]])
+def test_shared_prefix_ragged_tokens(gpu, dtype, hd, new, room):
+    p = Problem(dtype, hd, 16, 8, 4, ctx=[160, 165, 160, 200], new=new, prefix=160, seed=9, pad_rows=1,
+                spare_cols=cols(room, 16))
     check_attention(p, gpu)
 
 
-def test_shared_prefix_inside_a_page_and_short_sequences(gpu):
+@pytest.mark.parametrize("room,copies", [(0, 1), (5000, 1), (5000, 40)])
+def test_shared_prefix_inside_a_page_and_short_sequences(gpu, room, copies):
     """The prefix may end inside a page, its pages come as a list of their own; a padding
     row and sequences shorter than the prefix see what they hold."""
-    p = Problem(BF16, 64, 16, 4, 4, ctx=[160, 70, 170], new=[1, 1, 1], prefix=160, seed=10)
-    p.lens[1], p.total[1], p.ctx[1] = 71, 71, 70
+    p = Problem(BF16, 64, 16, 4, 4, ctx=[160, 70, 170] * copies, new=[1, 1, 1] * copies, prefix=160, seed=10,
+                spare_cols=cols(room, 16))
+    assert p.total[1] == 71
     want, bound = attention(p)
     d = p.on(gpu)
     got = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, 153, prefix_pages=d.table[2, :10].clone())
@@ -208,10 +231,11 @@ def test_shared_prefix_inside_a_page_and_short_sequences(gpu):
     assert torch.equal(again, got) and int(flag) == 0
 
 
+@WIDE
 @pytest.mark.parametrize("new", [1, 2, 40])
-def test_rows_without_a_key(gpu, new):
+def test_rows_without_a_key(gpu, new, room):
     """Padding rows (length 0) and tokens in front of position 0 give zeros."""
-    p = Problem(BF16, 64, 16, 2, 2, ctx=[5, 5, 5], new=[new] * 3, seed=11)
+    p = Problem(BF16, 64, 16, 2, 2, ctx=[5, 5, 5], new=[new] * 3, seed=11, spare_cols=cols(room, 16))
     p.lens[1] = 0
     p.lens[2] = p.total[2] = new // 2
     p.ctx[2] = new // 2 - new
@@ -223,10 +247,11 @@ def test_rows_without_a_key(gpu, new):
 @pytest.mark.parametrize("new", [1, 12, 90])
 @pytest.mark.parametrize("Hkv", [1, 4])
 @pytest.mark.parametrize("what", [NAN, float("inf"), -float("inf")])
-def test_masked_values_do_not_leak(gpu, dtype, new, Hkv, what):
+@WIDE
+def test_masked_values_do_not_leak(gpu, dtype, new, Hkv, what, room):
     """What a row may not see has no part in it: keys and values that later tokens of the same
     step brought, whatever they hold."""
-    p = Problem(dtype, 64, 16, 4, Hkv, ctx=[0, 21], new=[new, new], seed=12)
+    p = Problem(dtype, 64, 16, 4, Hkv, ctx=[0, 21], new=[new, new], seed=12, spare_cols=cols(room, 16))
     poison = max(0, new - 3)
     for b in range(2):
         for pos in range(p.ctx[b] + poison + 1, p.total[b]):
@@ -240,9 +265,11 @@ def test_masked_values_do_not_leak(gpu, dtype, new, Hkv, what):
         within(got[rows], want[rows], bound[rows], "rows in front of the poison")
 
 
+@WIDE
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("new", [1, 30])
-def test_value_of_a_seen_key_counts_whatever_it_is(gpu, new):
-    p = Problem(BF16, 64, 16, 2, 2, ctx=[40], new=[new], seed=13)
+def test_value_of_a_seen_key_counts_whatever_it_is(gpu, dtype, new, room):
+    p = Problem(dtype, 64, 16, 2, 2, ctx=[40], new=[new], seed=13, spare_cols=cols(room, 16))
     p.v_cache[int(p.table[0, 0]), :, 3, 9] = float("inf")
     p.v_cache[int(p.table[0, 1]), :, 3, 11] = NAN
     got = run_attention(p, gpu).float().cpu()
@@ -252,10 +279,13 @@ def test_value_of_a_seen_key_counts_whatever_it_is(gpu, new):
     within(got[:, :, rest], want[:, :, rest], bound[:, :, rest])
 
 
+@WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-def test_large_scores(gpu, dtype):
+@pytest.mark.parametrize("new", [[1, 60, 2], [1, 2, 1]])
+def test_large_scores(gpu, dtype, new, room):
     """Scores in the hundreds: the running maximum jumps from tile to tile."""
-    check_attention(Problem(dtype, 64, 16, 4, 2, ctx=[500, 3, 299], new=[1, 60, 2], seed=14, scale=5.0), gpu)
+    check_attention(Problem(dtype, 64, 16, 4, 2, ctx=[500, 3, 299], new=new, seed=14, scale=5.0,
+                            spare_cols=cols(room, 16)), gpu)
 
 
 def test_scale_and_out(gpu):
