@@ -196,6 +196,46 @@ __device__ __forceinline__ u32x2_t vt_read(const uint8_t* sv, int row, int dt, i
   return __builtin_bit_cast(u32x2_t, r);
 }
 
+// Adds the values of one key that are not finite to the rows that see it (key <=
+// lim): lane (g, frow) holds row frow's query chunks 4 ks + g and O[row][16 dt + 4 g + e];
+// nm is minus the shift of the row's weights.
+template <typename T, int HD, int QT, int NKS>
+__device__ __forceinline__ void add_odd_key(const T* k, const T* v, int key, int g, float scale_log2,
+                                            const int (&lim)[QT], const u32x4_t (&qf)[QT][NKS], const float (&nm)[QT],
+                                            f32x4_t (&o)[QT][HD / 16]) {
+  constexpr int EPC = 16 / sizeof(T), CPR = HD / EPC;
+  bool odd = false;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt)
+    for (int e = 0; e < 4; ++e) odd |= !(fabsf(Elem<T>::load(v + 16 * dt + 4 * g + e)) < INFINITY);
+  if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    float s = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = 4 * ks + g;
+      if (c < CPR) {
+        float x[EPC], y[EPC];
+        load_vec(k + c * EPC, x);
+        unpack_vec<T>(qf[qt][ks], y);
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) s = fmaf(x[e], y[e], s);
+      }
+    }
+    s = column_sum(s);
+    if (key > lim[qt]) continue;
+    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale_log2, nm[qt]));
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = Elem<T>::load(v + 16 * dt + 4 * g + e);
+        if (!(fabsf(x) < INFINITY)) o[qt][dt][e] = fmaf(p, x, o[qt][dt][e]);
+      }
+  }
+}
+
 #endif
 
 }  // namespace cgpt

@@ -1,9 +1,10 @@
 // Writing the paged key-value cache.
 //
 // append_kernel copies the step's keys and values into their pages and turns keys
-// and queries by their positions on the way.  Nothing is computed that matters: the
-// bound is the bytes (each token's k, v and q read once and written once) or, for a
-// decode step, the launch.
+// and queries by their positions on the way: (x, y) -> (x c - y s, y c + x s) in 32 bits.
+// The bound is the bytes (k, v and q of a token read once and written once) or, for a
+// decode step, the launch and three dependent loads (length, page id, row).
+#include "internal.h"
 #include "paged.h"
 
 namespace cgpt {
@@ -23,10 +24,25 @@ struct AppendArgs {
   int* err;
 };
 
-// One block per token; a thread owns element pairs of its heads.
-template <typename T>
-__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
-  const int t = blockIdx.x;
+// Four floats on a 4-byte boundary (rows of the rotation table may start anywhere).
+typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// A block holds `tokens` tokens.  A thread keeps one of a head's pairs of 16-byte chunks
+// of one token and goes through the token's heads (keys, values, queries): consecutive
+// lanes take the pairs of a head, then the next head, so a wave reads runs of a
+// projection's row, and the angles of its values stay in registers.  A pair is what a
+// rotation needs: chunks c and c + rot_dim / 2 (pairs of values a half apart), else two
+// neighbours.  PAIRS: the halves are whole chunks, or the pairs lie side by side; else
+// (rot_dim / 2 no multiple of a chunk) values are turned one by one.
+template <typename T, bool PAIRS>
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, int unit_log2, int tokens_log2) {
+  constexpr int EPV = Elem<T>::kVec;
+  const int tid = threadIdx.x;
+  const int u = tid & ((1 << unit_log2) - 1);
+  const int head_log2 = 8 - unit_log2 - tokens_log2;
+  const int h0 = (tid >> unit_log2) & ((1 << head_log2) - 1);
+  const int t = (blockIdx.x << tokens_log2) + (tid >> (unit_log2 + head_log2));
+  if (t >= a.seq.n_tokens) return;
   const int b = seq_of(a.seq, t);
   if (b >= a.seq.B) return;
   int first, count;
@@ -34,56 +50,126 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
   const int pos = a.seq.lens[b] - count + (t - first);
   if (pos < 0) return;  // a padding row
   bool bad = pos >= a.seq.cap;
-  int col = 0, slot = 0, page = 0;
+  int slot = 0, page = 0;
   if (!bad) {
-    col = a.seq.page.div(pos);
+    const int col = a.seq.page.div(pos);
     slot = pos - col * static_cast<int>(a.seq.page.d);
     page = page_of(a.seq.table + b * a.seq.stride, col, a.seq.n_pages, &bad);
   }
-  int at = pos;
-  bool off = false;
-  if (a.rot_dim > 0 && pos >= a.n_pos) {
-    off = true;
-    at = a.n_pos - 1;
+  const int half = a.rot_dim / 2;
+  const bool off = half > 0 && pos >= a.n_pos;
+  if ((bad || off) && a.err != nullptr) *a.err = 1;
+  const float* cs = a.rot + (off ? a.n_pos - 1 : pos) * a.rot_stride;
+
+  // The thread's two chunks (first value of each), and how its values are turned.
+  const int rh = half / EPV;
+  const bool apart = PAIRS && !a.interleaved && u < rh;
+  const int x0 = (apart ? u : 2 * u) * EPV;
+  const int x1 = apart ? x0 + half : x0 + EPV;
+  float c[EPV], sn[EPV];
+  if (PAIRS) {
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) {
+      c[e] = 1.f;
+      sn[e] = 0.f;
+    }
+    if (apart) {
+#pragma unroll
+      for (int e = 0; e < EPV; e += 4) {
+        const f32x4u_t cv = *reinterpret_cast<const f32x4u_t*>(cs + x0 + e);
+        const f32x4u_t sv = *reinterpret_cast<const f32x4u_t*>(cs + half + x0 + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[e + i] = cv[i];
+          sn[e + i] = sv[i];
+        }
+      }
+    } else if (a.interleaved) {
+      // Angle e belongs to values x0 + 2 e, x0 + 2 e + 1 of the two neighbours.
+#pragma unroll
+      for (int e = 0; e < EPV; ++e)
+        if (x0 / 2 + e < half) {
+          c[e] = cs[x0 / 2 + e];
+          sn[e] = cs[half + x0 / 2 + e];
+        }
+    }
   }
-  if ((bad || off) && a.err != nullptr && threadIdx.x == 0) *a.err = 1;
-  const float* cs = a.rot + at * a.rot_stride;
-  const int half = a.rot_dim / 2, pairs = a.head_dim / 2;
-  auto turn = [&](const T* src, T* dst, int i) {
-    int x = 2 * i, y = 2 * i + 1;
-    if (i < half && !a.interleaved) x = i, y = i + half;
-    const float u = Elem<T>::load(src + x), w = Elem<T>::load(src + y);
-    if (i < half) {
-      const float c = cs[i], s = cs[half + i];
-      Elem<T>::store(dst + x, u * c - w * s);
-      Elem<T>::store(dst + y, w * c + u * s);
+  const int heads = 2 * a.Hkv + (a.q != nullptr ? a.Hq : 0);
+  for (int h = h0; h < heads; h += 1 << head_log2) {
+    const T* src;
+    T* dst;
+    bool turned = true;
+    if (h < 2 * a.Hkv) {
+      if (bad) continue;
+      const bool is_v = h >= a.Hkv;
+      const int hk = is_v ? h - a.Hkv : h;
+      turned = !is_v;
+      src = is_v ? static_cast<const T*>(a.v) + t * a.v_st + hk * a.v_sh : static_cast<const T*>(a.k) + t * a.k_st + hk * a.k_sh;
+      dst = is_v ? static_cast<T*>(a.vc.base) + page * a.vc.sp + hk * a.vc.sh + slot * a.vc.ss
+                 : static_cast<T*>(a.kc.base) + page * a.kc.sp + hk * a.kc.sh + slot * a.kc.ss;
     } else {
-      dst[x] = src[x];
-      dst[y] = src[y];
+      src = static_cast<const T*>(a.q) + t * a.q_st + (h - 2 * a.Hkv) * a.q_sh;
+      dst = static_cast<T*>(a.q_out) + t * a.qo_st + (h - 2 * a.Hkv) * a.qo_sh;
     }
-  };
-  if (!bad)
-    for (int i = threadIdx.x; i < a.Hkv * pairs; i += kAppendThreads) {
-      const int h = i / pairs, p = i % pairs;
-      const T* ks = static_cast<const T*>(a.k) + t * a.k_st + h * a.k_sh;
-      const T* vs = static_cast<const T*>(a.v) + t * a.v_st + h * a.v_sh;
-      T* kd = static_cast<T*>(a.kc.base) + page * a.kc.sp + h * a.kc.sh + slot * a.kc.ss;
-      T* vd = static_cast<T*>(a.vc.base) + page * a.vc.sp + h * a.vc.sh + slot * a.vc.ss;
-      turn(ks, kd, p);
-      vd[2 * p] = vs[2 * p];
-      vd[2 * p + 1] = vs[2 * p + 1];
+    if (PAIRS) {
+      u32x4_t r0 = *reinterpret_cast<const u32x4_t*>(src + x0), r1 = *reinterpret_cast<const u32x4_t*>(src + x1);
+      if (turned && (apart || a.interleaved) && half > 0) {
+        float x[2 * EPV], y[2 * EPV];
+        unpack_vec<T>(r0, x);
+        unpack_vec<T>(r1, x + EPV);
+        if (apart) {
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) {
+            y[e] = x[e] * c[e] - x[EPV + e] * sn[e];
+            y[EPV + e] = x[EPV + e] * c[e] + x[e] * sn[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) {
+            const bool in = x0 / 2 + e < half;  // values past rot_dim go over as they are
+            y[2 * e] = in ? x[2 * e] * c[e] - x[2 * e + 1] * sn[e] : x[2 * e];
+            y[2 * e + 1] = in ? x[2 * e + 1] * c[e] + x[2 * e] * sn[e] : x[2 * e + 1];
+          }
+        }
+        store_vec(dst + x0, y);
+        store_vec(dst + x1, y + EPV);
+      } else {
+        *reinterpret_cast<u32x4_t*>(dst + x0) = r0;
+        *reinterpret_cast<u32x4_t*>(dst + x1) = r1;
+      }
+    } else {
+      // Values 2 u EPV .. + 2 EPV of the pairs' order: the turned pairs, then the rest.
+      for (int e = 0; e < EPV; ++e) {
+        const int i = u * EPV + e;  // pair i < half is (i, i + half), pair i >= half (2 i, 2 i + 1)
+        const int p0 = i < half ? i : 2 * i, p1 = i < half ? i + half : 2 * i + 1;
+        if (turned && i < half) {
+          const float x = Elem<T>::load(src + p0), y = Elem<T>::load(src + p1);
+          Elem<T>::store(dst + p0, x * cs[i] - y * cs[half + i]);
+          Elem<T>::store(dst + p1, y * cs[i] + x * cs[half + i]);
+        } else {
+          const T v0 = src[p0], v1 = src[p1];
+          dst[p0] = v0;
+          dst[p1] = v1;
+        }
+      }
     }
-  if (a.q != nullptr)
-    for (int i = threadIdx.x; i < a.Hq * pairs; i += kAppendThreads) {
-      const int h = i / pairs, p = i % pairs;
-      turn(static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh,
-           static_cast<T*>(a.q_out) + t * a.qo_st + h * a.qo_sh, p);
-    }
+  }
 }
 
 template <typename T>
 static int launch_append(const AppendArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(append_kernel<T>, dim3(static_cast<unsigned>(a.seq.n_tokens)), dim3(kAppendThreads), 0, s, a);
+  constexpr int EPV = Elem<T>::kVec;
+  int unit_log2 = 0;
+  while ((2 * EPV << unit_log2) < a.head_dim) ++unit_log2;
+  // As many tokens a block as leave eight blocks a CU, so that a wave's writes into a
+  // page run over neighbouring slots; a decode step gives each token a block.
+  int tokens_log2 = 0;
+  while (tokens_log2 < 8 - unit_log2 && (a.seq.n_tokens >> (tokens_log2 + 1)) >= 8 * num_cus()) ++tokens_log2;
+  const unsigned blocks = static_cast<unsigned>((a.seq.n_tokens + (1 << tokens_log2) - 1) >> tokens_log2);
+  if (a.interleaved || (a.rot_dim / 2) % EPV == 0)
+    hipLaunchKernelGGL((append_kernel<T, true>), dim3(blocks), dim3(kAppendThreads), 0, s, a, unit_log2, tokens_log2);
+  else
+    hipLaunchKernelGGL((append_kernel<T, false>), dim3(blocks), dim3(kAppendThreads), 0, s, a, unit_log2, tokens_log2);
   return hip_status(hipGetLastError());
 }
 

@@ -266,6 +266,7 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     const T* const vh = static_cast<const T*>(a.vc.base) + hk * a.vc.sh;
     const int sub0 = base0 + t0 * UK + wave * KT;  // first subtile; the next is UK further
     const int cnt = sub0 < n ? min(t1 - t0, (n - sub0 + UK - 1) / UK) : 0;
+    int odd_from = 0x7fffffff;  // first masked key tile of the wave with a value that is not finite
     u32x4_t kf[NT][NKS], vf[NT][NKS];
     // Pages of subtile i: one a 16-key tile, or one a lane's key.
     auto fetch = [&](int i, int (&pg)[NT]) __attribute__((always_inline)) {
@@ -309,12 +310,36 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
       return sv + key * C::KROW + (((4 * ks + g) ^ vswz<T, C::CPR>(key)) << 4);
     };
     auto compute = [&](int base, const u32x4_t (&kd)[NT][NKS], const u32x4_t (&vd)[NT][NKS]) __attribute__((always_inline)) {
+      bool masked = base < kb;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+        if (qt < nqt) masked |= __builtin_amdgcn_ballot_w64(lim[qt] < base + KT - 1) != 0;
       asm volatile("" ::: "memory");
+      if (!masked) {
 #pragma unroll
-      for (int kt = 0; kt < NT; ++kt)
+        for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
-          if (C::has(ks, g)) *reinterpret_cast<u32x4_t*>(v_slot(kt, ks)) = vd[kt][ks];
+          for (int ks = 0; ks < NKS; ++ks)
+            if (C::has(ks, g)) *reinterpret_cast<u32x4_t*>(v_slot(kt, ks)) = vd[kt][ks];
+      } else {
+        // A masked key's weight is 0, but 0 x NaN is NaN: where a row is masked the matrix
+        // cores get the finite values alone, and the others are added at the item's end to
+        // the rows that see them.
+        uint32_t bits = 0;
+#pragma unroll
+        for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+          for (int ks = 0; ks < NKS; ++ks) {
+            u32x4_t v = vd[kt][ks];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              bits |= special_bits<T>(v[e]);
+              v[e] = finite_part<T>(v[e]);
+            }
+            if (C::has(ks, g)) *reinterpret_cast<u32x4_t*>(v_slot(kt, ks)) = v;
+          }
+        if (__builtin_amdgcn_ballot_w64((bits & 0x80008000u) != 0) != 0) odd_from = min(odd_from, base);
+      }
       asm volatile("" ::: "memory");
       f32x4_t s[QT][NT];
 #pragma unroll
@@ -328,12 +353,10 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
           for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) Mfma<T>::run(kd[kt][ks], qf[qt][ks], s[qt][kt]);
-      bool masked = false;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
         if (qt < nqt) {
-          if (base < kb || __builtin_amdgcn_ballot_w64(lim[qt] < base + KT - 1) != 0) {
-            masked = true;
+          if (masked) {
             const int hi = lim[qt] - base - 4 * g, lo = kb - base - 4 * g;
 #pragma unroll
             for (int kt = 0; kt < NT; ++kt)
@@ -372,66 +395,6 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
             }
           l_run[qt] += sum;
         }
-      // A masked key's weight is 0, but 0 x NaN is NaN.  Where a masked subtile holds values
-      // that are not finite, those are added here, key by key, to the rows that see them,
-      // and the matrix cores get the finite ones.
-      if (masked) {
-        uint32_t odd[NT], any = 0;
-#pragma unroll
-        for (int kt = 0; kt < NT; ++kt) {
-          uint32_t bits = 0;
-#pragma unroll
-          for (int ks = 0; ks < NKS; ++ks)
-            if (C::has(ks, g)) {
-              const u32x4_t v = *reinterpret_cast<const u32x4_t*>(v_slot(kt, ks));
-#pragma unroll
-              for (int e = 0; e < 4; ++e) bits |= special_bits<T>(v[e]);
-            }
-          const uint64_t m = __builtin_amdgcn_ballot_w64((bits & 0x80008000u) != 0);
-          odd[kt] = static_cast<uint32_t>(m | m >> 16 | m >> 32 | m >> 48) & 0xffffu;
-          any |= odd[kt];
-        }
-        if (__builtin_expect(any != 0, 0)) {
-#pragma unroll 1
-          for (int j = 0; j < KT; ++j) {
-            uint32_t bits = 0;
-#pragma unroll
-            for (int kt = 0; kt < NT; ++kt) bits = kt == j >> 4 ? odd[kt] : bits;
-            if (!((bits >> (j & 15)) & 1)) continue;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              float p = 0.f;
-#pragma unroll
-              for (int kt = 0; kt < NT; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p = kt == j >> 4 && r == (j & 3) ? s[qt][kt][r] : p;
-              p = __shfl(p, (j & 12) * 4 + frow, 64);
-              const bool seen = base + j <= lim[qt] && base + j >= kb;
-#pragma unroll
-              for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int d = 16 * dt + 4 * g + e;
-                  const float v = Elem<T>::load(reinterpret_cast<const T*>(
-                      sv + j * C::KROW + (((d / C::EPC) ^ vswz<T, C::CPR>(j)) << 4)) + d % C::EPC);
-                  if (seen && !(fabsf(v) < INFINITY)) o[qt][dt][e] = fmaf(p, v, o[qt][dt][e]);
-                }
-            }
-          }
-#pragma unroll
-          for (int kt = 0; kt < NT; ++kt)
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks)
-              if (C::has(ks, g)) {
-                u32x4_t* const v = reinterpret_cast<u32x4_t*>(v_slot(kt, ks));
-                u32x4_t w = *v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = finite_part<T>(w[e]);
-                *v = w;
-              }
-          asm volatile("" ::: "memory");
-        }
-      }
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int c = 0; c < NT / 2; ++c) {
@@ -497,6 +460,29 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
             kf[kt][ks] = kn[kt][ks];
             vf[kt][ks] = vn[kt][ks];
           }
+      }
+    }
+
+    // ---- values that are not finite in masked subtiles: key by key, rarely
+    if (__builtin_expect(odd_from < n, 0)) {
+      float nm[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) nm[qt] = m_run[qt] == -INFINITY ? 0.f : -m_run[qt];
+      for (int i = 0; i < cnt; ++i) {
+        const int base = sub0 + i * UK;
+        // Subtiles that no row was masked in have their values in O already.
+        bool masked = base < kb;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+          if (qt < nqt) masked |= __builtin_amdgcn_ballot_w64(lim[qt] < base + KT - 1) != 0;
+        if (!masked) continue;
+        for (int key = max(base, kb); key < min(base + KT, n); ++key) {
+          const int slot = key - a.seq.page.div(key) * page_size;
+          int p = (WHOLE && key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
+          if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) p = 0;
+          add_odd_key<T, HD, QT>(kh + p * a.kc.sp + slot * a.kc.ss, vh + p * a.vc.sp + slot * a.vc.ss, key, g,
+                                 a.scale_log2, lim, qf, nm, o);
+        }
       }
     }
 
@@ -698,7 +684,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     return CGPT_OK;
   }
   const bool tile_ok = paged_tile_ok(call.dtype, HD);
-  p->flat = tile_ok && prefix_len > 0 && rows > 64 && rows <= 16 * B;
+  p->flat = tile_ok && prefix_len > 0 && rows > 16 && rows <= 16 * B;
   p->tile = p->flat || (tile_ok && rows > 16 * B);
   if (p->tile) {
     // 128-row tiles where they fill the card, else 64; then the keys split until the card
@@ -706,9 +692,9 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     const int64_t keys = p->flat ? prefix_len : cap;
     auto blocks = [&](int64_t bq) { return Hkv * (p->flat ? (rows + bq - 1) / bq : rows / bq + B); };
     p->tile_qt = blocks(128) >= 4 * cus || (p->flat && rows > 64) ? 2 : 1;
-    const int64_t n = blocks(64 * p->tile_qt);
-    p->n_split = static_cast<int>(std::max<int64_t>(1, std::min((3 * cus + n - 1) / n, keys / 256)));
-    if (!p->flat && n >= 2 * cus) p->n_split = 1;
+    const int64_t n = blocks(64 * p->tile_qt), fit = (HD == 64 ? (p->tile_qt == 2 ? 3 : 4) : 2) * cus;
+    p->n_split = static_cast<int>(std::max<int64_t>(1, std::min(fit / n, keys / 256)));
+    if (!p->flat && n >= cus) p->n_split = 1;
     if (n * p->n_split > 0x7fffffff) return CGPT_ESHAPE;
     const bool parts = p->flat || p->n_split > 1;
     p->o_tml = take(parts ? p->n_split * n_tokens * Hq * 8 : 0);

@@ -162,6 +162,7 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   wait_vmcnt<0>();
 
   const int tr_row = 4 * g + (frow >> 2);
+  int odd_from = 0x7fffffff;  // first masked block of keys with a value that is not finite
   for (int j = j0; j < j1; ++j) {
     raw_barrier();
     const uint8_t* sk = smem + ((j - j0) & 1) * STAGE;
@@ -246,46 +247,10 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
           for (int r = 0; r < 4; ++r) s[qt][kt][r] = p[kt][r];
         l_run[qt] += sum;
       }
-      // Values that are not finite at keys some row does not see (0 x NaN is NaN): added
-      // here, key by key, to the rows that see them, and taken out of the operand below.
-      bool odd = false;
-      if (masked) {
-        uint64_t keys = 0;
-#pragma unroll 1
-        for (int k8 = 0; k8 < BKV; k8 += RPI) {
-          const u32x4_t v = *reinterpret_cast<const u32x4_t*>(sv + (k8 + lrow) * KROW + (slot16 << 4));
-          const uint32_t bits = special_bits<T>(v[0]) | special_bits<T>(v[1]) | special_bits<T>(v[2]) | special_bits<T>(v[3]);
-          const uint64_t m = __builtin_amdgcn_ballot_w64((bits & 0x80008000u) != 0);
-          for (int k = 0; k < RPI; ++k)
-            if ((m >> (k * CPR)) & ((uint64_t{1} << CPR) - 1)) keys |= uint64_t{1} << (k8 + k);
-        }
-        odd = keys != 0;
-        if (__builtin_expect(odd, 0)) {
-#pragma unroll 1
-          for (int k = 0; k < BKV; ++k) {
-            if (!((keys >> k) & 1)) continue;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              float p = 0.f;
-#pragma unroll
-              for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p = kt == k >> 4 && r == (k & 3) ? s[qt][kt][r] : p;
-              p = __shfl(p, (k & 12) * 4 + frow, 64);
-              const bool seen = base + k <= lim[qt];
-#pragma unroll
-              for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int d = 16 * dt + 4 * g + e;
-                  const float v = Elem<T>::load(
-                      reinterpret_cast<const T*>(sv + k * KROW + (((d >> 3) ^ (k & 7)) << 4)) + (d & 7));
-                  if (seen && !(fabsf(v) < INFINITY)) o[qt][dt][e] = fmaf(p, v, o[qt][dt][e]);
-                }
-            }
-          }
-        }
-      }
+      // A masked key's weight is 0, but 0 x NaN is NaN: where a row is masked the matrix
+      // cores get the finite values alone, and the others are added after the loop to
+      // the rows that see them.
+      uint32_t bits = 0;
       auto pv = [&](auto clean) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -302,18 +267,37 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
             u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
             if constexpr (decltype(clean)::value)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = finite_part<T>(w[e]);
+              for (int e = 0; e < 4; ++e) {
+                bits |= special_bits<T>(w[e]);
+                w[e] = finite_part<T>(w[e]);
+              }
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(w, pf[qt], o[qt][dt]);
           }
         }
       };
-      if (__builtin_expect(odd, 0))
+      if (masked) {
         pv(std::true_type{});
-      else
+        if (__builtin_amdgcn_ballot_w64((bits & 0x80008000u) != 0) != 0) odd_from = min(odd_from, j);
+      } else {
         pv(std::false_type{});
+      }
     }
     if (j + 1 < j1) wait_vmcnt<0>();
+  }
+
+  // ---- values that are not finite in masked blocks: key by key, rarely
+  if (__builtin_expect(odd_from < j1, 0)) {
+    // (Rows past a block see it whole and have counted it already only where it was not
+    // masked for any row of the wave: the blocks from the first masked one on all are.)
+    for (int key = odd_from * BKV; key < min(n, j1 * BKV); ++key) {
+      const int slot = key - a.seq.page.div(key) * page_size;
+      int p = (FLAT || key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
+      if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) p = 0;
+      const T* kr = reinterpret_cast<const T*>(kh) + p * a.kc.sp + slot * a.kc.ss;
+      const T* vr = reinterpret_cast<const T*>(vh) + p * a.vc.sp + slot * a.vc.ss;
+      add_odd_key<T, HD, QT>(kr, vr, key, g, a.scale_log2, lim, qf, nm, o);
+    }
   }
 
   // ---- out: lane holds O[row][16 dt + 4 g .. +3]

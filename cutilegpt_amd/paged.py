@@ -43,7 +43,6 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .kernels import _require_gpu
 
 __all__ = ["rotary_table", "paged_kv_append", "paged_attention", "shared_prefix_attention"]
 
@@ -93,12 +92,15 @@ def _check_cache(name: str, x: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                  err_flag: Optional[torch.Tensor]):
     """Checks what every entry point takes; returns the rows' device index, the dtype's
     code, the elements in 16 bytes, the caches' sizes and strides and the table's sizes."""
-    _require_gpu(name, x, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
-    dev, dt = x.get_device(), x.dtype
-    if (k_cache.get_device() != dev or v_cache.get_device() != dev or block_table.get_device() != dev
-            or seq_lens.get_device() != dev or (cu_q is not None and cu_q.get_device() != dev)
-            or (err_flag is not None and err_flag.get_device() != dev)):
-        raise ValueError(f"{name}: every tensor must be on {x.device}")
+    try:
+        dev, dt = x.get_device(), x.dtype
+        same = (dev == k_cache.get_device() == v_cache.get_device() == block_table.get_device()
+                == seq_lens.get_device() and (cu_q is None or cu_q.get_device() == dev)
+                and (err_flag is None or err_flag.get_device() == dev))
+    except AttributeError:
+        same, dev = False, -1
+    if not same or dev < 0:
+        raise ValueError(f"{name}: tensors must be torch tensors on one GPU")
     code = _CODE.get(dt)
     if code is None:
         raise ValueError(f"{name}: unsupported dtype {dt} (float32, bfloat16 or float16)")
@@ -147,7 +149,7 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 def _launch(fn, args: bytes, dev: int, name: str) -> None:
     """One native call on the rows' device, on its current stream."""
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         rc = fn(args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
@@ -172,7 +174,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     name = "paged_kv_append"
     dev, code, vec, n_pages, hkv, page, hd, cs, B, cols, ts = _check_cache(
         name, k, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)
-    _require_gpu(name, v, q, rotary)
+    if not all(t is None or isinstance(t, torch.Tensor) for t in (v, q, rotary)):
+        raise ValueError(f"{name}: k, v, q and rotary must be torch tensors")
     n = k.shape[0]
     if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != dev or k.shape[1] != hkv:
         raise ValueError(f"{name}: k and v must be {k.dtype} (n_tokens, {hkv}, {hd}) rows, got "
@@ -286,14 +289,15 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     name = "shared_prefix_attention"
     if isinstance(prefix_len, bool) or not isinstance(prefix_len, int) or prefix_len < 0:
         raise ValueError(f"{name}: prefix_len must be an int >= 0, got {prefix_len!r}")
-    _require_gpu(name, q, k_cache, block_table, prefix_pages)
+    if not all(isinstance(t, torch.Tensor) for t in (q, k_cache, block_table)):
+        raise ValueError(f"{name}: tensors must be torch tensors on one GPU")
     if k_cache.dim() == 4 and block_table.dim() == 2:
         page = k_cache.shape[2]
         if prefix_len > page * block_table.shape[1]:
             raise ValueError(f"{name}: prefix_len {prefix_len} exceeds the {block_table.shape[1]} pages of a "
                              f"block_table row")
         if prefix_pages is not None and (
-                prefix_pages.dim() != 1 or prefix_pages.dtype != torch.int32 or prefix_pages.device != q.device
+                not isinstance(prefix_pages, torch.Tensor) or prefix_pages.dim() != 1 or prefix_pages.dtype != torch.int32 or prefix_pages.device != q.device
                 or not prefix_pages.is_contiguous() or prefix_pages.shape[0] * page < prefix_len):
             raise ValueError(f"{name}: prefix_pages must be a contiguous int32 list of at least "
                              f"{-(-prefix_len // max(page, 1))} pages on {q.device}")
