@@ -46,20 +46,25 @@ __device__ __forceinline__ SeqUnits seq_units(const PagedAttnArgs& a, int b) {
   u.n = u.count > 0 ? min(u.len, a.seq.cap) : 0;
   u.kb = a.prefix_len;
   u.base0 = u.kb & ~15;
-  u.rt = (u.count * (a.Hq / a.Hkv) + R - 1) / R;
+  u.rt = (u.count * static_cast<int>(a.group.d) + R - 1) / R;
   u.kt = u.n > u.kb ? (u.n - u.base0 + UK - 1) / UK : 0;
   return u;
 }
 
-// Blocks that share U units, and the block that owns unit u when block i owns
-// [i U / g, (i + 1) U / g).
-__device__ __forceinline__ int active_blocks(int grid, int U) { return min(grid, max(U, 1)); }
-__device__ __forceinline__ int unit_start(int i, int U, int g) {
-  return static_cast<int>(static_cast<int64_t>(i) * U / g);
-}
-__device__ __forceinline__ int unit_owner(int u, int U, int g) {
-  return static_cast<int>(((static_cast<int64_t>(u) + 1) * g - 1) / U);
-}
+// U units dealt to at most `grid` blocks: the first r blocks have q + 1, the rest q.
+struct Deal {
+  int g, q, r;
+  __device__ Deal(int grid, int U) {
+    g = min(grid, max(U, 1));
+    q = U / g;
+    r = U - q * g;
+  }
+  __device__ int start(int block) const { return block * q + min(block, r); }
+  __device__ int owner(int u) const {
+    const int t = r * (q + 1);
+    return u < t ? u / (q + 1) : r + (u - t) / q;
+  }
+};
 
 // The workspace: unit starts of the sequences; the two edge partials of every block
 // (2 x R rows each); with a prefix also one partial a row for the items that one block
@@ -74,7 +79,7 @@ struct PagedWs {
   float* tile_o;     // splits x n_tokens x Hq x HD
 };
 
-template <typename T, int HD, int QTW, int NW = 4>
+template <typename T, int HD, int QTW, int NW>
 struct StreamShape {
   static constexpr int ES = sizeof(T);
   static constexpr int EPC = 16 / ES;              // elements of a 16-byte chunk
@@ -83,7 +88,9 @@ struct StreamShape {
   static constexpr int KSTEP = 4 * EPC;            // head_dim of one k-slab
   static constexpr int NKS = (HD + KSTEP - 1) / KSTEP;
   static constexpr int ND = HD / 16;
-  static constexpr int NT = (ES == 2 ? 2 : 1) * (HD >= 64 ? 1 : 2);  // 16-key tiles a wave takes at once
+  // 16-key tiles a wave takes at once: 8 KiB of K and V, 16 KiB for the lone wave, which
+  // has the registers for it (and at head_dim 128).
+  static constexpr int NT = (ES == 2 ? 2 : 1) * (HD >= 64 ? 1 : 2) * (NW == 1 ? 2 : 1);
   static constexpr int KT = 16 * NT;
   static constexpr int UK = NW * KT;               // keys of a unit, KT a wave
   static constexpr int QT = QTW, R = 16 * QTW;
@@ -95,7 +102,12 @@ struct StreamShape {
   static_assert(VBYTES >= 16 * HD * 4, "the join of the waves reuses the V tiles");
 };
 
-constexpr int kStreamThreads = 256, kStreamWaves = 4;
+// Waves of a block with one row tile: lone waves need no join of the four and take
+// twice the keys at once (64 sequences x 25 heads of head_dim 64: 256 keys 39 -> 33 us,
+// 1024 keys 97 -> 88, 8192 keys 578 -> 569); at head_dim 128 four of them read a page's
+// rows together (128 x 8 heads, 2048 keys: 201 us alone, 192 together).
+constexpr int stream_waves(int hd) { return hd == 128 ? 4 : 1; }
+constexpr int kJoinThreads = 256;
 
 // Each wave streams keys by itself: K and V rows go from their pages into registers,
 // one subtile of KT keys ahead of the one in use, in the layout of the matrix cores' A
@@ -110,7 +122,7 @@ constexpr int kStreamThreads = 256, kStreamWaves = 4;
 // A16: 16 keys from a multiple of 16 on lie in one page (and on one side of the prefix's
 // end), whose id comes by a scalar load; else every lane looks its own key up.
 template <typename T, int HD, int QTW, bool A16, int NW, bool WHOLE>
-__global__ __launch_bounds__(64 * NW, NW == 4 && HD * QTW <= 64 && QTW == 1 ? 4 : NW == 16 ? 4 : 2) void
+__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void
 paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
   using C = StreamShape<T, HD, QTW, NW>;
   constexpr int QT = C::QT, NT = C::NT, NKS = C::NKS, ND = C::ND, KT = C::KT, UK = C::UK, R = C::R;
@@ -119,7 +131,7 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int g = lane >> 4, frow = lane & 15;
-  const int G = a.Hq / a.Hkv, page_size = static_cast<int>(a.seq.page.d);
+  const int G = static_cast<int>(a.group.d), page_size = static_cast<int>(a.seq.page.d);
   uint8_t* const sv = smem + wave * C::VBYTES;
   bool bad = false;
 
@@ -141,8 +153,52 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     }
     total = __builtin_amdgcn_readlane(incl, 63);
   };
-  int u = 0, u_end = 1;
-  if constexpr (!WHOLE) {
+  // The item at hand: rows of tile rt of key head hk, keys [kb, n), cut into kt_item units
+  // from base0 on; t0 is its first unit here.
+  int u = 0, u_end = 1, hk = 0, rt = 0, rts = 1, t0 = 0, kt_item = 0, kb = 0, base0 = 0, n_all = 0, rows = 0, first = 0,
+      pos0 = 0;
+  bool prefix = false;
+  const int* trow = nullptr;
+  // The sequence whose units u lies in; false when there is none (the lengths changed
+  // under the call).
+  auto enter_sequence = [&]() __attribute__((always_inline)) {
+    while (u >= before + total) {
+      if (c0 + 64 >= a.seq.B) return false;
+      before += total;
+      load_chunk(c0 + 64);
+    }
+    const int at = __popcll(__builtin_amdgcn_ballot_w64(before + incl <= u));
+    auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
+    prefix = false;
+    rts = of(mine.rt);
+    kt_item = of(mine.kt);
+    t0 = u - before - of(incl - n_units);  // units into the sequence
+    n_all = of(mine.n);
+    first = of(mine.first);
+    const int count = of(mine.count), len = of(mine.len);
+    rows = count * G;
+    pos0 = len - count;
+    kb = a.prefix_len;
+    base0 = kb & ~15;
+    trow = a.seq.table + (c0 + at) * a.seq.stride;
+    bad |= len > a.seq.cap;
+    return true;
+  };
+  if constexpr (WHOLE) {
+    rt = static_cast<int>(blockIdx.x) / a.Hkv;
+    hk = static_cast<int>(blockIdx.x) - rt * a.Hkv;
+    const int b = slot_seq<R>(a.seq, G, lane, &rt);
+    if (b >= a.seq.B) return;
+    int count;
+    seq_tokens(a.seq, b, &first, &count);
+    rows = count * G;
+    if (rt < 0 || rt * R >= rows) return;
+    const int len = max(a.seq.lens[b], 0);
+    n_all = min(len, a.seq.cap);
+    pos0 = len - count;
+    trow = a.seq.table + b * a.seq.stride;
+    bad = len > a.seq.cap;
+  } else {
     int U = prefix_units;
     for (int c = 0; c < a.seq.B; c += 64) {
       load_chunk(c);
@@ -151,76 +207,35 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     }
     if (blockIdx.x == 0 && tid == 0) ws.starts[a.seq.B] = U;
     if (a.seq.B > 64) load_chunk(0);
-    const int gblocks = active_blocks(gridDim.x, U);
-    if (static_cast<int>(blockIdx.x) >= gblocks || U == 0) return;
-    u = unit_start(blockIdx.x, U, gblocks);
-    u_end = unit_start(blockIdx.x + 1, U, gblocks);
+    const Deal deal(gridDim.x, U);
+    if (static_cast<int>(blockIdx.x) >= deal.g || U == 0) return;
+    u = deal.start(blockIdx.x);
+    u_end = deal.start(blockIdx.x + 1);
+    if (u < prefix_units) {
+      prefix = true;
+      kt_item = (a.prefix_len + UK - 1) / UK;
+      rows = a.seq.n_tokens * G;
+      rts = (rows + R - 1) / R;
+      n_all = a.prefix_len;
+      trow = a.prefix;
+      t0 = u;
+    } else if (!enter_sequence()) {
+      return;
+    }
+    const int item = t0 / kt_item;
+    t0 -= item * kt_item;
+    hk = item / rts;
+    rt = item - hk * rts;
   }
 
-  while (u < u_end) {
+  for (;;) {
     // Addresses are made anew for every item: kept over the loop they cost registers that
     // the loads in flight need.
     asm volatile("" : "+v"(g), "+v"(frow));
-    // ---- the item that unit u lies in
-    const bool prefix = !WHOLE && u < prefix_units;
-    int hk, rt, t0 = 0, kt_item, n, kb = 0, base0 = 0, rows, first = 0, pos0 = 0;
-    const int* trow;
-    if (prefix) {
-      kt_item = (a.prefix_len + UK - 1) / UK;
-      rows = a.seq.n_tokens * G;
-      const int rts = (rows + R - 1) / R;
-      const int item = u / kt_item;
-      t0 = u - item * kt_item;
-      hk = item / rts;
-      rt = item - hk * rts;
-      n = a.prefix_len;
-      trow = a.prefix;
-    } else {
-      int b, len, count, n_all;
-      if constexpr (WHOLE) {
-        const int tile = static_cast<int>(blockIdx.x) / a.Hkv;
-        hk = static_cast<int>(blockIdx.x) - tile * a.Hkv;
-        rt = tile;
-        b = slot_seq<R>(a.seq, G, lane, &rt);
-        if (b >= a.seq.B) return;
-        seq_tokens(a.seq, b, &first, &count);
-        len = max(a.seq.lens[b], 0);
-        n_all = min(len, a.seq.cap);
-        rows = count * G;
-        if (rt < 0 || rt * R >= rows) return;
-      } else {
-        while (u >= before + total) {
-          if (c0 + 64 >= a.seq.B) return;  // the lengths changed under the call
-          before += total;
-          load_chunk(c0 + 64);
-        }
-        const int at = __popcll(__builtin_amdgcn_ballot_w64(before + incl <= u));
-        auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
-        b = c0 + at;
-        const int rts = of(mine.rt);
-        const int rel = u - before - of(incl - n_units);
-        first = of(mine.first);
-        count = of(mine.count);
-        len = of(mine.len);
-        n_all = of(mine.n);
-        kt_item = of(mine.kt);
-        const int item = rel / kt_item;
-        t0 = rel - item * kt_item;
-        hk = item / rts;
-        rt = item - hk * rts;
-        kb = a.prefix_len;
-        base0 = kb & ~15;
-        rows = count * G;
-      }
-      pos0 = len - count;
-      // Keys that the tile's last row sees.
-      n = min(n_all, max(pos0 + a.group.div(min(rt * R + R, rows) - 1) + 1, 0));
-      if constexpr (WHOLE) kt_item = (n + UK - 1) / UK;
-      trow = a.seq.table + b * a.seq.stride;
-      bad |= len > a.seq.cap;
-    }
+    // Keys that the tile's last row sees.
+    const int n = prefix ? n_all : min(n_all, max(pos0 + a.group.div(min(rt * R + R, rows) - 1) + 1, 0));
+    if constexpr (WHOLE) kt_item = (n + UK - 1) / UK;
     const int t1 = WHOLE ? kt_item : min(kt_item, t0 + (u_end - u));
-    u += WHOLE ? 1 : t1 - t0;
 
     // ---- its rows: lane (g, frow) works for rows rt R + 16 qt + frow
     const int r0 = rt * R, nqt = min(QT, (rows - r0 + 15) >> 4);
@@ -515,9 +530,8 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
             *reinterpret_cast<f32x4_t*>(os + frow * HD + ((((4 * dt + g) ^ frow) & (HD / 4 - 1)) << 2)) = v;
           }
       __syncthreads();
-      for (int i = tid; i < 16 * (HD / 4); i += 64 * NW) {
+      for (int i = tid; i < min(16, rows - r0 - 16 * qt) * (HD / 4); i += 64 * NW) {
         const int rr = i / (HD / 4), c = i % (HD / 4), r = r0 + 16 * qt + rr;
-        if (r >= rows) continue;
         const int wr = 16 * qt + rr;
         float mm = wave_m[0][wr];
 #pragma unroll
@@ -556,6 +570,18 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
         }
       }
     }
+    if constexpr (WHOLE) break;
+    // ---- the next item
+    u += t1 - t0;
+    if (u >= u_end) break;
+    t0 = 0;
+    if (++rt == rts) {
+      rt = 0;
+      if (++hk == a.Hkv) {
+        hk = 0;
+        if (!enter_sequence()) break;
+      }
+    }
     __syncthreads();  // wave_m, wave_l and the tiles are free again
   }
   if (bad && a.err != nullptr) *a.err = 1;
@@ -565,24 +591,25 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
 // by group and then across the groups, always in the same order.  Rows that one block
 // has written whole are left; rows without a key become zeros.
 template <typename T, int HD, int R, int UK>
-__global__ __launch_bounds__(kStreamThreads) void paged_join_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units,
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units,
                                                                     int grid, int n_tile) {
-  constexpr int LP = HD / 4, NG = kStreamThreads / LP;
+  constexpr int LP = HD / 4, NG = kJoinThreads / LP;
   __shared__ float gm[NG], gl[NG];
   __shared__ __attribute__((aligned(16))) float go[NG][HD];
   const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq;
-  const int G = a.Hq / a.Hkv, hk = h / G;
+  const int G = static_cast<int>(a.group.d), hk = a.group.div(h);
   const int b = seq_of(a.seq, t);
   if (b >= a.seq.B) return;
   const SeqUnits su = seq_units<R, UK>(a, b);
-  const int U = grid > 0 ? ws.starts[a.seq.B] : 0, g = active_blocks(grid, U);
+  const int U = grid > 0 ? ws.starts[a.seq.B] : 0;
+  const Deal deal(max(grid, 1), U);
   // Runs of partials: the splits of the tile kernel, or blocks [i0, i1] of an item, or one
   // whole row.
   int i0[2] = {0, 0}, n_part[2] = {n_tile, 0}, wr[2] = {0, 0};
   const int64_t row = static_cast<int64_t>(t) * a.Hq + h;
   auto run = [&](int k, int start, int units, int r) {
-    i0[k] = unit_owner(start, U, g);
-    n_part[k] = unit_owner(start + units - 1, U, g) - i0[k] + 1;
+    i0[k] = deal.owner(start);
+    n_part[k] = deal.owner(start + units - 1) - i0[k] + 1;
     wr[k] = r;
   };
   if (prefix_units > 0) {
@@ -661,7 +688,13 @@ struct PagedPlan {
   int64_t o_starts = 0, o_eml = 0, o_eo = 0, o_wml = 0, o_wo = 0, o_tml = 0, o_to = 0, bytes = 0;
 };
 
-// Waves of a block that takes a whole item: as many as the registers allow.
+// A block that takes a whole item has as many waves as the registers allow.  It saves the
+// second launch (B x heads sequences of 256 keys, head_dim 64: 1 x 12 13 -> 9.6 us,
+// 16 x 12 15 -> 10.3, 16 x 25 17.7 -> 16.4, but 32 x 25 23 -> 28; head_dim 128: 8 x 8 15 ->
+// 11, 128 x 8 43 -> 39) while an item takes its waves few rounds: with few items and more
+// than two rounds the split over blocks is faster (1 x 12 of 2048 keys: 23 us whole, 15
+// split; 16 x 12: 26 and 32).  A prefix is then read again by every sequence, up to
+// kWholeAgain bytes.
 constexpr int whole_waves(int hd) { return hd == 128 ? 8 : 16; }
 constexpr int64_t kWholeKeys = 2048, kWholeAgain = int64_t{16} << 20;
 
@@ -674,13 +707,14 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     p->bytes += (bytes + 63) / 64 * 64;
     return o;
   };
-  // Short sequences: one launch.
+  // Short sequences: one launch, as long as the items do not crowd the card.
+  const int64_t items = Hkv * (call.cu_q == nullptr && Hq / Hkv <= 16 ? B : rows / 16 + B);
   const int64_t again = prefix_len * Hkv * HD * static_cast<int64_t>(sizeof(T)) * 2 * (B - 1);
-  if (rows <= 16 * B && cap <= kWholeKeys && again <= kWholeAgain) {
+  const int64_t most = 2 * items >= cus ? kWholeKeys : 2 * StreamShape<T, HD, 1, whole_waves(HD)>::UK;
+  if (rows <= 16 * B && cap <= most && (HD == 128 || 2 * items <= 3 * cus) && again <= kWholeAgain) {
+    if (items > 0x7fffffff) return CGPT_ESHAPE;
     p->whole = true;
-    const int64_t blocks = Hkv * (call.cu_q == nullptr && Hq / Hkv <= 16 ? B : rows / 16 + B);
-    if (blocks > 0x7fffffff) return CGPT_ESHAPE;
-    p->grid = static_cast<int>(blocks);
+    p->grid = static_cast<int>(items);
     return CGPT_OK;
   }
   const bool tile_ok = paged_tile_ok(call.dtype, HD);
@@ -705,11 +739,12 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     // sequence, or the batch against its prefix, has more than 16 rows a key head.
     const bool wide = !p->flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
     p->stream_qt = wide ? (HD == 128 ? 2 : 4) : 1;
-    const int64_t R = 16 * p->stream_qt, UK = StreamShape<T, HD, 1>::UK;
+    const int64_t R = 16 * p->stream_qt;
+    const int64_t UK = wide ? StreamShape<T, HD, 1, 4>::UK : StreamShape<T, HD, 1, stream_waves(HD)>::UK;
     const int64_t pu = prefix_len > 0 && !p->flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + UK - 1) / UK) : 0;
     const int64_t own = Hkv * (rows / R + B) * ((cap - (prefix_len & ~int64_t{15}) + UK - 1) / UK);
     if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
-    const int64_t per_cu = HD <= 64 && p->stream_qt == 1 ? 4 : 2;
+    const int64_t per_cu = wide || HD == 128 ? 2 : 8;  // eight waves a CU
     p->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pu + own, per_cu * cus)));
     p->prefix_units = static_cast<int>(pu);
     p->o_starts = take((B + 1) * 4);
@@ -732,11 +767,11 @@ static void launch_stream(const PagedAttnArgs& a, const PagedWs& ws, const Paged
                        p.prefix_units);
 }
 
-template <typename T, int HD, int QTW>
+template <typename T, int HD, int QTW, int NW>
 static void launch_join(const PagedAttnArgs& a, const PagedWs& ws, const PagedPlan& p, hipStream_t s) {
-  using C = StreamShape<T, HD, QTW>;
+  using C = StreamShape<T, HD, QTW, NW>;
   hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK>), dim3(static_cast<unsigned>(a.seq.n_tokens * a.Hq)),
-                     dim3(kStreamThreads), 0, s, a, ws, p.prefix_units, p.grid,
+                     dim3(kJoinThreads), 0, s, a, ws, p.prefix_units, p.grid,
                      p.flat || p.n_split > 1 ? p.n_split : 0);
 }
 
@@ -760,12 +795,12 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
     launch_stream<T, HD, 1, whole_waves(HD), true>(a, ws, p, s);
     return hip_status(hipGetLastError());
   }
-  if (p.stream_qt == 1) launch_stream<T, HD, 1, kStreamWaves, false>(a, ws, p, s);
-  if (p.stream_qt > 1) launch_stream<T, HD, WIDE, kStreamWaves, false>(a, ws, p, s);
+  if (p.stream_qt == 1) launch_stream<T, HD, 1, stream_waves(HD), false>(a, ws, p, s);
+  if (p.stream_qt > 1) launch_stream<T, HD, WIDE, 4, false>(a, ws, p, s);
   if (p.stream_qt > 1)
-    launch_join<T, HD, WIDE>(a, ws, p, s);
+    launch_join<T, HD, WIDE, 4>(a, ws, p, s);
   else if (p.stream_qt == 1 || p.n_split > 1)
-    launch_join<T, HD, 1>(a, ws, p, s);
+    launch_join<T, HD, 1, stream_waves(HD)>(a, ws, p, s);
   return hip_status(hipGetLastError());
 }
 

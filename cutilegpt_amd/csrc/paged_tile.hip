@@ -27,8 +27,36 @@ __device__ __forceinline__ void dma_lds16_at(const void* p, uint32_t lds) {
 #pragma clang diagnostic pop
 #endif
 
-template <typename T, int HD, int QTW, bool FLAT>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, 4))) void
+// Block i -> (key head, unit of that head), units 0 .. T - 1.  Blocks go to the eight XCDs
+// in turn, each with an L2 of its own: eight heads at a time take one XCD each, the
+// last Hkv % 8 (1, 2 or 4) share the XCDs evenly, so an L2 holds the keys of few heads.
+// (24 x 64 tokens, 12 heads, 2048 shared keys: TODO.)
+__host__ __device__ inline int head_blocks(int Hkv, int T) {
+  const int r = Hkv & 7;
+  return (Hkv - r) * T + (r == 0 ? 0 : 8 % r == 0 ? (T + 8 / r - 1) / (8 / r) * 8 : r * T);
+}
+__device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* unit) {
+  const int r = Hkv & 7, whole = Hkv - r;
+  if (i < whole * T) {
+    const int group = i / (8 * T), rem = i - group * 8 * T;
+    *hk = 8 * group + (rem & 7);
+    *unit = rem >> 3;
+    return true;
+  }
+  i -= whole * T;
+  if (8 % r == 0) {
+    const int per = 8 / r, x = i & 7;
+    *hk = whole + x / per;
+    *unit = (i >> 3) * per + x % per;
+  } else {
+    *hk = whole + i % r;
+    *unit = i / r;
+  }
+  return *unit < T;
+}
+
+template <typename T, int HD, int QTW, bool FLAT, bool A16, int STAGES>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 && STAGES == 2 ? 3 : 2, 4))) void
 paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, int n_tiles) {
 #if defined(__HIP_DEVICE_COMPILE__)
   static_assert(sizeof(T) == 2 && (HD == 64 || HD == 128), "16-bit types, head_dim 64 or 128");
@@ -37,18 +65,18 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   constexpr int XB = BKV * KROW, STAGE = 2 * XB;
   constexpr int INS = XB / 1024 / NWAVE;                         // loads a wave makes of K (and of V) a block
   constexpr int NKS = HD / 32, ND = HD / 16;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+  constexpr int LPS = 2 * INS;                                   // and of both
+  static_assert(A16 || STAGES == 2, "page ids by vector loads drain the queue at every block");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[STAGES * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, frow = lane & 15;
-  const int G = a.Hq / a.Hkv, page_size = static_cast<int>(a.seq.page.d);
+  const int G = static_cast<int>(a.group.d), page_size = static_cast<int>(a.seq.page.d);
 
-  // Key heads are the fastest index (blocks of one head on one XCD where their number
-  // allows), the last row tiles, which see most keys, start first.
-  int idx = blockIdx.x;
-  const int hk = idx % a.Hkv;
-  idx /= a.Hkv;
-  const int split = idx % n_split, tile = n_tiles - 1 - idx / n_split;
+  // The last row tiles, which see most keys, start first.
+  int hk, unit;
+  if (!head_unit(blockIdx.x, a.Hkv, n_tiles * n_split, &hk, &unit)) return;
+  const int rev = unit / n_split, split = unit - rev * n_split, tile = n_tiles - 1 - rev;
 
   // ---- rows
   int r0, rows, first = 0, pos0 = 0, n;
@@ -83,21 +111,24 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   const uint8_t* const kh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.kc.base) + hk * a.kc.sh);
   const uint8_t* const vh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.vc.base) + hk * a.vc.sh);
   int pg[INS];
+  // First key of load ii of block j (one page's, A16), or the lane's own.
   auto key_of = [&](int j, int ii) __attribute__((always_inline)) {
-    return min(j * BKV + (ii * NWAVE + wave) * RPI + lrow, n - 1);
+    const int key = j * BKV + (ii * NWAVE + wave) * RPI;
+    return A16 ? min(key, (n - 1) & ~(RPI - 1)) : min(key + lrow, n - 1);
   };
   auto fetch = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
     for (int ii = 0; ii < INS; ++ii) {
-      const int key = key_of(j, ii);
-      pg[ii] = (FLAT || key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
+      const int key = key_of(j, ii), col = a.seq.page.div(key);
+      const int* const row = FLAT || key < a.prefix_len ? a.prefix : trow;
+      pg[ii] = A16 ? ((const __attribute__((address_space(4))) int*)row)[__builtin_amdgcn_readfirstlane(col)] : row[col];
     }
   };
   auto issue = [&](int j, uint8_t* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int ii = 0; ii < INS; ++ii) {
       const int row = (ii * NWAVE + wave) * RPI + lrow, key = key_of(j, ii);
-      const int slot = key - a.seq.page.div(key) * page_size;
+      const int slot = (A16 ? min(key + lrow, n - 1) : key) - a.seq.page.div(key) * page_size;
       int p = pg[ii];
       if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) {
         p = 0;
@@ -105,15 +136,20 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
       }
       const int chunk = (slot16 ^ (row & 7)) << 4;
       const uint32_t lds = (ii * NWAVE + wave) * 1024;
-      dma_lds16_at(kh + 2 * (p * a.kc.sp + slot * a.kc.ss) + chunk, lds_addr(buf + lds));
-      dma_lds16_at(vh + 2 * (p * a.vc.sp + slot * a.vc.ss) + chunk, lds_addr(buf + XB + lds));
+      dma_lds16_at(kh + 2 * (p * a.kc.sp) + 2 * (slot * a.kc.ss) + chunk, lds_addr(buf + lds));
+      dma_lds16_at(vh + 2 * (p * a.vc.sp) + 2 * (slot * a.vc.ss) + chunk, lds_addr(buf + XB + lds));
     }
   };
 
+  // Blocks j0 .. j0 + STAGES - 2 are on their way before the loop; pg is one further.
   if (j0 < j1) {
     fetch(j0);
-    issue(j0, smem);
-    fetch(min(j0 + 1, j1 - 1));
+#pragma unroll
+    for (int st = 0; st < STAGES - 1; ++st)
+      if (j0 + st < j1) {
+        issue(j0 + st, smem + st * STAGE);
+        fetch(min(j0 + st + 1, j1 - 1));
+      }
   }
 
   u32x4_t qf[QT][NKS];
@@ -165,11 +201,11 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   int odd_from = 0x7fffffff;  // first masked block of keys with a value that is not finite
   for (int j = j0; j < j1; ++j) {
     raw_barrier();
-    const uint8_t* sk = smem + ((j - j0) & 1) * STAGE;
+    const uint8_t* sk = smem + ((j - j0) & (STAGES - 1)) * STAGE;
     const uint8_t* sv = sk + XB;
-    if (j + 1 < j1) {
-      issue(j + 1, smem + ((j - j0 + 1) & 1) * STAGE);
-      fetch(min(j + 2, j1 - 1));
+    if (j + STAGES - 1 < j1) {
+      issue(j + STAGES - 1, smem + ((j - j0 + STAGES - 1) & (STAGES - 1)) * STAGE);
+      fetch(min(j + STAGES, j1 - 1));
     }
     const int base = j * BKV;
     if (wave_live && base <= wave_last) {
@@ -283,7 +319,15 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
         pv(std::false_type{});
       }
     }
-    if (j + 1 < j1) wait_vmcnt<0>();
+    // This wave's part of block j + 1 has landed (loads return in order), and its LDS reads
+    // are done; the blocks behind it may be on their way.
+    const int later = min(j1 - 1, j + STAGES - 1) - (j + 1);
+    if (STAGES > 2 && later >= 2)
+      wait_vmcnt<STAGES == 4 ? 2 * LPS : 0>();
+    else if (STAGES > 2 && later == 1)
+      wait_vmcnt<STAGES == 4 ? LPS : 0>();
+    else
+      wait_vmcnt<0>();
   }
 
   // ---- values that are not finite in masked blocks: key by key, rarely
@@ -339,14 +383,33 @@ static int launch_tile(const PagedAttnArgs& a, bool flat, int n_split, float* pa
   const int64_t rows = static_cast<int64_t>(a.seq.n_tokens) * (a.Hq / a.Hkv);
   const int64_t tiles = flat ? (rows + BQ - 1) / BQ
                         : a.seq.cu == nullptr && a.Hq / a.Hkv <= BQ ? a.seq.B : rows / BQ + a.seq.B;
-  const int64_t blocks = tiles * n_split * a.Hkv;
-  if (blocks > 0x7fffffff) return CGPT_ESHAPE;
-  if (flat)
-    hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, true>), dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0,
-                       s, a, part_ml, part_o, n_split, static_cast<int>(tiles));
-  else
-    hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, false>), dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0,
-                       s, a, part_ml, part_o, n_split, static_cast<int>(tiles));
+  if (tiles * n_split * (a.Hkv + 8) > 0x7fffffff) return CGPT_ESHAPE;
+  const int blocks = head_blocks(a.Hkv, static_cast<int>(tiles * n_split));
+  // 16 keys lie in one page, and on one side of the prefix's end.
+  const bool a16 = a.seq.page.d % 16 == 0 && a.prefix_len % 16 == 0;
+  const int nt = static_cast<int>(tiles);
+#define CGPT_TILE(FLAT, A16, ST)                                                                                 \
+  hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, FLAT, A16, ST>), dim3(blocks), dim3(kTileThreads), 0, s, a, \
+                     part_ml, part_o, n_split, nt)
+  if (!a16) {
+    if (flat)
+      CGPT_TILE(true, false, 2);
+    else
+      CGPT_TILE(false, false, 2);
+  } else if (QTW == 1 && blocks <= (HD == 64 ? 2 : 1) * num_cus()) {
+    // Few blocks: nothing else on the CU hides the loads, so three blocks of keys are kept
+    // on their way.
+    if (flat)
+      CGPT_TILE(true, true, (QTW == 1 ? 4 : 2));
+    else
+      CGPT_TILE(false, true, (QTW == 1 ? 4 : 2));
+  } else {
+    if (flat)
+      CGPT_TILE(true, true, 2);
+    else
+      CGPT_TILE(false, true, 2);
+  }
+#undef CGPT_TILE
   return hip_status(hipGetLastError());
 }
 
