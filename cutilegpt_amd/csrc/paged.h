@@ -57,14 +57,21 @@ struct PagedAttnArgs {
   int* err;
 };
 
-// Attention of the query tiles of long steps (paged_tile.hip), 16-bit types of head_dim
-// 64 and 128.  flat: rows are all packed tokens, keys the shared prefix; else rows are a
-// sequence's and keys all of its own, those below prefix_len read from the prefix's
-// pages.  qt: 16-row sub-tiles of a wave (1 or 2; 4 waves).  n_split > 1 or flat: every
-// split leaves (m, l, O) of each (token, head) row in part_ml / part_o, else o is written.
+// What the tile kernel (paged_tile.hip; 16-bit types of head_dim 64 and 128) is to do:
+// all packed rows against the shared prefix in flat_split parts of its keys (0: not at
+// all), and every sequence's rows against its keys from `from` on, those below
+// prefix_len read from the prefix's pages, in `split` parts (0: not at all).  With ml each
+// part leaves (m, l, O) of its (token, head) rows there, the prefix's parts first; else the
+// rows' results are written.  The other fields are launch_paged_tile's.
+struct TileJob {
+  float* ml;
+  float* o;
+  int flat_split, split, from;
+  int flat_tiles, tiles, flat_blocks;
+};
 bool paged_tile_ok(int64_t dtype, int head_dim);
-int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split,
-                      float* part_ml, float* part_o, hipStream_t s);
+// qt: 16-row sub-tiles of each of a block's four waves, 1 or 2.
+int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const TileJob& job, int qt, hipStream_t s);
 
 // The checks that the entry points share: the sizes, then (with tokens to work on) the
 // pointers.  CGPT_OK with *empty when there is nothing to launch.
@@ -135,6 +142,18 @@ __device__ __forceinline__ int seq_of(const PagedBatch& s, int t) {
       lo = mid + 1;
   }
   return lo;
+}
+
+// seq_of for a token that the whole wave asks for.
+__device__ __forceinline__ int wave_seq_of(const PagedBatch& s, int t, int lane) {
+  if (s.cu == nullptr) return min(t, s.B);
+  int b = 0;
+  for (int c = 0; c < s.B; c += 64) {
+    const int k = __popcll(__builtin_amdgcn_ballot_w64(c + lane < s.B && s.cu[c + lane + 1] <= t));
+    b += k;
+    if (k < 64) break;
+  }
+  return b;
 }
 
 // Row tiles of R rows over sequences of any numbers of tokens: sequence b has the slots

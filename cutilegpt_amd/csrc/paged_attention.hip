@@ -107,7 +107,6 @@ struct StreamShape {
 // 1024 keys 97 -> 88, 8192 keys 578 -> 569); at head_dim 128 four of them read a page's
 // rows together (128 x 8 heads, 2048 keys: 201 us alone, 192 together).
 constexpr int stream_waves(int hd) { return hd == 128 ? 4 : 1; }
-constexpr int kJoinThreads = 256;
 
 // Each wave streams keys by itself: K and V rows go from their pages into registers,
 // one subtile of KT keys ahead of the one in use, in the layout of the matrix cores' A
@@ -587,44 +586,60 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
   if (bad && a.err != nullptr) *a.err = 1;
 }
 
-// One block a (token, head) row: its partials, each read by HD / 4 lanes, added group
-// by group and then across the groups, always in the same order.  Rows that one block
-// has written whole are left; rows without a key become zeros.
-template <typename T, int HD, int R, int UK>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units,
-                                                                    int grid, int n_tile) {
-  constexpr int LP = HD / 4, NG = kJoinThreads / LP;
-  __shared__ float gm[NG], gl[NG];
-  __shared__ __attribute__((aligned(16))) float go[NG][HD];
-  const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq;
+// One wave, or with WAVES = 4 one block, a (token, head) row: its partials, each read by
+// HD / 4 lanes, added group of lanes by group and then across the groups, always in the
+// same order.  Rows that one block has written whole are left; rows without a key become
+// zeros.
+template <typename T, int HD, int R, int UK, int WAVES>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units, int grid,
+                                                         int n_tile) {
+  constexpr int LP = HD / 4, GW = 64 / LP, NG = GW * WAVES;
+  __shared__ float gm[WAVES], gl[WAVES];
+  __shared__ __attribute__((aligned(16))) float go[WAVES][HD];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = WAVES == 1 ? static_cast<int>(blockIdx.x) * 4 + wave : static_cast<int>(blockIdx.x);
+  if (row >= a.seq.n_tokens * a.Hq) return;
+  const int t = row / a.Hq, h = row - t * a.Hq;
   const int G = static_cast<int>(a.group.d), hk = a.group.div(h);
-  const int b = seq_of(a.seq, t);
-  if (b >= a.seq.B) return;
-  const SeqUnits su = seq_units<R, UK>(a, b);
-  const int U = grid > 0 ? ws.starts[a.seq.B] : 0;
-  const Deal deal(max(grid, 1), U);
   // Runs of partials: the splits of the tile kernel, or blocks [i0, i1] of an item, or one
   // whole row.
   int i0[2] = {0, 0}, n_part[2] = {n_tile, 0}, wr[2] = {0, 0};
-  const int64_t row = static_cast<int64_t>(t) * a.Hq + h;
-  auto run = [&](int k, int start, int units, int r) {
-    i0[k] = deal.owner(start);
-    n_part[k] = deal.owner(start + units - 1) - i0[k] + 1;
-    wr[k] = r;
-  };
-  if (prefix_units > 0) {
-    const int rows = a.seq.n_tokens * G, rts = (rows + R - 1) / R, kt = (a.prefix_len + UK - 1) / UK;
-    const int r = t * G + h - hk * G;
-    run(0, (hk * rts + r / R) * kt, kt, r % R);
+  if (grid == 0) {
+    if (a.seq.cu != nullptr && t >= a.seq.cu[a.seq.B]) return;
+  } else {
+    const int b = wave_seq_of(a.seq, t, lane);
+    if (b >= a.seq.B) return;
+    const SeqUnits su = seq_units<R, UK>(a, b);
+    const int U = ws.starts[a.seq.B], start = ws.starts[b];
+    const Deal deal(grid, U);
+    auto run = [&](int k, int from, int units, int r) {
+      i0[k] = deal.owner(from);
+      n_part[k] = deal.owner(from + units - 1) - i0[k] + 1;
+      wr[k] = r;
+    };
+    if (prefix_units > 0) {
+      const int rows = a.seq.n_tokens * G, rts = (rows + R - 1) / R, kt = (a.prefix_len + UK - 1) / UK;
+      const int r = t * G + h - hk * G;
+      run(0, (hk * rts + r / R) * kt, kt, r % R);
+    }
+    if (su.kt > 0) {
+      const int r = (t - su.first) * G + h - hk * G;
+      run(1, start + (hk * su.rt + r / R) * su.kt, su.kt, r % R);
+    }
+    if (a.prefix_len == 0 && n_part[1] == 1) return;
   }
-  if (grid > 0 && su.kt > 0) {
-    const int r = (t - su.first) * G + h - hk * G;
-    run(1, ws.starts[b] + (hk * su.rt + r / R) * su.kt, su.kt, r % R);
-  }
-  if (a.prefix_len == 0 && n_part[1] == 1) return;
-  const int lg = threadIdx.x / LP, c = threadIdx.x % LP;
+  const int lg = wave % WAVES * GW + lane / LP, c = lane % LP;
   float m = -INFINITY, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float mi, float li, const f32x4_t& x) __attribute__((always_inline)) {
+    const float mn = fmaxf(m, mi);
+    const float fo = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    const float fi = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - mn);
+    m = mn;
+    l = l * fo + li * fi;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * fo + x[e] * fi;
+  };
   const int np = n_part[0] + n_part[1];
 #pragma unroll 4
   for (int j = lg; j < np; j += NG) {
@@ -643,36 +658,29 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs 
       ml = ws.edge_ml + 2 * at;
       ov = ws.edge_o + HD * at;
     }
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(ov + 4 * c);
-    const float mi = ml[0], li = ml[1], mn = fmaxf(m, mi);
-    const float fo = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-    const float fi = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - mn);
-    m = mn;
-    l = l * fo + li * fi;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * fo + x[e] * fi;
+    add(ml[0], ml[1], *reinterpret_cast<const f32x4_t*>(ov + 4 * c));
   }
-  if (c == 0) {
-    gm[lg] = m;
-    gl[lg] = l;
-  }
-  *reinterpret_cast<f32x4_t*>(&go[lg][4 * c]) = o;
-  __syncthreads();
-  if (lg != 0) return;
-  const int used = min(NG, np);
-  float mm = -INFINITY;
-  for (int k = 0; k < used; ++k) mm = fmaxf(mm, gm[k]);
-  float lt = 0.f, out[4] = {0.f, 0.f, 0.f, 0.f};
-  if (mm != -INFINITY)
-    for (int k = 0; k < used; ++k) {
-      const float f = __builtin_amdgcn_exp2f(gm[k] - mm);
-      lt += gl[k] * f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = fmaf(go[k][4 * c + e], f, out[e]);
+  for (int off = LP; off < 64; off <<= 1) {
+    const float mi = __shfl_xor(m, off, 64), li = __shfl_xor(l, off, 64);
+    const f32x4_t x = {__shfl_xor(o[0], off, 64), __shfl_xor(o[1], off, 64), __shfl_xor(o[2], off, 64),
+                       __shfl_xor(o[3], off, 64)};
+    add(mi, li, x);
+  }
+  if constexpr (WAVES > 1) {
+    if (lane == 0) {
+      gm[wave] = m;
+      gl[wave] = l;
     }
-  const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // no key, or a NaN that stays one
+    if (lane < LP) *reinterpret_cast<f32x4_t*>(&go[wave][4 * c]) = o;
+    __syncthreads();
+    if (wave != 0) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] *= inv;
+    for (int w = 1; w < WAVES; ++w) add(gm[w], gl[w], *reinterpret_cast<const f32x4_t*>(&go[w][4 * c]));
+  }
+  if (lane >= LP) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key, or a NaN that stays one
+  const float out[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
   store4_out(static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh + 4 * c, out);
 }
 
@@ -682,8 +690,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs 
 // prefix, the stream kernel, and the join.  Workspace offsets in bytes.
 struct PagedPlan {
   bool whole = false;               // stream kernel, a block an item
-  bool tile = false, flat = false;  // tile kernel; its rows are the whole batch's
-  int tile_qt = 1, n_split = 1;
+  int tile_qt = 1, flat_split = 0, split = 0, n_tile = 0;  // tile kernel, and its partials a row
   int stream_qt = 0, grid = 0, prefix_units = 0;  // stream kernel (stream_qt 0: none)
   int64_t o_starts = 0, o_eml = 0, o_eo = 0, o_wml = 0, o_wo = 0, o_tml = 0, o_to = 0, bytes = 0;
 };
@@ -697,6 +704,8 @@ struct PagedPlan {
 // kWholeAgain bytes.
 constexpr int whole_waves(int hd) { return hd == 128 ? 8 : 16; }
 constexpr int64_t kWholeKeys = 2048, kWholeAgain = int64_t{16} << 20;
+// Rows of a sequence from which on it reads a prefix by itself.
+constexpr int64_t kAloneRows = 96;
 
 template <typename T, int HD>
 static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
@@ -717,31 +726,33 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     p->grid = static_cast<int>(items);
     return CGPT_OK;
   }
-  const bool tile_ok = paged_tile_ok(call.dtype, HD);
-  p->flat = tile_ok && prefix_len > 0 && rows > 16 && rows <= 16 * B;
-  p->tile = p->flat || (tile_ok && rows > 16 * B);
-  if (p->tile) {
+  if (paged_tile_ok(call.dtype, HD) && rows > 16) {
+    // The batch's rows against the prefix together as long as a sequence alone fills no
+    // tiles; its own keys by the tile kernel from 16 rows a sequence on, else by the stream
+    // kernel.
+    const bool flat = prefix_len > 0 && rows <= kAloneRows * B, own = rows > 16 * B;
+    const int64_t keys = flat ? prefix_len : cap;
+    auto blocks = [&](int64_t bq) { return Hkv * (flat ? (rows + bq - 1) / bq : rows / bq + B); };
     // 128-row tiles where they fill the card, else 64; then the keys split until the card
-    // is full, 256 keys a split at least.
-    const int64_t keys = p->flat ? prefix_len : cap;
-    auto blocks = [&](int64_t bq) { return Hkv * (p->flat ? (rows + bq - 1) / bq : rows / bq + B); };
-    p->tile_qt = blocks(128) >= 4 * cus || (p->flat && rows > 64) ? 2 : 1;
+    // is full, 256 keys a part at least.
+    p->tile_qt = blocks(128) >= 4 * cus || (flat && rows > 64) ? 2 : 1;
     const int64_t n = blocks(64 * p->tile_qt), fit = (HD == 64 ? (p->tile_qt == 2 ? 3 : 4) : 2) * cus;
-    p->n_split = static_cast<int>(std::max<int64_t>(1, std::min(fit / n, keys / 256)));
-    if (!p->flat && n >= cus) p->n_split = 1;
-    if (n * p->n_split > 0x7fffffff) return CGPT_ESHAPE;
-    const bool parts = p->flat || p->n_split > 1;
-    p->o_tml = take(parts ? p->n_split * n_tokens * Hq * 8 : 0);
-    p->o_to = take(parts ? p->n_split * n_tokens * Hq * HD * 4 : 0);
+    const int split = static_cast<int>(std::max<int64_t>(1, std::min(fit / n, keys / 256)));
+    if (flat) p->flat_split = split;
+    if (own) p->split = flat ? 1 : split;
+    if (n * split > 0x7fffffff) return CGPT_ESHAPE;
+    p->n_tile = flat || split > 1 ? p->flat_split + p->split : 0;
+    p->o_tml = take(p->n_tile * n_tokens * Hq * 8);
+    p->o_to = take(p->n_tile * n_tokens * Hq * HD * 4);
   }
-  if (!p->tile || p->flat) {
+  if (p->split == 0) {
     // 64-row tiles (32 at head_dim 128, whose accumulators are twice as wide) where a
     // sequence, or the batch against its prefix, has more than 16 rows a key head.
-    const bool wide = !p->flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
+    const bool flat = p->flat_split > 0, wide = !flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
     p->stream_qt = wide ? (HD == 128 ? 2 : 4) : 1;
     const int64_t R = 16 * p->stream_qt;
     const int64_t UK = wide ? StreamShape<T, HD, 1, 4>::UK : StreamShape<T, HD, 1, stream_waves(HD)>::UK;
-    const int64_t pu = prefix_len > 0 && !p->flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + UK - 1) / UK) : 0;
+    const int64_t pu = prefix_len > 0 && !flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + UK - 1) / UK) : 0;
     const int64_t own = Hkv * (rows / R + B) * ((cap - (prefix_len & ~int64_t{15}) + UK - 1) / UK);
     if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
     const int64_t per_cu = wide || HD == 128 ? 2 : 8;  // eight waves a CU
@@ -770,9 +781,16 @@ static void launch_stream(const PagedAttnArgs& a, const PagedWs& ws, const Paged
 template <typename T, int HD, int QTW, int NW>
 static void launch_join(const PagedAttnArgs& a, const PagedWs& ws, const PagedPlan& p, hipStream_t s) {
   using C = StreamShape<T, HD, QTW, NW>;
-  hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK>), dim3(static_cast<unsigned>(a.seq.n_tokens * a.Hq)),
-                     dim3(kJoinThreads), 0, s, a, ws, p.prefix_units, p.grid,
-                     p.flat || p.n_split > 1 ? p.n_split : 0);
+  const int rows = a.seq.n_tokens * a.Hq;
+  // Few rows have many partials each; many rows want many of them on a CU, since each
+  // is a chain of dependent loads (10 thousand rows of two partials: 16 us a block
+  // each, TODO a wave each).
+  if (rows < 4 * num_cus())
+    hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK, 4>), dim3(rows), dim3(256), 0, s, a, ws, p.prefix_units,
+                       p.grid, p.n_tile);
+  else
+    hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a, ws,
+                       p.prefix_units, p.grid, p.n_tile);
 }
 
 template <typename T, int HD>
@@ -787,8 +805,16 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
   const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), f32(p.o_eml), f32(p.o_eo), f32(p.o_wml), f32(p.o_wo),
                    f32(p.o_tml), f32(p.o_to)};
   constexpr int WIDE = HD == 128 ? 2 : 4;
-  if (p.tile) {
-    rc = launch_paged_tile(call.dtype, HD, a, p.flat, p.tile_qt, p.n_split, ws.tile_ml, ws.tile_o, s);
+  if (p.flat_split + p.split > 0) {
+    TileJob job{};
+    if (p.n_tile > 0) {
+      job.ml = ws.tile_ml;
+      job.o = ws.tile_o;
+    }
+    job.flat_split = p.flat_split;
+    job.split = p.split;
+    job.from = p.flat_split > 0 ? a.prefix_len : 0;
+    rc = launch_paged_tile(call.dtype, HD, a, job, p.tile_qt, s);
     if (rc != CGPT_OK) return rc;
   }
   if (p.whole) {
@@ -799,7 +825,7 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
   if (p.stream_qt > 1) launch_stream<T, HD, WIDE, 4, false>(a, ws, p, s);
   if (p.stream_qt > 1)
     launch_join<T, HD, WIDE, 4>(a, ws, p, s);
-  else if (p.stream_qt == 1 || p.n_split > 1)
+  else if (p.stream_qt == 1 || p.n_tile > 0)
     launch_join<T, HD, 1, stream_waves(HD)>(a, ws, p, s);
   return hip_status(hipGetLastError());
 }

@@ -55,9 +55,12 @@ __device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* u
   return *unit < T;
 }
 
-template <typename T, int HD, int QTW, bool FLAT, bool A16, int STAGES>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 && STAGES == 2 ? 3 : 2, 4))) void
-paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, int n_tiles) {
+// What a launch holds (compiled apart: the choices cost 8 % inside the key loop).
+enum TileMode { kOwnRows, kFlatRows, kBoth };
+
+template <typename T, int HD, int QTW, TileMode MODE, bool A16, int STAGES>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 && STAGES == 2 ? 3 : HD == 64 || STAGES == 2 ? 2 : 1, 4))) void
+paged_tile_kernel(PagedAttnArgs a, TileJob job) {
 #if defined(__HIP_DEVICE_COMPILE__)
   static_assert(sizeof(T) == 2 && (HD == 64 || HD == 128), "16-bit types, head_dim 64 or 128");
   constexpr int QT = QTW, BQ = 64 * QTW, BKV = kTileKeys, NWAVE = 4;
@@ -73,16 +76,20 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   const int g = lane >> 4, frow = lane & 15;
   const int G = static_cast<int>(a.group.d), page_size = static_cast<int>(a.seq.page.d);
 
-  // The last row tiles, which see most keys, start first.
+  // Blocks of the whole batch against the prefix come first; then, like them, the last row
+  // tiles, which see most keys.
+  const bool flat = MODE == kFlatRows || (MODE == kBoth && static_cast<int>(blockIdx.x) < job.flat_blocks);
+  const int n_split = flat ? job.flat_split : job.split, n_tiles = flat ? job.flat_tiles : job.tiles;
   int hk, unit;
-  if (!head_unit(blockIdx.x, a.Hkv, n_tiles * n_split, &hk, &unit)) return;
+  if (!head_unit(blockIdx.x - (flat ? 0 : job.flat_blocks), a.Hkv, n_tiles * n_split, &hk, &unit)) return;
   const int rev = unit / n_split, split = unit - rev * n_split, tile = n_tiles - 1 - rev;
+  const int kb = MODE == kBoth && !flat ? job.from : 0;  // first key
 
   // ---- rows
   int r0, rows, first = 0, pos0 = 0, n;
   const int* trow = nullptr;
   bool bad = false;
-  if (FLAT) {
+  if (flat) {
     r0 = tile * BQ;
     rows = a.seq.n_tokens * G;
     n = a.prefix_len;
@@ -104,8 +111,8 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   const bool wave_live = wr0 < rows;
 
   // ---- keys of this split, in blocks of 64
-  const int n_kv = (n + BKV - 1) / BKV, per = (n_kv + n_split - 1) / n_split;
-  const int j0 = split * per, j1 = min(j0 + per, n_kv);
+  const int jb = kb / BKV, n_kv = max((n + BKV - 1) / BKV - jb, 0), per = (n_kv + n_split - 1) / n_split;
+  const int j0 = jb + split * per, j1 = min(j0 + per, jb + n_kv);
 
   const int lrow = lane / CPR, slot16 = lane % CPR;
   const uint8_t* const kh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.kc.base) + hk * a.kc.sh);
@@ -114,13 +121,13 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
   // First key of load ii of block j (one page's, A16), or the lane's own.
   auto key_of = [&](int j, int ii) __attribute__((always_inline)) {
     const int key = j * BKV + (ii * NWAVE + wave) * RPI;
-    return A16 ? min(key, (n - 1) & ~(RPI - 1)) : min(key + lrow, n - 1);
+    return max(A16 ? min(key, (n - 1) & ~(RPI - 1)) : min(key + lrow, n - 1), kb);
   };
   auto fetch = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
     for (int ii = 0; ii < INS; ++ii) {
       const int key = key_of(j, ii), col = a.seq.page.div(key);
-      const int* const row = FLAT || key < a.prefix_len ? a.prefix : trow;
+      const int* const row = flat || key < a.prefix_len ? a.prefix : trow;
       pg[ii] = A16 ? ((const __attribute__((address_space(4))) int*)row)[__builtin_amdgcn_readfirstlane(col)] : row[col];
     }
   };
@@ -159,7 +166,7 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
     const int r = wr0 + 16 * qt + frow;
     const bool live = r < rows;
     const int i = a.group.div(live ? r : 0), h = hk * G + (live ? r : 0) - i * G, t = first + i;
-    if (FLAT) {
+    if (flat) {
       const int b = seq_of(a.seq, t);
       lim[qt] = -1;
       if (b < a.seq.B) {
@@ -189,12 +196,7 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
     for (int dt = 0; dt < ND; ++dt) o[qt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   // The last key that any row of the wave sees.
-  int wave_last;
-  if (FLAT) {
-    wave_last = n - 1;
-  } else {
-    wave_last = pos0 + a.group.div(min(wr0 + 16 * QT, rows) - 1);
-  }
+  const int wave_last = flat ? n - 1 : pos0 + a.group.div(min(wr0 + 16 * QT, rows) - 1);
   wait_vmcnt<0>();
 
   const int tr_row = 4 * g + (frow >> 2);
@@ -226,13 +228,14 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
       bool masked = false;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
-        if (__builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0) {
+        if (base < kb || __builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0) {
           masked = true;
-          const int hi = lim[qt] - base - 4 * g;
+          const int hi = lim[qt] - base - 4 * g, lo = kb - base - 4 * g;
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[qt][kt][r] = 16 * kt + r > hi ? -INFINITY : s[qt][kt][r];
+            for (int r = 0; r < 4; ++r)
+              s[qt][kt][r] = 16 * kt + r > hi || 16 * kt + r < lo ? -INFINITY : s[qt][kt][r];
         }
       // P against the running maximum as it stands.  A lane whose 16 values sum to at most
       // 2^7 has none above it, so its maximum need not move; only when some lane fails that
@@ -332,11 +335,16 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
 
   // ---- values that are not finite in masked blocks: key by key, rarely
   if (__builtin_expect(odd_from < j1, 0)) {
-    // (Rows past a block see it whole and have counted it already only where it was not
-    // masked for any row of the wave: the blocks from the first masked one on all are.)
-    for (int key = odd_from * BKV; key < min(n, j1 * BKV); ++key) {
+    // Blocks that no row of the wave was masked in have theirs in O already; once a row is
+    // masked at its end it stays so, but the block across kb stands alone.
+    for (int key = max(odd_from * BKV, kb); key < min(n, j1 * BKV); ++key) {
+      const int base = key & ~(BKV - 1);
+      bool masked = base < kb;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) masked |= __builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0;
+      if (!masked) continue;
       const int slot = key - a.seq.page.div(key) * page_size;
-      int p = (FLAT || key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
+      int p = (flat || key < a.prefix_len ? a.prefix : trow)[a.seq.page.div(key)];
       if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) p = 0;
       const T* kr = reinterpret_cast<const T*>(kh) + p * a.kc.sp + slot * a.kc.ss;
       const T* vr = reinterpret_cast<const T*>(vh) + p * a.vc.sp + slot * a.vc.ss;
@@ -351,7 +359,7 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
     const int r = wr0 + 16 * qt + frow;
     if (r >= rows) continue;
     const int i = a.group.div(r), h = hk * G + r - i * G, t = first + i;
-    if (!FLAT && n_split == 1) {
+    if (job.ml == nullptr) {
       const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key, or a NaN that stays one
       T* orow = static_cast<T*>(a.o) + t * a.o_st + h * a.o_sh;
 #pragma unroll
@@ -360,73 +368,72 @@ paged_tile_kernel(PagedAttnArgs a, float* part_ml, float* part_o, int n_split, i
         store4_out(orow + 16 * dt + 4 * g, v);
       }
     } else {
-      const int64_t at = (static_cast<int64_t>(split) * a.seq.n_tokens + t) * a.Hq + h;
+      const int64_t part = flat ? split : job.flat_split + split;
+      const int64_t at = (part * a.seq.n_tokens + t) * a.Hq + h;
       if (g == 0) {
-        part_ml[2 * at] = -nm[qt];
-        part_ml[2 * at + 1] = l;
+        job.ml[2 * at] = -nm[qt];
+        job.ml[2 * at + 1] = l;
       }
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * HD + 16 * dt + 4 * g) = o[qt][dt];
+      for (int dt = 0; dt < ND; ++dt) *reinterpret_cast<f32x4_t*>(job.o + at * HD + 16 * dt + 4 * g) = o[qt][dt];
     }
   }
   if (bad && a.err != nullptr) *a.err = 1;
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
-bool paged_tile_ok(int64_t dtype, int head_dim) {
-  return dtype != CGPT_F32 && (head_dim == 64 || head_dim == 128);
-}
-
 template <typename T, int HD, int QTW>
-static int launch_tile(const PagedAttnArgs& a, bool flat, int n_split, float* part_ml, float* part_o, hipStream_t s) {
+static int launch_tile(const PagedAttnArgs& a, TileJob job, hipStream_t s) {
   constexpr int BQ = 64 * QTW;
   const int64_t rows = static_cast<int64_t>(a.seq.n_tokens) * (a.Hq / a.Hkv);
-  const int64_t tiles = flat ? (rows + BQ - 1) / BQ
-                        : a.seq.cu == nullptr && a.Hq / a.Hkv <= BQ ? a.seq.B : rows / BQ + a.seq.B;
-  if (tiles * n_split * (a.Hkv + 8) > 0x7fffffff) return CGPT_ESHAPE;
-  const int blocks = head_blocks(a.Hkv, static_cast<int>(tiles * n_split));
+  const int64_t flat = job.flat_split > 0 ? (rows + BQ - 1) / BQ : 0;
+  const int64_t own = job.split == 0 ? 0 : a.seq.cu == nullptr && a.Hq / a.Hkv <= BQ ? a.seq.B : rows / BQ + a.seq.B;
+  if ((flat * job.flat_split + own * job.split) * (a.Hkv + 8) > 0x7fffffff) return CGPT_ESHAPE;
+  job.flat_tiles = static_cast<int>(flat);
+  job.tiles = static_cast<int>(own);
+  job.flat_blocks = head_blocks(a.Hkv, job.flat_tiles * job.flat_split);
+  const int blocks = job.flat_blocks + head_blocks(a.Hkv, job.tiles * job.split);
   // 16 keys lie in one page, and on one side of the prefix's end.
   const bool a16 = a.seq.page.d % 16 == 0 && a.prefix_len % 16 == 0;
-  const int nt = static_cast<int>(tiles);
-#define CGPT_TILE(FLAT, A16, ST)                                                                                 \
-  hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, FLAT, A16, ST>), dim3(blocks), dim3(kTileThreads), 0, s, a, \
-                     part_ml, part_o, n_split, nt)
-  if (!a16) {
-    if (flat)
-      CGPT_TILE(true, false, 2);
-    else
-      CGPT_TILE(false, false, 2);
-  } else if (QTW == 1 && blocks <= (HD == 64 ? 2 : 1) * num_cus()) {
-    // Few blocks: nothing else on the CU hides the loads, so three blocks of keys are kept
+#define CGPT_TILE(A16, ST)                                                                                           \
+  do {                                                                                                               \
+    if (own == 0)                                                                                                    \
+      hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, kFlatRows, A16, ST>), dim3(blocks), dim3(kTileThreads), 0, s, \
+                         a, job);                                                                                    \
+    else if (flat == 0)                                                                                              \
+      hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, kOwnRows, A16, ST>), dim3(blocks), dim3(kTileThreads), 0, s, \
+                         a, job);                                                                                    \
+    else                                                                                                             \
+      hipLaunchKernelGGL((paged_tile_kernel<T, HD, QTW, kBoth, A16, ST>), dim3(blocks), dim3(kTileThreads), 0, s, a, \
+                         job);                                                                                       \
+  } while (0)
+  if (!a16)
+    CGPT_TILE(false, 2);
+  else if (QTW == 1 && blocks <= (HD == 64 ? 2 : 1) * num_cus())
+    // Few blocks: little else on the CU hides the loads, so three blocks of keys are kept
     // on their way.
-    if (flat)
-      CGPT_TILE(true, true, (QTW == 1 ? 4 : 2));
-    else
-      CGPT_TILE(false, true, (QTW == 1 ? 4 : 2));
-  } else {
-    if (flat)
-      CGPT_TILE(true, true, 2);
-    else
-      CGPT_TILE(false, true, 2);
-  }
+    CGPT_TILE(true, (QTW == 1 ? 4 : 2));
+  else
+    CGPT_TILE(true, 2);
 #undef CGPT_TILE
   return hip_status(hipGetLastError());
 }
 
 template <typename T, int HD>
-static int launch_tile_qt(const PagedAttnArgs& a, bool flat, int qt, int n_split, float* part_ml, float* part_o,
-                          hipStream_t s) {
-  return qt == 2 ? launch_tile<T, HD, 2>(a, flat, n_split, part_ml, part_o, s)
-                 : launch_tile<T, HD, 1>(a, flat, n_split, part_ml, part_o, s);
+static int launch_tile_qt(const PagedAttnArgs& a, const TileJob& job, int qt, hipStream_t s) {
+  return qt == 2 ? launch_tile<T, HD, 2>(a, job, s) : launch_tile<T, HD, 1>(a, job, s);
 }
 
-int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, bool flat, int qt, int n_split, float* part_ml,
-                      float* part_o, hipStream_t s) {
-  if (dtype == CGPT_BF16 && head_dim == 64) return launch_tile_qt<bf16_t, 64>(a, flat, qt, n_split, part_ml, part_o, s);
-  if (dtype == CGPT_BF16 && head_dim == 128) return launch_tile_qt<bf16_t, 128>(a, flat, qt, n_split, part_ml, part_o, s);
-  if (dtype == CGPT_F16 && head_dim == 64) return launch_tile_qt<f16_t, 64>(a, flat, qt, n_split, part_ml, part_o, s);
-  if (dtype == CGPT_F16 && head_dim == 128) return launch_tile_qt<f16_t, 128>(a, flat, qt, n_split, part_ml, part_o, s);
+int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const TileJob& job, int qt, hipStream_t s) {
+  if (dtype == CGPT_BF16 && head_dim == 64) return launch_tile_qt<bf16_t, 64>(a, job, qt, s);
+  if (dtype == CGPT_BF16 && head_dim == 128) return launch_tile_qt<bf16_t, 128>(a, job, qt, s);
+  if (dtype == CGPT_F16 && head_dim == 64) return launch_tile_qt<f16_t, 64>(a, job, qt, s);
+  if (dtype == CGPT_F16 && head_dim == 128) return launch_tile_qt<f16_t, 128>(a, job, qt, s);
   return CGPT_EDTYPE;
+}
+
+bool paged_tile_ok(int64_t dtype, int head_dim) {
+  return dtype != CGPT_F32 && (head_dim == 64 || head_dim == 128);
 }
 
 }  // namespace cgpt
