@@ -719,7 +719,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
   // Short sequences: one launch, as long as the items do not crowd the card.
   const int64_t items = Hkv * (call.cu_q == nullptr && Hq / Hkv <= 16 ? B : rows / 16 + B);
   const int64_t again = prefix_len * Hkv * HD * static_cast<int64_t>(sizeof(T)) * 2 * (B - 1);
-  const int64_t most = 2 * items >= cus ? kWholeKeys : 2 * StreamShape<T, HD, 1, whole_waves(HD)>::UK;
+  const int64_t most = 2 * items >= cus ? kWholeKeys : 5 * StreamShape<T, HD, 1, whole_waves(HD)>::UK / 2;
   if (rows <= 16 * B && cap <= most && (HD == 128 || 2 * items <= 3 * cus) && again <= kWholeAgain) {
     if (items > 0x7fffffff) return CGPT_ESHAPE;
     p->whole = true;
