@@ -121,7 +121,7 @@ constexpr int stream_waves(int hd) { return hd == 128 ? 4 : 1; }
 // A16: 16 keys from a multiple of 16 on lie in one page (and on one side of the prefix's
 // end), whose id comes by a scalar load; else every lane looks its own key up.
 template <typename T, int HD, int QTW, bool A16, int NW, bool WHOLE>
-__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void
+__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : HD == 128 && QTW > 1 ? 1 : 2) void
 paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
   using C = StreamShape<T, HD, QTW, NW>;
   constexpr int QT = C::QT, NT = C::NT, NKS = C::NKS, ND = C::ND, KT = C::KT, UK = C::UK, R = C::R;
@@ -706,6 +706,7 @@ constexpr int whole_waves(int hd) { return hd == 128 ? 8 : 16; }
 constexpr int64_t kWholeKeys = 2048, kWholeAgain = int64_t{16} << 20;
 // Rows of a sequence from which on it reads a prefix by itself.
 constexpr int64_t kAloneRows = 96;
+constexpr int64_t kOwnKeys = 4096;
 
 template <typename T, int HD>
 static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
@@ -728,20 +729,32 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
   }
   if (paged_tile_ok(call.dtype, HD) && rows > 16) {
     // The batch's rows against the prefix together as long as a sequence alone fills no
-    // tiles; its own keys by the tile kernel from 16 rows a sequence on, else by the stream
-    // kernel.
-    const bool flat = prefix_len > 0 && rows <= kAloneRows * B, own = rows > 16 * B;
+    // tiles.
+    const bool flat = prefix_len > 0 && rows <= kAloneRows * B;
     const int64_t keys = flat ? prefix_len : cap;
     auto blocks = [&](int64_t bq) { return Hkv * (flat ? (rows + bq - 1) / bq : rows / bq + B); };
-    // 128-row tiles where they fill the card, else 64; then the keys split until the card
-    // is full, 256 keys a part at least.
-    p->tile_qt = blocks(128) >= 4 * cus || (flat && rows > 64) ? 2 : 1;
-    const int64_t n = blocks(64 * p->tile_qt), fit = (HD == 64 ? (p->tile_qt == 2 ? 3 : 4) : 2) * cus;
-    const int split = static_cast<int>(std::max<int64_t>(1, std::min(fit / n, keys / 256)));
-    if (flat) p->flat_split = split;
-    if (own) p->split = flat ? 1 : split;
-    if (n * split > 0x7fffffff) return CGPT_ESHAPE;
-    p->n_tile = flat || split > 1 ? p->flat_split + p->split : 0;
+    // 128-row tiles where there are four of them a CU, or at head_dim 128 against a prefix
+    // (32768 keys, 512 rows a head: 188 us, 218 in tiles of 64; at head_dim 64 tiles of 64
+    // rows win up to 2048 rows, 61 us against 65), else 64.  The keys are split, 256 a part at least,
+    // while a CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12
+    // heads of head_dim 64: 55 us whole, 43 in 3 parts; of up to 512: 67 whole, 86 in 2) or
+    // the resident number of prefix rows, whose partials are many.
+    p->tile_qt = blocks(128) >= 4 * cus || (flat && HD == 128 && rows > 128) ? 2 : 1;
+    const int64_t BQ = 64 * p->tile_qt;
+    auto parts = [&](int64_t n, int64_t room, int64_t of) {
+      return static_cast<int>(std::max<int64_t>(1, std::min(room * cus / n, of / 256)));
+    };
+    // A sequence's own keys behind a prefix go by the same launch, even for a single row
+    // (64 sequences, 25 heads, 4096 keys shared: 64 keys of their own 42 -> 36 us, 512 69 ->
+    // 60, 2048 159 -> 153), unless its tiles have 128 rows (128 sequences, 8 heads of
+    // head_dim 128, 2048 keys: 226 us, 211 by the stream kernel) or one sequence may have
+    // so many that its few blocks end last.
+    const bool own = rows > 16 * B || (flat && p->tile_qt == 1 && cap - prefix_len <= kOwnKeys);
+    const int64_t n_own = Hkv * (rows / BQ + B);
+    if (flat) p->flat_split = parts(blocks(BQ), HD == 64 ? 4 : 2, prefix_len);
+    if (own) p->split = parts(n_own, 6, cap - (flat ? prefix_len : 0));
+    if (blocks(BQ) * p->flat_split + n_own * p->split > 0x7fffffff) return CGPT_ESHAPE;
+    p->n_tile = flat || p->split > 1 ? p->flat_split + p->split : 0;
     p->o_tml = take(p->n_tile * n_tokens * Hq * 8);
     p->o_to = take(p->n_tile * n_tokens * Hq * HD * 4);
   }
@@ -755,7 +768,9 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     const int64_t pu = prefix_len > 0 && !flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + UK - 1) / UK) : 0;
     const int64_t own = Hkv * (rows / R + B) * ((cap - (prefix_len & ~int64_t{15}) + UK - 1) / UK);
     if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
-    const int64_t per_cu = wide || HD == 128 ? 2 : 8;  // eight waves a CU
+    // Eight waves a CU; four of the widest, which need more registers than two a SIMD
+    // leave (fp32, 8 x 512 tokens: 712 us with spills, 321 without).
+    const int64_t per_cu = HD == 128 ? (wide ? 1 : 2) : wide ? 2 : 8;
     p->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pu + own, per_cu * cus)));
     p->prefix_units = static_cast<int>(pu);
     p->o_starts = take((B + 1) * 4);
