@@ -130,7 +130,8 @@ __device__ __forceinline__ void seq_tokens(const PagedBatch& s, int b, int* firs
   *count = max(e - f, 0);
 }
 
-// The sequence that packed token t belongs to, B when it lies behind the last.
+// The sequence that packed token t belongs to, B when it lies behind the last (a token in
+// front of the first gets sequence 0, whose first token is behind it).
 __device__ __forceinline__ int seq_of(const PagedBatch& s, int t) {
   if (s.cu == nullptr) return min(t, s.B);
   int lo = 0, hi = s.B;  // the first b with cu[b + 1] > t
@@ -144,16 +145,23 @@ __device__ __forceinline__ int seq_of(const PagedBatch& s, int t) {
   return lo;
 }
 
+// How many of pred(0) .. pred(n - 1), true up to some index and false from there on, are
+// true: 64 probes at a time, all lanes with the same answer.
+template <typename F> __device__ __forceinline__ int wave_count(int n, int lane, F&& pred) {
+  int lo = 0, hi = n;
+  for (;;) {
+    const int step = (hi - lo + 63) >> 6, i = lo + (lane + 1) * max(step, 1) - 1;
+    const int k = __popcll(__builtin_amdgcn_ballot_w64(i < hi && pred(i)));
+    lo += k * step;
+    if (step <= 1) return lo;
+    hi = min(hi, lo + step - 1);
+  }
+}
+
 // seq_of for a token that the whole wave asks for.
 __device__ __forceinline__ int wave_seq_of(const PagedBatch& s, int t, int lane) {
   if (s.cu == nullptr) return min(t, s.B);
-  int b = 0;
-  for (int c = 0; c < s.B; c += 64) {
-    const int k = __popcll(__builtin_amdgcn_ballot_w64(c + lane < s.B && s.cu[c + lane + 1] <= t));
-    b += k;
-    if (k < 64) break;
-  }
-  return b;
+  return wave_count(s.B, lane, [&](int b) { return s.cu[b + 1] <= t; });
 }
 
 // Row tiles of R rows over sequences of any numbers of tokens: sequence b has the slots
@@ -167,15 +175,9 @@ __device__ __forceinline__ int slot_seq(const PagedBatch& s, int G, int lane, in
     *slot = 0;
     return b;
   }
-  int b = 0;
-  for (int c = 0; c < s.B; c += 64) {
-    const int bb = c + lane + 1;
-    const int at = s.cu == nullptr || bb > s.B ? bb : min(max(s.cu[bb], 0), s.n_tokens);
-    const int k = __popcll(__builtin_amdgcn_ballot_w64(bb <= s.B && at * G / R + bb <= *slot));
-    b += k;
-    if (k < 64) break;
-  }
-  if (b < s.B) *slot -= (s.cu == nullptr ? b : min(max(s.cu[b], 0), s.n_tokens)) * G / R + b;
+  auto start = [&](int b) { return (s.cu == nullptr ? b : min(max(s.cu[b], 0), s.n_tokens)) * G / R + b; };
+  const int b = wave_count(s.B, lane, [&](int i) { return start(i + 1) <= *slot; });
+  if (b < s.B) *slot -= start(b);
   return b;
 }
 

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
   int first, count;
   seq_tokens(a.seq, b, &first, &count);
   const int pos = a.seq.lens[b] - count + (t - first);
-  if (pos < 0) return;  // a padding row
+  if (t < first || pos < 0) return;  // a padding row
   bool bad = pos >= a.seq.cap;
   int slot = 0, page = 0;
   if (!bad) {

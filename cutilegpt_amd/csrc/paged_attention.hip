@@ -134,24 +134,31 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
   uint8_t* const sv = smem + wave * C::VBYTES;
   bool bad = false;
 
-  // Units of the sequences, 64 at a time: lane l holds sequence c0 + l.
+  // Units of up to 64 sequences from c0 on: lane l holds sequence c0 + l.  `before` counts
+  // the units in front of them.
   int c0 = 0, n_units = 0, incl = 0, before = prefix_units, total = 0;
   SeqUnits mine{};
-  auto load_chunk = [&](int c) __attribute__((always_inline)) {
+  auto scan = [&](int v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int w = __shfl_up(v, off, 64);
+      if (lane >= off) v += w;
+    }
+    return v;
+  };
+  auto load_chunk = [&](int c, int end) __attribute__((always_inline)) {
     c0 = c;
     n_units = 0;
-    if (c + lane < a.seq.B) {
+    if (c + lane < end) {
       mine = seq_units<R, UK>(a, c + lane);
       n_units = mine.rt * mine.kt * a.Hkv;
     }
-    incl = n_units;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += v;
-    }
+    incl = scan(n_units);
     total = __builtin_amdgcn_readlane(incl, 63);
   };
+  // More than 64 sequences: lane l adds up `per` of them, from l per on.
+  const int per = (a.seq.B + 63) >> 6;
+  int group_units = 0, group_incl = 0;
   // The item at hand: rows of tile rt of key head hk, keys [kb, n), cut into kt_item units
   // from base0 on; t0 is its first unit here.
   int u = 0, u_end = 1, hk = 0, rt = 0, rts = 1, t0 = 0, kt_item = 0, kb = 0, base0 = 0, n_all = 0, rows = 0, first = 0,
@@ -161,11 +168,17 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
   // The sequence whose units u lies in; false when there is none (the lengths changed
   // under the call).
   auto enter_sequence = [&]() __attribute__((always_inline)) {
-    while (u >= before + total) {
-      if (c0 + 64 >= a.seq.B) return false;
-      before += total;
-      load_chunk(c0 + 64);
+    if (per > 1) {
+      const int gi = __popcll(__builtin_amdgcn_ballot_w64(prefix_units + group_incl <= u));
+      if (gi >= 64) return false;
+      const int end = min((gi + 1) * per, a.seq.B);
+      before = prefix_units + __builtin_amdgcn_readlane(group_incl - group_units, gi);
+      for (load_chunk(gi * per, end); u >= before + total; load_chunk(c0 + 64, end)) {
+        if (c0 + 64 >= end) return false;
+        before += total;
+      }
     }
+    if (u >= before + total) return false;
     const int at = __popcll(__builtin_amdgcn_ballot_w64(before + incl <= u));
     auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, at); };
     prefix = false;
@@ -198,14 +211,30 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     trow = a.seq.table + b * a.seq.stride;
     bad = len > a.seq.cap;
   } else {
-    int U = prefix_units;
-    for (int c = 0; c < a.seq.B; c += 64) {
-      load_chunk(c);
-      if (blockIdx.x == 0 && wave == 0 && c + lane < a.seq.B) ws.starts[c + lane] = U + incl - n_units;
-      U += total;
+    const bool writes = blockIdx.x == 0 && wave == 0;
+    if (per == 1) {
+      load_chunk(0, a.seq.B);
+      group_incl = incl;
+      if (writes && lane < a.seq.B) ws.starts[lane] = prefix_units + incl - n_units;
+    } else {
+      const int first_b = lane * per, end_b = min(first_b + per, a.seq.B);
+#pragma unroll 4
+      for (int b = first_b; b < end_b; ++b) {
+        const SeqUnits su = seq_units<R, UK>(a, b);
+        group_units += su.rt * su.kt * a.Hkv;
+      }
+      group_incl = scan(group_units);
+      if (writes) {
+        int at = prefix_units + group_incl - group_units;
+        for (int b = first_b; b < end_b; ++b) {
+          const SeqUnits su = seq_units<R, UK>(a, b);
+          ws.starts[b] = at;
+          at += su.rt * su.kt * a.Hkv;
+        }
+      }
     }
+    const int U = prefix_units + __builtin_amdgcn_readlane(group_incl, 63);
     if (blockIdx.x == 0 && tid == 0) ws.starts[a.seq.B] = U;
-    if (a.seq.B > 64) load_chunk(0);
     const Deal deal(gridDim.x, U);
     if (static_cast<int>(blockIdx.x) >= deal.g || U == 0) return;
     u = deal.start(blockIdx.x);
@@ -543,7 +572,7 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
           const f32x4_t x = *reinterpret_cast<const f32x4_t*>(ow + rr * HD + (((c ^ rr) & (HD / 4 - 1)) << 2));
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] += x[e];
-          l += mm == -INFINITY ? 0.f : wave_l[w][wr] * __builtin_amdgcn_exp2f(wave_m[w][wr] - mm);
+          l += wave_l[w][wr] * (mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wave_m[w][wr] - mm));
         }
         const int tok = a.group.div(r), h = hk * G + r - tok * G, t = first + tok;
         if (WHOLE || (whole && a.prefix_len == 0)) {
@@ -605,16 +634,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PagedW
   // whole row.
   int i0[2] = {0, 0}, n_part[2] = {n_tile, 0}, wr[2] = {0, 0};
   if (grid == 0) {
-    if (a.seq.cu != nullptr && t >= a.seq.cu[a.seq.B]) return;
+    if (a.seq.cu != nullptr && (t < a.seq.cu[0] || t >= a.seq.cu[a.seq.B])) return;
   } else {
     const int b = wave_seq_of(a.seq, t, lane);
     if (b >= a.seq.B) return;
     const SeqUnits su = seq_units<R, UK>(a, b);
+    if (t < su.first || t >= su.first + su.count) return;  // in front of the first sequence
     const int U = ws.starts[a.seq.B], start = ws.starts[b];
     const Deal deal(grid, U);
     auto run = [&](int k, int from, int units, int r) {
-      i0[k] = deal.owner(from);
-      n_part[k] = deal.owner(from + units - 1) - i0[k] + 1;
+      if (U <= 0) return;
+      // (The bounds hold by themselves unless the lengths change under the call.)
+      i0[k] = deal.owner(max(min(from, U - 1), 0));
+      n_part[k] = deal.owner(max(min(from + units, U) - 1, 0)) - i0[k] + 1;
       wr[k] = r;
     };
     if (prefix_units > 0) {

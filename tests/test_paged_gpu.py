@@ -281,11 +281,74 @@ def test_value_of_a_seen_key_counts_whatever_it_is(gpu, dtype, new, room):
 
 @WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("new,prefix", [([1, 1, 1], 0), ([1, 3, 1], 0), ([20, 40, 30], 0), ([1] * 30, 64), ([8] * 4, 64)])
+def test_a_query_that_is_not_a_number(gpu, dtype, new, prefix, room):
+    """Its row is NaN, its neighbours' are not."""
+    p = Problem(dtype, 64, 16, 4, 2, ctx=[100 + b for b in range(len(new))], new=new, prefix=prefix, seed=31,
+                spare_cols=cols(room, 16))
+    bad = int(p.cu[1])
+    p.q[bad, 2, 5] = NAN
+    want, bound = attention(p)
+    got = run_attention(p, gpu)
+    assert torch.isnan(got[bad, 2]).all()
+    got = got.clone()
+    got[bad, 2], want[bad, 2], bound[bad, 2] = 0, 0, 0
+    within(got, want, bound)
+
+
+@WIDE
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B", [65, 200, 300])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (2, 0), (1, 32), (24, 0)])
+def test_many_sequences(gpu, dtype, B, new, prefix, room):
+    """More sequences than a wave looks at at once, lengths of zero among them."""
+    ctx = [prefix + (b * 37) % 90 for b in range(B)]
+    p = Problem(dtype, 64, 16, 2, 1, ctx, [new if b % 5 else 0 for b in range(B)] if new > 1 else [1] * B,
+                prefix=prefix, seed=B, spare_cols=cols(room, 16))
+    check_attention(p, gpu)
+
+
+def test_rows_in_front_of_the_first_sequence(gpu):
+    """Offsets that do not begin at 0: the rows before the first are padding too."""
+    for new, room in (([3, 2], 0), ([3, 2], 5000), ([40, 30], 0)):
+        p = Problem(BF16, 64, 16, 4, 2, ctx=[33, 60], new=new, seed=33, spare_cols=cols(room, 16))
+        want, bound = attention(p)
+        kc, vc, q, kb, qb = append(p)
+        d = p.on(gpu)
+        shift = 2
+        d.cu = d.cu + shift
+        rows = lambda t: torch.cat([torch.full_like(t[:shift], 3.0), t])
+        out = torch.full_like(rows(d.q), 7.0)
+        cg.paged_attention(rows(d.q), d.k_cache, d.v_cache, d.table, d.lens, cu_q=d.cu, out=out)
+        assert (out[:shift] == 7.0).all()
+        within(out[shift:], want, bound)
+        got = cg.paged_kv_append(rows(d.k), rows(d.v), d.k_cache, d.v_cache, d.table, d.lens, cu_q=d.cu, q=rows(d.q),
+                                 q_out=torch.full_like(out, 7.0))
+        assert (got[:shift] == 7.0).all()
+        within(got[shift:], q, qb)
+        within(d.k_cache, kc, kb)
+        within(d.v_cache, vc, torch.zeros_like(vc))
+
+
+@WIDE
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("new", [[1, 60, 2], [1, 2, 1]])
 def test_large_scores(gpu, dtype, new, room):
     """Scores in the hundreds: the running maximum jumps from tile to tile."""
     check_attention(Problem(dtype, 64, 16, 4, 2, ctx=[500, 3, 299], new=new, seed=14, scale=5.0,
                             spare_cols=cols(room, 16)), gpu)
+
+
+@pytest.mark.parametrize("new,prefix", [(1, 0), (1, 512), (50, 0), (8, 64)])
+def test_out_may_be_q(gpu, new, prefix):
+    for room in (0, 5000):
+        p = Problem(BF16, 64, 16, 4, 2, ctx=[600, 530, 900] * 8, new=[new] * 24, prefix=prefix, seed=34, spare_cols=cols(room, 16))
+        d = p.on(gpu)
+        want = run_attention(p, gpu)
+        call = cg.shared_prefix_attention if prefix else cg.paged_attention
+        got = call(d.q, d.k_cache, d.v_cache, d.table, d.lens, *([prefix] if prefix else []),
+                   cu_q=None if new == 1 else d.cu, out=d.q)
+        assert got is d.q and torch.equal(got, want)
 
 
 def test_scale_and_out(gpu):
