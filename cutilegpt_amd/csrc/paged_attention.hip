@@ -3,6 +3,18 @@
 // o[i, h] = softmax(scale q[i, h] K^T) V over the keys 0 .. pos(i) of token i's
 // sequence, read from its pages; with a shared prefix the first prefix_len keys of
 // every sequence are read from one list of pages.
+//
+// Softmax runs in base 2 in one pass over the keys with a running shift m: p = 2^(s
+// scale log2(e) - m), l = sum p, O = sum p v; parts of a row's keys join by m = max m_i,
+// l = sum l_i 2^(m_i - m), O likewise.  m, l, O and the scores are 32-bit; p is rounded to
+// the 16-bit type for the second product (the other operand has no more bits), while l adds
+// the unrounded ones.
+//
+// Three kernels: the stream kernel here for few rows (a decode step reads every key once:
+// the bound is HBM), the tile kernel (paged_tile.hip) for many, the join of their
+// partials.  make_plan below chooses.  Measured: 64 sequences of 1 to 8192 keys, 25 heads
+// of head_dim 64, bf16 294 us, 5.7 TB/s; four of 90 to 130 thousand, 8 heads of 128, fp16
+// 308 us, 5.8 TB/s (a large copy reaches 4.9 on the same card); one of 500 keys 8 us.
 #include <algorithm>
 
 #include "internal.h"
@@ -84,7 +96,7 @@ struct StreamShape {
   static constexpr int ES = sizeof(T);
   static constexpr int EPC = 16 / ES;              // elements of a 16-byte chunk
   static constexpr int CPR = HD / EPC;             // chunks of a row
-  static constexpr int SWZ = (CPR < 8 ? CPR : 8) - 1;
+  static constexpr int SWZ = (CPR < 8 ? CPR : 8) - 1;  // see vswz
   static constexpr int KSTEP = 4 * EPC;            // head_dim of one k-slab
   static constexpr int NKS = (HD + KSTEP - 1) / KSTEP;
   static constexpr int ND = HD / 16;
@@ -115,6 +127,10 @@ constexpr int stream_waves(int hd) { return hd == 128 ? 4 : 1; }
 // The NW waves of a block take a unit's KT-key parts and meet only at an item's end.
 // P comes straight from the S^T accumulators, the key order inside a slab permuted alike
 // on both operands.
+//
+// A subtile costs some 450 instructions whatever rows it serves, an item 1200 (scan of the
+// lengths, addresses, join): 60 % of the issue slots at the rate HBM delivers, so short
+// items are bound by them (64 x 25 items of 256 keys: 33 us, 3.2 TB/s).
 //
 // WHOLE: a block is one item with all its keys, the prefix's among them, and writes its
 // rows' results; no workspace, no join.
@@ -736,8 +752,15 @@ struct PagedPlan {
 // kWholeAgain bytes.
 constexpr int whole_waves(int hd) { return hd == 128 ? 8 : 16; }
 constexpr int64_t kWholeKeys = 2048, kWholeAgain = int64_t{16} << 20;
-// Rows of a sequence from which on it reads a prefix by itself.
-constexpr int64_t kAloneRows = 96;
+// Rows of a sequence up to which it shares the reading of a prefix: tiles filled by all
+// sequences and keys that stay in the L2s, against partials written and joined (32
+// sequences, 12 heads of head_dim 64: 63 rows each behind 1024 keys 60 us alone, 52 shared;
+// 104 rows 58 and 63; behind 16384 keys 255 rows 794 and 707, 455 rows 681 and 694; 8 heads
+// of 128, 255 rows behind 512 keys 97 and 113, 2048 keys 216 and 176, 16384 keys 1349 and 740).
+constexpr int64_t shared_rows(int64_t prefix_len, int hd) {
+  const int64_t r = prefix_len * hd / 1024;
+  return r < 96 ? 96 : r > 4 * hd ? 4 * hd : r;
+}
 constexpr int64_t kOwnKeys = 4096;
 
 template <typename T, int HD>
@@ -760,9 +783,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     return CGPT_OK;
   }
   if (paged_tile_ok(call.dtype, HD) && rows > 16) {
-    // The batch's rows against the prefix together as long as a sequence alone fills no
-    // tiles.
-    const bool flat = prefix_len > 0 && rows <= kAloneRows * B;
+    const bool flat = prefix_len > 0 && rows <= shared_rows(prefix_len, HD) * B;
     const int64_t keys = flat ? prefix_len : cap;
     auto blocks = [&](int64_t bq) { return Hkv * (flat ? (rows + bq - 1) / bq : rows / bq + B); };
     // 128-row tiles where there are four of them a CU, or at head_dim 128 against a prefix
@@ -831,7 +852,7 @@ static void launch_join(const PagedAttnArgs& a, const PagedWs& ws, const PagedPl
   const int rows = a.seq.n_tokens * a.Hq;
   // Few rows have many partials each; many rows want many of them on a CU, since each
   // is a chain of dependent loads (10 thousand rows of two partials: 16 us a block
-  // each, TODO a wave each).
+  // each, 5 us a wave each).
   if (rows < 4 * num_cus())
     hipLaunchKernelGGL((paged_join_kernel<T, HD, C::R, C::UK, 4>), dim3(rows), dim3(256), 0, s, a, ws, p.prefix_units,
                        p.grid, p.n_tile);

@@ -5,10 +5,20 @@
 // rows are token-major, the group's heads side by side, so a key row is read once for
 // all of them); keys come 64 at a time, K and V straight from their pages into LDS by
 // direct-to-LDS loads with an address a lane, the next 64 in flight while these are
-// used.  The page ids are read one block of keys ahead of the loads that need them.
+// used.  The page ids are read one block of keys ahead of the loads that need them: where
+// a page is a multiple of 16 keys (A16) by scalar loads, which do not queue with the
+// key loads, so more than one block may be on its way.
 // S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs as in cgpt_attention_fwd's kernel: a
 // lane owns one query row, P goes from the accumulators straight into the second
 // product, V is transposed by the LDS read.
+//
+// Bound: the exponentials.  A P costs an FMA, an exponential (a quarter of the rate), an
+// add and half a conversion, 26 cycles a 64 of them, against 16 on the matrix cores at
+// head_dim 64; 16 chunks of up to 2048 tokens behind up to 4096 keys, 16 heads of
+// head_dim 64, take 300 us: 630 TFLOP/s of what the mask leaves, VALU busy 55 % and
+// matrix cores 26 % of the time.  128 rows a block (two sub-tiles a wave) use a loaded
+// key for twice the rows of 64; blocks of eight waves with 128 or 256 rows were slower
+// (350 and 412 us), and 128 registers, for four waves a SIMD, spill (524 us).
 #include "internal.h"
 #include "paged.h"
 
@@ -30,7 +40,8 @@ __device__ __forceinline__ void dma_lds16_at(const void* p, uint32_t lds) {
 // Block i -> (key head, unit of that head), units 0 .. T - 1.  Blocks go to the eight XCDs
 // in turn, each with an L2 of its own: eight heads at a time take one XCD each, the
 // last Hkv % 8 (1, 2 or 4) share the XCDs evenly, so an L2 holds the keys of few heads.
-// (24 x 64 tokens, 12 heads, 2048 shared keys: TODO.)
+// Against heads in turn: 2048 tokens behind 20000 keys, 25 heads 274 -> 198 us, 12 heads
+// 116 -> 112; 16 prompts, 4 heads 322 -> 302, 25 heads 521 -> 499, 16 heads 392 -> 396.
 __host__ __device__ inline int head_blocks(int Hkv, int T) {
   const int r = Hkv & 7;
   return (Hkv - r) * T + (r == 0 ? 0 : 8 % r == 0 ? (T + 8 / r - 1) / (8 / r) * 8 : r * T);
