@@ -90,8 +90,10 @@ def _check_out(name: str, out: torch.Tensor, like: torch.Tensor, vec: int) -> No
 def _check_cache(name: str, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  block_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: Optional[torch.Tensor],
                  err_flag: Optional[torch.Tensor]):
-    """Checks what every entry point takes; returns the rows' device index, the dtype's
-    code, the elements in 16 bytes, the caches' sizes and strides and the table's sizes."""
+    """Checks what every entry point takes, as far as the native call cannot (it refuses
+    sizes, strides and alignments that the kernels do not take); returns the rows' device
+    index, the dtype's code, the elements in 16 bytes, the caches' sizes and strides and
+    the table's sizes and row stride."""
     try:
         dev, dt = x.get_device(), x.dtype
         same = (dev == k_cache.get_device() == v_cache.get_device() == block_table.get_device()
@@ -104,43 +106,39 @@ def _check_cache(name: str, x: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     code = _CODE.get(dt)
     if code is None:
         raise ValueError(f"{name}: unsupported dtype {dt} (float32, bfloat16 or float16)")
-    if k_cache.dtype != dt or v_cache.dtype != dt:
+    if k_cache.dtype is not dt or v_cache.dtype is not dt:
         raise ValueError(f"{name}: the caches hold {k_cache.dtype} and {v_cache.dtype}, the rows {dt}")
     shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or 0 in shape:
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"{name}: k_cache and v_cache must share a shape (n_pages, n_kv_head, page_size, "
                          f"head_dim), got {tuple(shape)} and {tuple(v_cache.shape)}")
     n_pages, heads, page, hd = shape
-    if x.dim() != 3 or x.shape[2] != hd or hd not in _HEAD_DIMS:
-        raise ValueError(f"{name}: the step's rows must be (n_tokens, heads, head_dim), head_dim one of "
-                         f"{_HEAD_DIMS} and the caches' {hd}, got {tuple(x.shape)}")
-    vec = 4 if code == 0 else 8
+    rows = x.shape
+    if len(rows) != 3 or rows[2] != hd:
+        raise ValueError(f"{name}: the step's rows must be (n_tokens, heads, {hd}), got {tuple(rows)}")
+    if hd not in _HEAD_DIMS:
+        raise ValueError(f"{name}: head_dim {hd} is not one of {_HEAD_DIMS}")
     kp, kh, ks, kd = k_cache.stride()
     vp, vh, vs, vd = v_cache.stride()
-    if (kd != 1 or vd != 1 or (kp | kh | ks | vp | vh | vs) % vec
-            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or (n_pages > 1 and min(kp, vp) < hd)
-            or (heads > 1 and min(kh, vh) < hd) or (page > 1 and min(ks, vs) < hd)):
-        raise ValueError(f"{name}: cache rows must be separate, contiguous and 16-byte aligned")
+    if kd != 1 or vd != 1:
+        raise ValueError(f"{name}: cache rows must be contiguous")
+    if block_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32:
+        raise ValueError(f"{name}: block_table and seq_lens must be int32")
     if block_table.dim() != 2 or seq_lens.dim() != 1:
         raise ValueError(f"{name}: block_table must be (B, pages) and seq_lens (B,), got "
                          f"{tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
     B, cols = block_table.shape
     ts, t1 = block_table.stride()
-    if seq_lens.shape[0] != B:
-        raise ValueError(f"{name}: block_table has {B} rows for {seq_lens.shape[0]} seq_lens")
-    if (block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32
-            or (cu_q is not None and cu_q.dtype != torch.int32)):
-        raise ValueError(f"{name}: block_table, seq_lens and cu_q must be int32")
-    if (t1 != 1 and cols > 1) or not seq_lens.is_contiguous():
-        raise ValueError(f"{name}: block_table rows and seq_lens must be contiguous")
+    if (t1 != 1 and cols > 1) or not seq_lens.is_contiguous() or seq_lens.shape[0] != B:
+        raise ValueError(f"{name}: block_table must have contiguous rows and seq_lens be {B} contiguous lengths")
     if cu_q is None:
-        if x.shape[0] != B:
-            raise ValueError(f"{name}: {x.shape[0]} rows for {B} sequences need cu_q")
-    elif cu_q.dim() != 1 or cu_q.shape[0] != B + 1 or not cu_q.is_contiguous():
-        raise ValueError(f"{name}: cu_q must be {B + 1} contiguous offsets, got {tuple(cu_q.shape)}")
-    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() != 1):
+        if rows[0] != B:
+            raise ValueError(f"{name}: {rows[0]} rows for {B} sequences need cu_q")
+    elif cu_q.dtype is not torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] != B + 1 or not cu_q.is_contiguous():
+        raise ValueError(f"{name}: cu_q must be {B + 1} contiguous int32 offsets, got {cu_q.dtype} {tuple(cu_q.shape)}")
+    if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
         raise ValueError(f"{name}: err_flag must be one int32")
-    return dev, code, vec, n_pages, heads, page, hd, (kp, kh, ks, vp, vh, vs), B, cols, ts
+    return dev, code, 8 if code else 4, n_pages, heads, page, hd, (kp, kh, ks, vp, vh, vs), B, cols, ts
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
