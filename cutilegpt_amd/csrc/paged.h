@@ -73,6 +73,9 @@ bool paged_tile_ok(int64_t dtype, int head_dim);
 // qt: 16-row sub-tiles of each of a block's four waves, 1 or 2.
 int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const TileJob& job, int qt, hipStream_t s);
 
+// Offsets within 16 consecutive slots of a page fit 32 bits.
+inline bool short_rows(const PagedAttnArgs& a) { return a.kc.ss <= (1 << 25) && a.vc.ss <= (1 << 25); }
+
 // The checks that the entry points share: the sizes, then (with tokens to work on) the
 // pointers.  CGPT_OK with *empty when there is nothing to launch.
 inline int check_paged(const cgpt_paged_args* p, bool* empty) {

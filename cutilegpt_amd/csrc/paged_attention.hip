@@ -342,23 +342,29 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
         }
       }
     };
+    // A lane's bytes into a key tile, and into its chunk of the row (A16).
+    const uint32_t k_row = static_cast<uint32_t>(sizeof(T) * a.kc.ss), v_row = static_cast<uint32_t>(sizeof(T) * a.vc.ss);
     auto load = [&](int i, const int (&pg)[NT], u32x4_t (&kd)[NT][NKS], u32x4_t (&vd)[NT][NKS]) __attribute__((always_inline)) {
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) {
-        const int key = max(min(sub0 + i * UK + 16 * kt + frow, n - 1), kb);
+        const int tile = sub0 + i * UK + 16 * kt;
+        const int key = A16 ? min(tile, (n - 1) & ~15) : max(min(tile + frow, n - 1), kb);
         const int slot = key - a.seq.page.div(key) * page_size;
-        int p = pg[kt];
+        int p = A16 ? __builtin_amdgcn_readfirstlane(pg[kt]) : pg[kt];
         if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) {
           p = 0;
           bad = true;
         }
-        const T* kp = kh + p * a.kc.sp + slot * a.kc.ss;
-        const T* vp = vh + p * a.vc.sp + slot * a.vc.ss;
+        const uint8_t* const kp = reinterpret_cast<const uint8_t*>(kh + p * a.kc.sp + slot * a.kc.ss);
+        const uint8_t* const vp = reinterpret_cast<const uint8_t*>(vh + p * a.vc.sp + slot * a.vc.ss);
+        uint32_t row = 0;
+        if (A16) row = tile >= kb && tile + 16 <= n ? frow : max(min(tile + frow, n - 1), kb) - key;
+        const uint32_t ko = row * k_row, vo = row * v_row;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
-          const int c = C::chunk(ks, g);
-          kd[kt][ks] = *reinterpret_cast<const u32x4_t*>(kp + c * C::EPC);
-          vd[kt][ks] = *reinterpret_cast<const u32x4_t*>(vp + c * C::EPC);
+          const int c = 16 * C::chunk(ks, g);
+          kd[kt][ks] = *reinterpret_cast<const u32x4_t*>(kp + (ko + c));
+          vd[kt][ks] = *reinterpret_cast<const u32x4_t*>(vp + (vo + c));
           // Lanes past a short row's chunks: 0 x inf would be NaN.
           if (!C::has(ks, g)) kd[kt][ks] = u32x4_t{0, 0, 0, 0};
         }
@@ -837,7 +843,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
 
 template <typename T, int HD, int QTW, int NW, bool WHOLE>
 static void launch_stream(const PagedAttnArgs& a, const PagedWs& ws, const PagedPlan& p, hipStream_t s) {
-  const bool a16 = a.seq.page.d % 16 == 0 && (!WHOLE || a.prefix_len % 16 == 0);
+  const bool a16 = a.seq.page.d % 16 == 0 && (!WHOLE || a.prefix_len % 16 == 0) && short_rows(a);
   if (a16)
     hipLaunchKernelGGL((paged_stream_kernel<T, HD, QTW, true, NW, WHOLE>), dim3(p.grid), dim3(64 * NW), 0, s, a, ws,
                        p.prefix_units);

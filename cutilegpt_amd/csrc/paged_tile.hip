@@ -122,7 +122,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
   const bool wave_live = wr0 < rows;
 
   // ---- keys of this split, in blocks of 64
-  const int jb = kb / BKV, n_kv = max((n + BKV - 1) / BKV - jb, 0), per = (n_kv + n_split - 1) / n_split;
+  const int jb = MODE == kBoth ? kb / BKV : 0, n_kv = max((n + BKV - 1) / BKV - jb, 0), per = (n_kv + n_split - 1) / n_split;
   const int j0 = jb + split * per, j1 = min(j0 + per, jb + n_kv);
 
   const int lrow = lane / CPR, slot16 = lane % CPR;
@@ -132,7 +132,8 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
   // First key of load ii of block j (one page's, A16), or the lane's own.
   auto key_of = [&](int j, int ii) __attribute__((always_inline)) {
     const int key = j * BKV + (ii * NWAVE + wave) * RPI;
-    return max(A16 ? min(key, (n - 1) & ~(RPI - 1)) : min(key + lrow, n - 1), kb);
+    const int k = A16 ? min(key, (n - 1) & ~(RPI - 1)) : min(key + lrow, n - 1);
+    return MODE == kBoth ? max(k, kb) : k;
   };
   auto fetch = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
@@ -239,14 +240,14 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
       bool masked = false;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
-        if (base < kb || __builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0) {
+        if ((MODE == kBoth && base < kb) || __builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0) {
           masked = true;
-          const int hi = lim[qt] - base - 4 * g, lo = kb - base - 4 * g;
+          const int hi = lim[qt] - base - 4 * g, lo = MODE == kBoth ? kb - base - 4 * g : -0x7fffffff;
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              s[qt][kt][r] = 16 * kt + r > hi || 16 * kt + r < lo ? -INFINITY : s[qt][kt][r];
+              s[qt][kt][r] = 16 * kt + r > hi || (MODE == kBoth && 16 * kt + r < lo) ? -INFINITY : s[qt][kt][r];
         }
       // P against the running maximum as it stands.  A lane whose 16 values sum to at most
       // 2^7 has none above it, so its maximum need not move; only when some lane fails that
@@ -350,7 +351,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
     // masked at its end it stays so, but the block across kb stands alone.
     for (int key = max(odd_from * BKV, kb); key < min(n, j1 * BKV); ++key) {
       const int base = key & ~(BKV - 1);
-      bool masked = base < kb;
+      bool masked = MODE == kBoth && base < kb;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) masked |= __builtin_amdgcn_ballot_w64(lim[qt] < base + BKV - 1) != 0;
       if (!masked) continue;
