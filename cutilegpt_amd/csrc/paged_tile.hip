@@ -122,7 +122,9 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
   const bool wave_live = wr0 < rows;
 
   // ---- keys of this split, in blocks of 64
-  const int jb = MODE == kBoth ? kb / BKV : 0, n_kv = max((n + BKV - 1) / BKV - jb, 0), per = (n_kv + n_split - 1) / n_split;
+  // (None for rows that see nothing past the prefix, whose table may end with it.)
+  const int jb = MODE == kBoth ? kb / BKV : 0, n_kv = n > kb ? (n + BKV - 1) / BKV - jb : 0,
+            per = (n_kv + n_split - 1) / n_split;
   const int j0 = jb + split * per, j1 = min(j0 + per, jb + n_kv);
 
   const int lrow = lane / CPR, slot16 = lane % CPR;

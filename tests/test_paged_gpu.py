@@ -231,6 +231,21 @@ def test_shared_prefix_inside_a_page_and_short_sequences(gpu, room, copies):
     assert torch.equal(again, got) and int(flag) == 0
 
 
+@pytest.mark.parametrize("most", [80, 100])
+def test_tables_that_end_with_the_prefix(gpu, most):
+    """Sequences that hold no key past the prefix: nothing is read behind their last page,
+    where the row may end or name no page."""
+    ctx = [65, 69, 78, 79, most - 1] * 24
+    p = Problem(BF16, 64, 16, 4, 4, ctx=ctx, new=[1] * len(ctx), prefix=80, seed=15, spare_cols=0)
+    assert p.table.shape[1] == -(-most // 16)
+    want, bound = attention(p)
+    d = p.on(gpu)
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    got = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, 80, err_flag=flag)
+    within(got, want, bound)
+    assert int(flag) == 0
+
+
 @WIDE
 @pytest.mark.parametrize("new", [1, 2, 40])
 def test_rows_without_a_key(gpu, new, room):
