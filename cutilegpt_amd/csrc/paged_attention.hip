@@ -928,15 +928,15 @@ extern "C" int cgpt_paged_attention(const cgpt_paged_args* args, void* stream) {
   const int rc = check_paged(args, &empty);
   if (rc != CGPT_OK) return rc;
   const cgpt_paged_args& p = *args;
-  const float scale = static_cast<float>(p.scale);
-  if (p.prefix_len < 0 || p.prefix_len > p.page_size * p.max_pages || !(scale > 0.f) || !(scale < INFINITY))
+  const float scale = static_cast<float>(p.scale), scale_log2 = scale * 1.4426950408889634f;
+  if (p.prefix_len < 0 || p.prefix_len > p.page_size * p.max_pages || !(scale > 0.f) || !(scale_log2 < INFINITY))
     return CGPT_EINVAL;
   if (empty) return CGPT_OK;
   if (p.q == nullptr || p.out == nullptr || (p.prefix_len > 0 && p.prefix_pages == nullptr)) return CGPT_EINVAL;
   const PagedAttnArgs a{p.q, p.out, PagePool{p.k_cache, p.kc_sp, p.kc_sh, p.kc_ss},
                         PagePool{p.v_cache, p.vc_sp, p.vc_sh, p.vc_ss}, paged_batch(p), p.prefix_pages,
                         static_cast<int>(p.prefix_len), p.q_st, p.q_sh, p.out_st, p.out_sh, static_cast<int>(p.Hq),
-                        static_cast<int>(p.Hkv), FastDiv(p.Hq / p.Hkv), scale * 1.4426950408889634f, p.err_flag};
+                        static_cast<int>(p.Hkv), FastDiv(p.Hq / p.Hkv), scale_log2, p.err_flag};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(p, [&](auto t, auto hd) {
     return run_plan<decltype(t), decltype(hd)::value>(a, p, s);

@@ -63,7 +63,7 @@ def test_c_append_refuses():
 def test_c_attention_refuses():
     fn = FNS[1]
     for change in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e-60),
-                   dict(scale=1e60), dict(prefix_len=-1), dict(prefix_len=65)):
+                   dict(scale=1e60), dict(scale=3e38), dict(prefix_len=-1), dict(prefix_len=65)):
         assert call(fn, **change) == EINVAL, change
     for change in (dict(prefix_pages=0), dict(q=0), dict(out=0)):
         assert call(fn, n_tokens=3, **change) == EINVAL, change
