@@ -210,11 +210,11 @@ template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w
 
 // Half of a V^T operand: the 16-lane group's lane k points at 4 consecutive d of its
 // row and receives the 4 keys of column 16 dt + k.
-template <int KROW, int SWZ>
-__device__ __forceinline__ u32x2_t vt_read(const uint8_t* sv, int row, int dt, int frow) {
+template <int KROW>
+__device__ __forceinline__ u32x2_t vt_read(const uint8_t* sv, int row, int swz, int dt, int frow) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   const int byte = dt * 32 + 8 * (frow & 3);
-  const uint8_t* p = sv + row * KROW + (((byte >> 4) ^ (row & SWZ)) << 4) + (byte & 15);
+  const uint8_t* p = sv + row * KROW + (((byte >> 4) ^ swz) << 4) + (byte & 15);
   const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (__attribute__((address_space(3))) s16x4*)((__attribute__((address_space(3))) uint8_t*)(p)));
   return __builtin_bit_cast(u32x2_t, r);

@@ -461,6 +461,7 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
           l_run[qt] += sum;
         }
       if constexpr (sizeof(T) == 2) {
+        const int vrow = 4 * g + (frow >> 2);
 #pragma unroll
         for (int c = 0; c < NT / 2; ++c) {
           u32x4_t pf[QT];
@@ -471,8 +472,8 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
                              pack2<T>(s[qt][2 * c + 1][2], s[qt][2 * c + 1][3])};
 #pragma unroll
           for (int dt = 0; dt < ND; ++dt) {
-            const u32x2_t lo = vt_read<C::KROW, C::SWZ>(sv, 32 * c + 4 * g + (frow >> 2), dt, frow);
-            const u32x2_t hi = vt_read<C::KROW, C::SWZ>(sv, 32 * c + 16 + 4 * g + (frow >> 2), dt, frow);
+            const u32x2_t lo = vt_read<C::KROW>(sv, 32 * c + vrow, vrow & C::SWZ, dt, frow);
+            const u32x2_t hi = vt_read<C::KROW>(sv, 32 * c + 16 + vrow, vrow & C::SWZ, dt, frow);
             const u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
@@ -810,7 +811,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     // so many that its few blocks end last.
     const bool own = rows > 16 * B || (flat && p->tile_qt == 1 && cap - prefix_len <= kOwnKeys);
     const int64_t n_own = Hkv * (rows / BQ + B);
-    if (flat) p->flat_split = parts(blocks(BQ), HD == 64 ? 4 : 2, prefix_len);
+    if (flat) p->flat_split = parts(blocks(BQ), HD <= 64 ? 4 : 2, prefix_len);
     if (own) p->split = parts(n_own, 6, cap - (flat ? prefix_len : 0));
     if (blocks(BQ) * p->flat_split + n_own * p->split > 0x7fffffff) return CGPT_ESHAPE;
     p->n_tile = flat || p->split > 1 ? p->flat_split + p->split : 0;

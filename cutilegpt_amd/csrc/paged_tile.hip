@@ -18,7 +18,8 @@
 // head_dim 64, take 300 us: 630 TFLOP/s of what the mask leaves, VALU busy 55 % and
 // matrix cores 26 % of the time.  128 rows a block (two sub-tiles a wave) use a loaded
 // key for twice the rows of 64; blocks of eight waves with 128 or 256 rows were slower
-// (350 and 412 us), and 128 registers, for four waves a SIMD, spill (524 us).
+// (350 and 412 us), and 128 registers, for four waves a SIMD, spill (524 us).  At head_dim
+// 32 the same chunks take 236 us, 561 by the stream kernel.
 #include "internal.h"
 #include "paged.h"
 
@@ -66,14 +67,21 @@ __device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* u
   return *unit < T;
 }
 
+// Chunk swizzle of a key's row in LDS.  Rows of 64 bytes lie four to the banks' 256: a
+// K read's 16 rows then take each chunk four times, and neighbouring groups of four
+// rows, which a transposing V read takes two chunks of, the other two.
+template <int HD> __device__ __forceinline__ int tile_swz(int row) {
+  return HD == 32 ? ((row >> 1) & 2) | ((row >> 3) & 1) : row & 7;
+}
+
 // What a launch holds (compiled apart: the choices cost 8 % inside the key loop).
 enum TileMode { kOwnRows, kFlatRows, kBoth };
 
 template <typename T, int HD, int QTW, TileMode MODE, bool A16, int STAGES>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 && STAGES == 2 ? 3 : HD == 64 || STAGES == 2 ? 2 : 1, 4))) void
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD <= 64 && STAGES == 2 ? 3 : HD <= 64 || STAGES == 2 ? 2 : 1, 4))) void
 paged_tile_kernel(PagedAttnArgs a, TileJob job) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  static_assert(sizeof(T) == 2 && (HD == 64 || HD == 128), "16-bit types, head_dim 64 or 128");
+  static_assert(sizeof(T) == 2 && (HD == 32 || HD == 64 || HD == 128), "16-bit types, head_dim 32, 64 or 128");
   constexpr int QT = QTW, BQ = 64 * QTW, BKV = kTileKeys, NWAVE = 4;
   constexpr int KROW = HD * 2, CPR = KROW / 16, RPI = 64 / CPR;  // bytes, chunks of a row; rows of a 1 KiB load
   constexpr int XB = BKV * KROW, STAGE = 2 * XB;
@@ -155,7 +163,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
         p = 0;
         bad = true;
       }
-      const int chunk = (slot16 ^ (row & 7)) << 4;
+      const int chunk = (slot16 ^ tile_swz<HD>(row)) << 4;
       const uint32_t lds = (ii * NWAVE + wave) * 1024;
       dma_lds16_at(kh + 2 * (p * a.kc.sp) + 2 * (slot * a.kc.ss) + chunk, lds_addr(buf + lds));
       dma_lds16_at(vh + 2 * (p * a.vc.sp) + 2 * (slot * a.vc.ss) + chunk, lds_addr(buf + XB + lds));
@@ -235,7 +243,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
           const int key = kt * 16 + frow, c = 4 * ks + g;
-          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ (key & 7)) << 4));
+          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ tile_swz<HD>(key)) << 4));
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(kf, qf[qt][ks], s[qt][kt]);
         }
@@ -315,8 +323,8 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
                              pack2<T>(s[qt][2 * c + 1][2], s[qt][2 * c + 1][3])};
 #pragma unroll
           for (int dt = 0; dt < ND; ++dt) {
-            const u32x2_t lo = vt_read<KROW, 7>(sv, 32 * c + tr_row, dt, frow);
-            const u32x2_t hi = vt_read<KROW, 7>(sv, 32 * c + 16 + tr_row, dt, frow);
+            const u32x2_t lo = vt_read<KROW>(sv, 32 * c + tr_row, tile_swz<HD>(tr_row), dt, frow);
+            const u32x2_t hi = vt_read<KROW>(sv, 32 * c + 16 + tr_row, tile_swz<HD>(tr_row), dt, frow);
             u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
             if constexpr (decltype(clean)::value)
 #pragma unroll
@@ -423,7 +431,7 @@ static int launch_tile(const PagedAttnArgs& a, TileJob job, hipStream_t s) {
   } while (0)
   if (!a16)
     CGPT_TILE(false, 2);
-  else if (QTW == 1 && blocks <= (HD == 64 ? 2 : 1) * num_cus())
+  else if (QTW == 1 && blocks <= (HD <= 64 ? 2 : 1) * num_cus())
     // Few blocks: little else on the CU hides the loads, so three blocks of keys are kept
     // on their way.
     CGPT_TILE(true, (QTW == 1 ? 4 : 2));
@@ -443,11 +451,13 @@ int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const
   if (dtype == CGPT_BF16 && head_dim == 128) return launch_tile_qt<bf16_t, 128>(a, job, qt, s);
   if (dtype == CGPT_F16 && head_dim == 64) return launch_tile_qt<f16_t, 64>(a, job, qt, s);
   if (dtype == CGPT_F16 && head_dim == 128) return launch_tile_qt<f16_t, 128>(a, job, qt, s);
+  if (dtype == CGPT_BF16 && head_dim == 32) return launch_tile_qt<bf16_t, 32>(a, job, qt, s);
+  if (dtype == CGPT_F16 && head_dim == 32) return launch_tile_qt<f16_t, 32>(a, job, qt, s);
   return CGPT_EDTYPE;
 }
 
 bool paged_tile_ok(int64_t dtype, int head_dim) {
-  return dtype != CGPT_F32 && (head_dim == 64 || head_dim == 128);
+  return dtype != CGPT_F32 && head_dim >= 32;
 }
 
 }  // namespace cgpt

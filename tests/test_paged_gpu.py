@@ -262,11 +262,12 @@ def test_rows_without_a_key(gpu, new, room):
 @pytest.mark.parametrize("new", [1, 12, 90])
 @pytest.mark.parametrize("Hkv", [1, 4])
 @pytest.mark.parametrize("what", [NAN, float("inf"), -float("inf")])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
 @WIDE
-def test_masked_values_do_not_leak(gpu, dtype, new, Hkv, what, room):
+def test_masked_values_do_not_leak(gpu, dtype, new, Hkv, what, hd, room):
     """What a row may not see has no part in it: keys and values that later tokens of the same
     step brought, whatever they hold."""
-    p = Problem(dtype, 64, 16, 4, Hkv, ctx=[0, 21], new=[new, new], seed=12, spare_cols=cols(room, 16))
+    p = Problem(dtype, hd, 16, 4, Hkv, ctx=[0, 21], new=[new, new], seed=12, spare_cols=cols(room, 16))
     poison = max(0, new - 3)
     for b in range(2):
         for pos in range(p.ctx[b] + poison + 1, p.total[b]):
@@ -283,13 +284,14 @@ def test_masked_values_do_not_leak(gpu, dtype, new, Hkv, what, room):
 @WIDE
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("new", [1, 30])
-def test_value_of_a_seen_key_counts_whatever_it_is(gpu, dtype, new, room):
-    p = Problem(dtype, 64, 16, 2, 2, ctx=[40], new=[new], seed=13, spare_cols=cols(room, 16))
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+def test_value_of_a_seen_key_counts_whatever_it_is(gpu, dtype, new, hd, room):
+    p = Problem(dtype, hd, 16, 2, 2, ctx=[40], new=[new], seed=13, spare_cols=cols(room, 16))
     p.v_cache[int(p.table[0, 0]), :, 3, 9] = float("inf")
     p.v_cache[int(p.table[0, 1]), :, 3, 11] = NAN
     got = run_attention(p, gpu).float().cpu()
     assert (got[:, :, 9] == float("inf")).all() and torch.isnan(got[:, :, 11]).all()
-    rest = [d for d in range(64) if d not in (9, 11)]
+    rest = [d for d in range(hd) if d not in (9, 11)]
     want, bound = attention(p)
     within(got[:, :, rest], want[:, :, rest], bound[:, :, rest])
 
