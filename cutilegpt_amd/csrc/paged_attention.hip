@@ -769,6 +769,10 @@ constexpr int64_t shared_rows(int64_t prefix_len, int hd) {
   return r < 96 ? 96 : r > 4 * hd ? 4 * hd : r;
 }
 constexpr int64_t kOwnKeys = 4096;
+// Where the fp32 products are the bound and a tile's empty rows cost: from head_dim 64 on.
+template <typename T, int HD> constexpr bool kDear = sizeof(T) == 4 && HD >= 64;
+// The types that leave more than 16 rows of a sequence to the stream kernel.
+template <typename T, int HD> constexpr bool kWide = kDear<T, HD> || !paged_tile_ok(sizeof(T), HD);
 
 template <typename T, int HD>
 static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
@@ -789,27 +793,35 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     p->grid = static_cast<int>(items);
     return CGPT_OK;
   }
-  if (paged_tile_ok(call.dtype, HD) && rows > 16) {
+  // Rows that the tile kernel takes: more than 16 a sequence, or a batch's against a prefix.
+  // Where empty rows cost, more than 32 a sequence (100 sequences of up to 2000 keys, 1 to 2
+  // tokens, 16 heads to a key head of 64: 120 us by the stream kernel, 173 in tiles; 24 of up
+  // to 64 tokens behind 2048, 12 heads: 144 and 89), or a full tile of rows against 1024 keys
+  // (20 rows, 12 heads, 16000 keys: 46 and 58; 100 rows, 500 keys: 36 and 45; 64 rows, 25
+  // heads, 4096 keys: 116 and 89).
+  constexpr bool dear = kDear<T, HD>;
+  const bool tall = rows > (dear ? 32 : 16) * B;
+  if (paged_tile_ok(sizeof(T), HD) &&
+      (tall || (prefix_len > 0 && (dear ? rows >= 64 && prefix_len >= 1024 : rows > 16)))) {
     const bool flat = prefix_len > 0 && rows <= shared_rows(prefix_len, HD) * B;
-    const int64_t keys = flat ? prefix_len : cap;
     auto blocks = [&](int64_t bq) { return Hkv * (flat ? (rows + bq - 1) / bq : rows / bq + B); };
     // 128-row tiles where there are four of them a CU, or at head_dim 128 against a prefix
     // (32768 keys, 512 rows a head: 188 us, 218 in tiles of 64; at head_dim 64 tiles of 64
-    // rows win up to 2048 rows, 61 us against 65), else 64.  The keys are split, 256 a part at least,
-    // while a CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12
+    // rows win up to 2048 rows, 61 us against 65), else 64.  The keys are split, 256 a part at
+    // least (128 of fp32 rows of 128: 64 tokens behind 1000, 12 heads 34 -> 23 us), while a CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12
     // heads of head_dim 64: 55 us whole, 43 in 3 parts; of up to 512: 67 whole, 86 in 2) or
     // the resident number of prefix rows, whose partials are many.
     p->tile_qt = blocks(128) >= 4 * cus || (flat && HD == 128 && rows > 128) ? 2 : 1;
     const int64_t BQ = 64 * p->tile_qt;
     auto parts = [&](int64_t n, int64_t room, int64_t of) {
-      return static_cast<int>(std::max<int64_t>(1, std::min(room * cus / n, of / 256)));
+      return static_cast<int>(std::max<int64_t>(1, std::min(room * cus / n, of / (dear && HD == 128 && !flat ? 128 : 256))));
     };
     // A sequence's own keys behind a prefix go by the same launch, even for a single row
     // (64 sequences, 25 heads, 4096 keys shared: 64 keys of their own 42 -> 36 us, 512 69 ->
     // 60, 2048 159 -> 153), unless its tiles have 128 rows (128 sequences, 8 heads of
     // head_dim 128, 2048 keys: 226 us, 211 by the stream kernel) or one sequence may have
     // so many that its few blocks end last.
-    const bool own = rows > 16 * B || (flat && p->tile_qt == 1 && cap - prefix_len <= kOwnKeys);
+    const bool own = tall || (flat && !dear && p->tile_qt == 1 && cap - prefix_len <= kOwnKeys);
     const int64_t n_own = Hkv * (rows / BQ + B);
     if (flat) p->flat_split = parts(blocks(BQ), HD <= 64 ? 4 : 2, prefix_len);
     if (own) p->split = parts(n_own, 6, cap - (flat ? prefix_len : 0));
@@ -821,7 +833,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
   if (p->split == 0) {
     // 64-row tiles (32 at head_dim 128, whose accumulators are twice as wide) where a
     // sequence, or the batch against its prefix, has more than 16 rows a key head.
-    const bool flat = p->flat_split > 0, wide = !flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
+    const bool flat = p->flat_split > 0, wide = kWide<T, HD> && !flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
     p->stream_qt = wide ? (HD == 128 ? 2 : 4) : 1;
     const int64_t R = 16 * p->stream_qt;
     const int64_t UK = wide ? StreamShape<T, HD, 1, 4>::UK : StreamShape<T, HD, 1, stream_waves(HD)>::UK;
@@ -879,7 +891,6 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
   auto f32 = [&](int64_t o) { return reinterpret_cast<float*>(w + o); };
   const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), f32(p.o_eml), f32(p.o_eo), f32(p.o_wml), f32(p.o_wo),
                    f32(p.o_tml), f32(p.o_to)};
-  constexpr int WIDE = HD == 128 ? 2 : 4;
   if (p.flat_split + p.split > 0) {
     TileJob job{};
     if (p.n_tile > 0) {
@@ -896,12 +907,15 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
     launch_stream<T, HD, 1, whole_waves(HD), true>(a, ws, p, s);
     return hip_status(hipGetLastError());
   }
+  if constexpr (kWide<T, HD>) {
+    if (p.stream_qt > 1) {
+      constexpr int QT = HD == 128 ? 2 : 4;
+      launch_stream<T, HD, QT, 4, false>(a, ws, p, s);
+      launch_join<T, HD, QT, 4>(a, ws, p, s);
+    }
+  }
   if (p.stream_qt == 1) launch_stream<T, HD, 1, stream_waves(HD), false>(a, ws, p, s);
-  if (p.stream_qt > 1) launch_stream<T, HD, WIDE, 4, false>(a, ws, p, s);
-  if (p.stream_qt > 1)
-    launch_join<T, HD, WIDE, 4>(a, ws, p, s);
-  else if (p.stream_qt == 1 || p.n_tile > 0)
-    launch_join<T, HD, 1, stream_waves(HD)>(a, ws, p, s);
+  if (p.stream_qt == 1 || (p.stream_qt == 0 && p.n_tile > 0)) launch_join<T, HD, 1, stream_waves(HD)>(a, ws, p, s);
   return hip_status(hipGetLastError());
 }
 

@@ -8,9 +8,9 @@
 // used.  The page ids are read one block of keys ahead of the loads that need them: where
 // a page is a multiple of 16 keys (A16) by scalar loads, which do not queue with the
 // key loads, so more than one block may be on its way.
-// S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs as in cgpt_attention_fwd's kernel: a
-// lane owns one query row, P goes from the accumulators straight into the second
-// product, V is transposed by the LDS read.
+// S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs (fp32: 16x16x4) as in cgpt_attention_fwd's
+// kernel: a lane owns one query row, P goes from the accumulators straight into the second
+// product, V is transposed by the LDS read (fp32: read word by word).
 //
 // Bound: the exponentials.  A P costs an FMA, an exponential (a quarter of the rate), an
 // add and half a conversion, 26 cycles a 64 of them, against 16 on the matrix cores at
@@ -19,7 +19,9 @@
 // matrix cores 26 % of the time.  128 rows a block (two sub-tiles a wave) use a loaded
 // key for twice the rows of 64; blocks of eight waves with 128 or 256 rows were slower
 // (350 and 412 us), and 128 registers, for four waves a SIMD, spill (524 us).  At head_dim
-// 32 the same chunks take 236 us, 561 by the stream kernel.
+// 32 the same chunks take 236 us, 561 by the stream kernel.  fp32 is bound by its products:
+// 1896 us at head_dim 64, 99 TFLOP/s where a large product reaches 153 (2227 by the stream
+// kernel), 3940 at 128 (6570).
 #include "internal.h"
 #include "paged.h"
 
@@ -70,23 +72,28 @@ __device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* u
 // Chunk swizzle of a key's row in LDS.  Rows of 64 bytes lie four to the banks' 256: a
 // K read's 16 rows then take each chunk four times, and neighbouring groups of four
 // rows, which a transposing V read takes two chunks of, the other two.
-template <int HD> __device__ __forceinline__ int tile_swz(int row) {
-  return HD == 32 ? ((row >> 1) & 2) | ((row >> 3) & 1) : row & 7;
+template <int KROW> __device__ __forceinline__ int tile_swz(int row) {
+  return KROW == 64 ? ((row >> 1) & 2) | ((row >> 3) & 1) : row & (KROW >= 256 ? 15 : 7);
+}
+// And of V's: fp32 columns are read by four lane groups, four rows apart and 64 bytes wide each.
+template <typename T, int KROW> __device__ __forceinline__ int tile_vswz(int row) {
+  return sizeof(T) == 2 ? tile_swz<KROW>(row) : row & 12 & (KROW / 16 - 1);
 }
 
 // What a launch holds (compiled apart: the choices cost 8 % inside the key loop).
 enum TileMode { kOwnRows, kFlatRows, kBoth };
 
 template <typename T, int HD, int QTW, TileMode MODE, bool A16, int STAGES>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(HD <= 64 && STAGES == 2 ? 3 : HD <= 64 || STAGES == 2 ? 2 : 1, 4))) void
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? (HD <= 32 ? 3 : HD == 64 ? 2 : 1) : HD <= 64 && STAGES == 2 ? 3 : HD <= 64 || STAGES == 2 ? 2 : 1, 4))) void
 paged_tile_kernel(PagedAttnArgs a, TileJob job) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  static_assert(sizeof(T) == 2 && (HD == 32 || HD == 64 || HD == 128), "16-bit types, head_dim 32, 64 or 128");
   constexpr int QT = QTW, BQ = 64 * QTW, BKV = kTileKeys, NWAVE = 4;
-  constexpr int KROW = HD * 2, CPR = KROW / 16, RPI = 64 / CPR;  // bytes, chunks of a row; rows of a 1 KiB load
+  constexpr int ES = sizeof(T), EPC = 16 / ES;
+  constexpr int KROW = HD * ES, CPR = KROW / 16, RPI = 64 / CPR;  // bytes, chunks of a row; rows of a 1 KiB load
+  static_assert(KROW >= 64, "a wave loads whole KiBs of K and of V");
   constexpr int XB = BKV * KROW, STAGE = 2 * XB;
   constexpr int INS = XB / 1024 / NWAVE;                         // loads a wave makes of K (and of V) a block
-  constexpr int NKS = HD / 32, ND = HD / 16;
+  constexpr int NKS = HD / (4 * EPC), ND = HD / 16;
   constexpr int LPS = 2 * INS;                                   // and of both
   static_assert(A16 || STAGES == 2, "page ids by vector loads drain the queue at every block");
   __shared__ __attribute__((aligned(1024))) uint8_t smem[STAGES * STAGE];
@@ -163,10 +170,10 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
         p = 0;
         bad = true;
       }
-      const int chunk = (slot16 ^ tile_swz<HD>(row)) << 4;
+      const int k_chunk = (slot16 ^ tile_swz<KROW>(row)) << 4, v_chunk = (slot16 ^ tile_vswz<T, KROW>(row)) << 4;
       const uint32_t lds = (ii * NWAVE + wave) * 1024;
-      dma_lds16_at(kh + 2 * (p * a.kc.sp) + 2 * (slot * a.kc.ss) + chunk, lds_addr(buf + lds));
-      dma_lds16_at(vh + 2 * (p * a.vc.sp) + 2 * (slot * a.vc.ss) + chunk, lds_addr(buf + XB + lds));
+      dma_lds16_at(kh + ES * (p * a.kc.sp) + ES * (slot * a.kc.ss) + k_chunk, lds_addr(buf + lds));
+      dma_lds16_at(vh + ES * (p * a.vc.sp) + ES * (slot * a.vc.ss) + v_chunk, lds_addr(buf + XB + lds));
     }
   };
 
@@ -203,7 +210,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
     const T* qp = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) {
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + (4 * ks + g) * 8);
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + (4 * ks + g) * EPC);
       qf[qt][ks] = live ? v : u32x4_t{0, 0, 0, 0};
     }
   }
@@ -243,7 +250,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
           const int key = kt * 16 + frow, c = 4 * ks + g;
-          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ tile_swz<HD>(key)) << 4));
+          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ tile_swz<KROW>(key)) << 4));
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(kf, qf[qt][ks], s[qt][kt]);
         }
@@ -313,28 +320,53 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
       // the rows that see them.
       uint32_t bits = 0;
       auto pv = [&](auto clean) __attribute__((always_inline)) {
+        if constexpr (ES == 2) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          u32x4_t pf[QT];
+          for (int c = 0; c < 2; ++c) {
+            u32x4_t pf[QT];
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-            pf[qt] = u32x4_t{pack2<T>(s[qt][2 * c][0], s[qt][2 * c][1]), pack2<T>(s[qt][2 * c][2], s[qt][2 * c][3]),
-                             pack2<T>(s[qt][2 * c + 1][0], s[qt][2 * c + 1][1]),
-                             pack2<T>(s[qt][2 * c + 1][2], s[qt][2 * c + 1][3])};
+            for (int qt = 0; qt < QT; ++qt)
+              pf[qt] = u32x4_t{pack2<T>(s[qt][2 * c][0], s[qt][2 * c][1]), pack2<T>(s[qt][2 * c][2], s[qt][2 * c][3]),
+                               pack2<T>(s[qt][2 * c + 1][0], s[qt][2 * c + 1][1]),
+                               pack2<T>(s[qt][2 * c + 1][2], s[qt][2 * c + 1][3])};
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) {
-            const u32x2_t lo = vt_read<KROW>(sv, 32 * c + tr_row, tile_swz<HD>(tr_row), dt, frow);
-            const u32x2_t hi = vt_read<KROW>(sv, 32 * c + 16 + tr_row, tile_swz<HD>(tr_row), dt, frow);
-            u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
-            if constexpr (decltype(clean)::value)
+            for (int dt = 0; dt < ND; ++dt) {
+              const u32x2_t lo = vt_read<KROW>(sv, 32 * c + tr_row, tile_vswz<T, KROW>(tr_row), dt, frow);
+              const u32x2_t hi = vt_read<KROW>(sv, 32 * c + 16 + tr_row, tile_vswz<T, KROW>(tr_row), dt, frow);
+              u32x4_t w = {lo[0], lo[1], hi[0], hi[1]};
+              if constexpr (decltype(clean)::value)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  bits |= special_bits<T>(w[e]);
+                  w[e] = finite_part<T>(w[e]);
+                }
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(w, pf[qt], o[qt][dt]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+              u32x4_t w;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                bits |= special_bits<T>(w[e]);
-                w[e] = finite_part<T>(w[e]);
+                const int key = 16 * kt + 4 * g + e, d = 16 * dt + frow;
+                w[e] = *reinterpret_cast<const uint32_t*>(sv + key * KROW + (((d >> 2) ^ tile_vswz<T, KROW>(key)) << 4) +
+                                                          4 * (d & 3));
+                if constexpr (decltype(clean)::value) {
+                  bits |= special_bits<T>(w[e]);
+                  w[e] = finite_part<T>(w[e]);
+                }
               }
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(w, pf[qt], o[qt][dt]);
-          }
+              for (int qt = 0; qt < QT; ++qt) {
+                const u32x4_t pf = {__float_as_uint(s[qt][kt][0]), __float_as_uint(s[qt][kt][1]),
+                                    __float_as_uint(s[qt][kt][2]), __float_as_uint(s[qt][kt][3])};
+                Mfma<T>::run(w, pf, o[qt][dt]);
+              }
+            }
         }
       };
       if (masked) {
@@ -431,10 +463,10 @@ static int launch_tile(const PagedAttnArgs& a, TileJob job, hipStream_t s) {
   } while (0)
   if (!a16)
     CGPT_TILE(false, 2);
-  else if (QTW == 1 && blocks <= (HD <= 64 ? 2 : 1) * num_cus())
+  else if (sizeof(T) == 2 && QTW == 1 && blocks <= (HD <= 64 ? 2 : 1) * num_cus())
     // Few blocks: little else on the CU hides the loads, so three blocks of keys are kept
     // on their way.
-    CGPT_TILE(true, (QTW == 1 ? 4 : 2));
+    CGPT_TILE(true, (sizeof(T) == 2 && QTW == 1 ? 4 : 2));
   else
     CGPT_TILE(true, 2);
 #undef CGPT_TILE
@@ -453,11 +485,11 @@ int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const
   if (dtype == CGPT_F16 && head_dim == 128) return launch_tile_qt<f16_t, 128>(a, job, qt, s);
   if (dtype == CGPT_BF16 && head_dim == 32) return launch_tile_qt<bf16_t, 32>(a, job, qt, s);
   if (dtype == CGPT_F16 && head_dim == 32) return launch_tile_qt<f16_t, 32>(a, job, qt, s);
+  if (dtype == CGPT_F32 && head_dim == 16) return launch_tile_qt<float, 16>(a, job, qt, s);
+  if (dtype == CGPT_F32 && head_dim == 32) return launch_tile_qt<float, 32>(a, job, qt, s);
+  if (dtype == CGPT_F32 && head_dim == 64) return launch_tile_qt<float, 64>(a, job, qt, s);
+  if (dtype == CGPT_F32 && head_dim == 128) return launch_tile_qt<float, 128>(a, job, qt, s);
   return CGPT_EDTYPE;
-}
-
-bool paged_tile_ok(int64_t dtype, int head_dim) {
-  return dtype != CGPT_F32 && head_dim >= 32;
 }
 
 }  // namespace cgpt
