@@ -11,8 +11,8 @@
 // the unrounded ones.
 //
 // Three kernels: the stream kernel here for few rows (a decode step reads every key once:
-// the bound is HBM), the tile kernel (paged_tile.hip) for many, the join of their
-// partials.  make_plan below chooses.  Measured: 64 sequences of 1 to 8192 keys, 25 heads
+// the bound is HBM), the tile kernel (paged_tile.hip) for many (16-bit rows of head_dim 16
+// apart, which stay here), the join of their partials.  make_plan below chooses.  Measured: 64 sequences of 1 to 8192 keys, 25 heads
 // of head_dim 64, bf16 294 us, 5.7 TB/s; four of 90 to 130 thousand, 8 heads of 128, fp16
 // 308 us, 5.8 TB/s (a large copy reaches 4.9 on the same card); one of 500 keys 8 us.
 #include <algorithm>
@@ -808,9 +808,10 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     // 128-row tiles where there are four of them a CU, or at head_dim 128 against a prefix
     // (32768 keys, 512 rows a head: 188 us, 218 in tiles of 64; at head_dim 64 tiles of 64
     // rows win up to 2048 rows, 61 us against 65), else 64.  The keys are split, 256 a part at
-    // least (128 of fp32 rows of 128: 64 tokens behind 1000, 12 heads 34 -> 23 us), while a CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12
-    // heads of head_dim 64: 55 us whole, 43 in 3 parts; of up to 512: 67 whole, 86 in 2) or
-    // the resident number of prefix rows, whose partials are many.
+    // least (128 of fp32 rows of 128: 64 tokens behind 1000, 12 heads 34 -> 23 us), while a
+    // CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12 heads of
+    // head_dim 64: 55 us whole, 43 in 3 parts; of up to 512: 67 whole, 86 in 2) or the
+    // resident number of prefix rows, whose partials are many.
     p->tile_qt = blocks(128) >= 4 * cus || (flat && HD == 128 && rows > 128) ? 2 : 1;
     const int64_t BQ = 64 * p->tile_qt;
     auto parts = [&](int64_t n, int64_t room, int64_t of) {
