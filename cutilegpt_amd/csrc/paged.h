@@ -69,8 +69,6 @@ struct TileJob {
   int flat_split, split, from;
   int flat_tiles, tiles, flat_blocks;
 };
-// What it takes: rows of at least 64 bytes.
-constexpr bool paged_tile_ok(int elem_size, int head_dim) { return elem_size * head_dim >= 64; }
 // qt: 16-row sub-tiles of each of a block's four waves, 1 or 2.
 int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const TileJob& job, int qt, hipStream_t s);
 

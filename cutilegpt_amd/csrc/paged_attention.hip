@@ -11,8 +11,8 @@
 // the unrounded ones.
 //
 // Three kernels: the stream kernel here for few rows (a decode step reads every key once:
-// the bound is HBM), the tile kernel (paged_tile.hip) for many (16-bit rows of head_dim 16
-// apart, which stay here), the join of their partials.  make_plan below chooses.  Measured: 64 sequences of 1 to 8192 keys, 25 heads
+// the bound is HBM), the tile kernel (paged_tile.hip) for many, the join of their
+// partials.  make_plan below chooses.  Measured: 64 sequences of 1 to 8192 keys, 25 heads
 // of head_dim 64, bf16 294 us, 5.7 TB/s; four of 90 to 130 thousand, 8 heads of 128, fp16
 // 308 us, 5.8 TB/s (a large copy reaches 4.9 on the same card); one of 500 keys 8 us.
 #include <algorithm>
@@ -771,8 +771,6 @@ constexpr int64_t shared_rows(int64_t prefix_len, int hd) {
 constexpr int64_t kOwnKeys = 4096;
 // Where the fp32 products are the bound and a tile's empty rows cost: from head_dim 64 on.
 template <typename T, int HD> constexpr bool kDear = sizeof(T) == 4 && HD >= 64;
-// The types that leave more than 16 rows of a sequence to the stream kernel.
-template <typename T, int HD> constexpr bool kWide = kDear<T, HD> || !paged_tile_ok(sizeof(T), HD);
 
 template <typename T, int HD>
 static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
@@ -801,8 +799,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
   // heads, 4096 keys: 116 and 89).
   constexpr bool dear = kDear<T, HD>;
   const bool tall = rows > (dear ? 32 : 16) * B;
-  if (paged_tile_ok(sizeof(T), HD) &&
-      (tall || (prefix_len > 0 && (dear ? rows >= 64 && prefix_len >= 1024 : rows > 16)))) {
+  if (tall || (prefix_len > 0 && (dear ? rows >= 64 && prefix_len >= 1024 : rows > 16))) {
     const bool flat = prefix_len > 0 && rows <= shared_rows(prefix_len, HD) * B;
     auto blocks = [&](int64_t bq) { return Hkv * (flat ? (rows + bq - 1) / bq : rows / bq + B); };
     // 128-row tiles where there are four of them a CU, or at head_dim 128 against a prefix
@@ -834,7 +831,7 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
   if (p->split == 0) {
     // 64-row tiles (32 at head_dim 128, whose accumulators are twice as wide) where a
     // sequence, or the batch against its prefix, has more than 16 rows a key head.
-    const bool flat = p->flat_split > 0, wide = kWide<T, HD> && !flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
+    const bool flat = p->flat_split > 0, wide = kDear<T, HD> && !flat && (prefix_len > 0 ? rows > 16 : rows > 16 * B);
     p->stream_qt = wide ? (HD == 128 ? 2 : 4) : 1;
     const int64_t R = 16 * p->stream_qt;
     const int64_t UK = wide ? StreamShape<T, HD, 1, 4>::UK : StreamShape<T, HD, 1, stream_waves(HD)>::UK;
@@ -908,7 +905,7 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
     launch_stream<T, HD, 1, whole_waves(HD), true>(a, ws, p, s);
     return hip_status(hipGetLastError());
   }
-  if constexpr (kWide<T, HD>) {
+  if constexpr (kDear<T, HD>) {
     if (p.stream_qt > 1) {
       constexpr int QT = HD == 128 ? 2 : 4;
       launch_stream<T, HD, QT, 4, false>(a, ws, p, s);

@@ -19,7 +19,7 @@
 // matrix cores 26 % of the time.  128 rows a block (two sub-tiles a wave) use a loaded
 // key for twice the rows of 64; blocks of eight waves with 128 or 256 rows were slower
 // (350 and 412 us), and 128 registers, for four waves a SIMD, spill (524 us).  At head_dim
-// 32 the same chunks take 236 us, 561 by the stream kernel.  fp32 is bound by its products:
+// 32 the same chunks take 236 us, 561 by the stream kernel, at 16 215 and 548.  fp32 is bound by its products:
 // 1896 us at head_dim 64, 99 TFLOP/s where a large product reaches 153 (2227 by the stream
 // kernel), 3940 at 128 (6570).
 #include "internal.h"
@@ -71,8 +71,10 @@ __device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* u
 
 // Chunk swizzle of a key's row in LDS.  Rows of 64 bytes lie four to the banks' 256: a
 // K read's 16 rows then take each chunk four times, and neighbouring groups of four
-// rows, which a transposing V read takes two chunks of, the other two.
+// rows, which a transposing V read takes two chunks of, the other two.  Of 32-byte rows the
+// first eight and the next take the other chunk.
 template <int KROW> __device__ __forceinline__ int tile_swz(int row) {
+  if (KROW == 32) return (row >> 3) & 1;
   return KROW == 64 ? ((row >> 1) & 2) | ((row >> 3) & 1) : row & (KROW >= 256 ? 15 : 7);
 }
 // And of V's: fp32 columns are read by four lane groups, four rows apart and 64 bytes wide each.
@@ -90,11 +92,12 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
   constexpr int QT = QTW, BQ = 64 * QTW, BKV = kTileKeys, NWAVE = 4;
   constexpr int ES = sizeof(T), EPC = 16 / ES;
   constexpr int KROW = HD * ES, CPR = KROW / 16, RPI = 64 / CPR;  // bytes, chunks of a row; rows of a 1 KiB load
-  static_assert(KROW >= 64, "a wave loads whole KiBs of K and of V");
   constexpr int XB = BKV * KROW, STAGE = 2 * XB;
-  constexpr int INS = XB / 1024 / NWAVE;                         // loads a wave makes of K (and of V) a block
-  constexpr int NKS = HD / (4 * EPC), ND = HD / 16;
-  constexpr int LPS = 2 * INS;                                   // and of both
+  constexpr bool HALF = KROW == 32;                              // two waves load K, two V; else each both
+  constexpr int INS = HALF ? 1 : XB / 1024 / NWAVE;              // loads a wave makes of K (and of V) a block
+  constexpr int NKS = (HD + 4 * EPC - 1) / (4 * EPC), ND = HD / 16;
+  constexpr int LPS = HALF ? 1 : 2 * INS;                        // and of both
+  static_assert(CPR % 4 == 0 || HALF, "a lane group has a chunk in every slab, or two of the four do");
   static_assert(A16 || STAGES == 2, "page ids by vector loads drain the queue at every block");
   __shared__ __attribute__((aligned(1024))) uint8_t smem[STAGES * STAGE];
 
@@ -142,13 +145,13 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
             per = (n_kv + n_split - 1) / n_split;
   const int j0 = jb + split * per, j1 = min(j0 + per, jb + n_kv);
 
-  const int lrow = lane / CPR, slot16 = lane % CPR;
+  const int lrow = lane / CPR, slot16 = lane % CPR, part = HALF ? wave & 1 : wave;
   const uint8_t* const kh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.kc.base) + hk * a.kc.sh);
   const uint8_t* const vh = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.vc.base) + hk * a.vc.sh);
   int pg[INS];
   // First key of load ii of block j (one page's, A16), or the lane's own.
   auto key_of = [&](int j, int ii) __attribute__((always_inline)) {
-    const int key = j * BKV + (ii * NWAVE + wave) * RPI;
+    const int key = j * BKV + (ii * NWAVE + part) * RPI;
     const int k = A16 ? min(key, (n - 1) & ~(RPI - 1)) : min(key + lrow, n - 1);
     return MODE == kBoth ? max(k, kb) : k;
   };
@@ -163,7 +166,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
   auto issue = [&](int j, uint8_t* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int ii = 0; ii < INS; ++ii) {
-      const int row = (ii * NWAVE + wave) * RPI + lrow, key = key_of(j, ii);
+      const int row = (ii * NWAVE + part) * RPI + lrow, key = key_of(j, ii);
       const int slot = (A16 ? min(key + lrow, n - 1) : key) - a.seq.page.div(key) * page_size;
       int p = pg[ii];
       if (static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.seq.n_pages)) {
@@ -171,9 +174,11 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
         bad = true;
       }
       const int k_chunk = (slot16 ^ tile_swz<KROW>(row)) << 4, v_chunk = (slot16 ^ tile_vswz<T, KROW>(row)) << 4;
-      const uint32_t lds = (ii * NWAVE + wave) * 1024;
-      dma_lds16_at(kh + ES * (p * a.kc.sp) + ES * (slot * a.kc.ss) + k_chunk, lds_addr(buf + lds));
-      dma_lds16_at(vh + ES * (p * a.vc.sp) + ES * (slot * a.vc.ss) + v_chunk, lds_addr(buf + XB + lds));
+      const uint32_t lds = (ii * NWAVE + part) * 1024;
+      if (!HALF || wave < 2)
+        dma_lds16_at(kh + ES * (p * a.kc.sp) + ES * (slot * a.kc.ss) + k_chunk, lds_addr(buf + lds));
+      if (!HALF || wave >= 2)
+        dma_lds16_at(vh + ES * (p * a.vc.sp) + ES * (slot * a.vc.ss) + v_chunk, lds_addr(buf + XB + lds));
     }
   };
 
@@ -210,8 +215,8 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
     const T* qp = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) {
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + (4 * ks + g) * EPC);
-      qf[qt][ks] = live ? v : u32x4_t{0, 0, 0, 0};
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + (HALF ? g & 1 : 4 * ks + g) * EPC);
+      qf[qt][ks] = live && (!HALF || g < 2) ? v : u32x4_t{0, 0, 0, 0};
     }
   }
   // nm = minus the running maximum of a row's scaled scores, +inf while it has none.
@@ -249,8 +254,9 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
       for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-          const int key = kt * 16 + frow, c = 4 * ks + g;
-          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ tile_swz<KROW>(key)) << 4));
+          const int key = kt * 16 + frow, c = HALF ? g & 1 : 4 * ks + g;
+          u32x4_t kf = *reinterpret_cast<const u32x4_t*>(sk + key * KROW + ((c ^ tile_swz<KROW>(key)) << 4));
+          if (HALF && g >= 2) kf = u32x4_t{0, 0, 0, 0};  // 0 x inf would be NaN
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) Mfma<T>::run(kf, qf[qt][ks], s[qt][kt]);
         }
@@ -447,8 +453,10 @@ static int launch_tile(const PagedAttnArgs& a, TileJob job, hipStream_t s) {
   job.tiles = static_cast<int>(own);
   job.flat_blocks = head_blocks(a.Hkv, job.flat_tiles * job.flat_split);
   const int blocks = job.flat_blocks + head_blocks(a.Hkv, job.tiles * job.split);
-  // 16 keys lie in one page, and on one side of the prefix's end.
-  const bool a16 = a.seq.page.d % 16 == 0 && a.prefix_len % 16 == 0;
+  // The keys of a load (at most 16, 32 of 32-byte rows) lie in one page, and on one side of
+  // the prefix's end.
+  constexpr int RUN = HD * sizeof(T) == 32 ? 32 : 16;
+  const bool a16 = a.seq.page.d % RUN == 0 && a.prefix_len % RUN == 0;
 #define CGPT_TILE(A16, ST)                                                                                           \
   do {                                                                                                               \
     if (own == 0)                                                                                                    \
@@ -485,6 +493,8 @@ int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const
   if (dtype == CGPT_F16 && head_dim == 128) return launch_tile_qt<f16_t, 128>(a, job, qt, s);
   if (dtype == CGPT_BF16 && head_dim == 32) return launch_tile_qt<bf16_t, 32>(a, job, qt, s);
   if (dtype == CGPT_F16 && head_dim == 32) return launch_tile_qt<f16_t, 32>(a, job, qt, s);
+  if (dtype == CGPT_BF16 && head_dim == 16) return launch_tile_qt<bf16_t, 16>(a, job, qt, s);
+  if (dtype == CGPT_F16 && head_dim == 16) return launch_tile_qt<f16_t, 16>(a, job, qt, s);
   if (dtype == CGPT_F32 && head_dim == 16) return launch_tile_qt<float, 16>(a, job, qt, s);
   if (dtype == CGPT_F32 && head_dim == 32) return launch_tile_qt<float, 32>(a, job, qt, s);
   if (dtype == CGPT_F32 && head_dim == 64) return launch_tile_qt<float, 64>(a, job, qt, s);
