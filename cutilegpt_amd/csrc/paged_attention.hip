@@ -804,15 +804,16 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     auto blocks = [&](int64_t bq) { return Hkv * (flat ? (rows + bq - 1) / bq : rows / bq + B); };
     // 128-row tiles where there are four of them a CU, or at head_dim 128 against a prefix
     // (32768 keys, 512 rows a head: 188 us, 218 in tiles of 64; at head_dim 64 tiles of 64
-    // rows win up to 2048 rows, 61 us against 65), else 64.  The keys are split, 256 a part at
-    // least (128 of fp32 rows of 128: 64 tokens behind 1000, 12 heads 34 -> 23 us), while a
-    // CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12 heads of
+    // rows win up to 2048 rows, 61 us against 65; fp32 tiles that sequences leave half empty
+    // too: 24 of up to 64 tokens behind 2048 keys, 12 heads 190 us, 174 in tiles of 64), else
+    // 64.  The keys are split, 256 a part at least (fp32 from head_dim 64 on 128: 64 tokens
+    // behind 1000 keys, 12 heads of 128 34 -> 23 us), while a CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12 heads of
     // head_dim 64: 55 us whole, 43 in 3 parts; of up to 512: 67 whole, 86 in 2) or the
     // resident number of prefix rows, whose partials are many.
-    p->tile_qt = blocks(128) >= 4 * cus || (flat && HD == 128 && rows > 128) ? 2 : 1;
+    p->tile_qt = blocks(128) >= 4 * cus || (flat && HD == 128 && rows > 128 && (!dear || !tall || rows >= 128 * B)) ? 2 : 1;
     const int64_t BQ = 64 * p->tile_qt;
     auto parts = [&](int64_t n, int64_t room, int64_t of) {
-      return static_cast<int>(std::max<int64_t>(1, std::min(room * cus / n, of / (dear && HD == 128 && !flat ? 128 : 256))));
+      return static_cast<int>(std::max<int64_t>(1, std::min(room * cus / n, of / (dear ? 128 : 256))));
     };
     // A sequence's own keys behind a prefix go by the same launch, even for a single row
     // (64 sequences, 25 heads, 4096 keys shared: 64 keys of their own 42 -> 36 us, 512 69 ->
