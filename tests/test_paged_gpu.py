@@ -1,6 +1,8 @@
 """The paged key-value cache on the GPU: every operator against float64 at the sizes,
 lengths, layouts and masks where it can go wrong."""
 
+import random
+
 import pytest
 import torch
 
@@ -229,6 +231,34 @@ def test_shared_prefix_inside_a_page_and_short_sequences(gpu, room, copies):
     flag = torch.zeros(1, dtype=torch.int32, device=gpu)
     again = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, 160, prefix_pages=pages, err_flag=flag)
     assert torch.equal(again, got) and int(flag) == 0
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_mixed_batches(gpu, seed):
+    """Types, heads, pages, lengths (none among them) and prefix ends drawn together, so that
+    the kernels meet in combinations that the tests above take one at a time."""
+    rng = random.Random(seed)
+    B = rng.choice([1, 2, 7, 65, 130])
+    Hkv, G = (rng.choice([1, 2, 3, 5, 9]), rng.choice([1, 2, 3, 8, 17])) if B <= 7 else (rng.choice([1, 2]), rng.choice([1, 2]))
+    page = rng.choice([1, 8, 10, 16, 24, 32, 64, 100, 128])
+    prefix = page * rng.randint(1, max(1, 300 // page)) if rng.random() < 0.6 else 0
+    top = rng.choice([1, 1, 5, 40, 130 if B <= 7 else 9])
+    new = [rng.randint(0 if rng.random() < 0.2 else 1, top) for _ in range(B)]
+    new[0] = max(new[0], 1)
+    ctx = [prefix + rng.randint(0, 200) if b == 0 or rng.random() < 0.8 else rng.randint(0, prefix + 20) for b in range(B)]
+    p = Problem(rng.choice([F32, BF16, F16]), rng.choice([16, 32, 64, 128]), page, Hkv * G, Hkv, ctx=ctx, new=new,
+                prefix=prefix, seed=seed, spare_cols=rng.choice([0, 1, 1 + 300 // page, 1 + 5000 // page]),
+                pad_rows=rng.choice([0, 3]))
+    want, bound = attention(p)
+    d = p.on(gpu)
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    end = max(1, prefix - rng.choice([0, 0, rng.randint(0, page)]))
+    if prefix:
+        got = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, end, cu_q=d.cu, err_flag=flag)
+    else:
+        got = cg.paged_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, cu_q=d.cu, err_flag=flag)
+    within(got, want, bound)
+    assert int(flag) == 0
 
 
 @pytest.mark.parametrize("most", [80, 100])
