@@ -207,6 +207,14 @@ template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t w
   return w & ~(((bits & 0x80000000u) ? 0xffff0000u : 0u) | ((bits & 0x8000u) ? 0xffffu : 0u));
 }
 
+// The largest weight of a row is made 2^kDrop at least and 2^(kDrop + 8) at most (the shift
+// moves up only where it would pass that).  fp16 ends at 2^-24 below and 2^16 above: with
+// weights of 1 and more, keys of 2^-25 and less are lost however many they are (2^17 beside
+// one key in a block: 0.3 % of the result, five of its half steps).  2^7 further up, a key's
+// weight is off by 2^-32 of the largest at most, below the result's half step up to 2^20 keys.
+// The other types reach as far down as fp32 itself.
+template <typename T> constexpr float kDrop = std::is_same<T, f16_t>::value ? 7.f : 0.f;
+
 // Half of a V^T operand: the 16-lane group's lane k points at 4 consecutive d of its
 // row and receives the 4 keys of column 16 dt + k.
 template <int KROW>

@@ -7,8 +7,8 @@
 // Softmax runs in base 2 in one pass over the keys with a running shift m: p = 2^(s
 // scale log2(e) - m), l = sum p, O = sum p v; parts of a row's keys join by m = max m_i,
 // l = sum l_i 2^(m_i - m), O likewise.  m, l, O and the scores are 32-bit; p is rounded to
-// the 16-bit type for the second product (the other operand has no more bits), while l adds
-// the unrounded ones.
+// the 16-bit type for the second product (the other operand has no more bits; kDrop keeps
+// fp16's range from losing small ones), while l adds the unrounded ones.
 //
 // Three kernels: the stream kernel here for few rows (a decode step reads every key once:
 // the bound is HBM), the tile kernel (paged_tile.hip) for many, the join of their
@@ -435,11 +435,11 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[qt][kt][r]);
           mx = column_max(mx) * a.scale_log2;
-          // The shift moves only when the maximum outgrows it by more than 8, so P <= 2^8
-          // and the accumulators are rescaled on few subtiles.
-          const bool grow = mx > m_run[qt] + 8.0f;
+          // The shift moves only when the maximum outgrows it by more than 8 (see kDrop), so
+          // P <= 2^8 and the accumulators are rescaled on few subtiles.
+          const bool grow = mx > m_run[qt] + (8.0f + kDrop<T>);
           if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float m_new = grow ? mx : m_run[qt];
+            const float m_new = grow ? mx - kDrop<T> : m_run[qt];
             const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[qt] - m_new) : 1.0f;
             m_run[qt] = m_new;
             l_run[qt] *= alpha;

@@ -219,7 +219,8 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
       qf[qt][ks] = live && (!HALF || g < 2) ? v : u32x4_t{0, 0, 0, 0};
     }
   }
-  // nm = minus the running maximum of a row's scaled scores, +inf while it has none.
+  // nm = minus the shift of a row's scaled scores (their running maximum, less kDrop), +inf
+  // while it has none.
   f32x4_t o[QT][ND];
   float nm[QT], l_run[QT];
 #pragma unroll
@@ -272,11 +273,11 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
             for (int r = 0; r < 4; ++r)
               s[qt][kt][r] = 16 * kt + r > hi || (MODE == kBoth && 16 * kt + r < lo) ? -INFINITY : s[qt][kt][r];
         }
-      // P against the running maximum as it stands.  A lane whose 16 values sum to at most
-      // 2^7 has none above it, so its maximum need not move; only when some lane fails that
-      // (a NaN sum fails it, and a row without a maximum) is the block's maximum taken and,
-      // where it outgrows the running one by more than 8, the row rescaled and its P
-      // made again.
+      // P against the running shift as it stands.  A lane whose 16 values sum to at most 2^7
+      // (2^14 in fp16, see kDrop) has none above it, so its shift need not move; only when some
+      // lane fails that (a NaN sum fails it, and a row without a maximum) is the block's maximum
+      // taken and, where it outgrows the one behind the shift by more than 8, the row rescaled
+      // and its P made again.
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         float p[4][4], sum = 0.f;
@@ -287,7 +288,7 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
             p[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][kt][r], a.scale_log2, nm[qt]));
             sum += p[kt][r];
           }
-        if (__builtin_amdgcn_ballot_w64(sum <= 128.0f) != __builtin_amdgcn_read_exec()) {
+        if (__builtin_amdgcn_ballot_w64(sum <= (kDrop<T> > 0 ? 16384.0f : 128.0f)) != __builtin_amdgcn_read_exec()) {
           const float m_old = -nm[qt];
           float mx = -INFINITY;
 #pragma unroll
@@ -295,8 +296,8 @@ paged_tile_kernel(PagedAttnArgs a, TileJob job) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[qt][kt][r]);
           mx = column_max(mx) * a.scale_log2;
-          const bool grow = mx > m_old + 8.0f;
-          const float m_new = grow ? mx : m_old;
+          const bool grow = mx > m_old + (8.0f + kDrop<T>);
+          const float m_new = grow ? mx - kDrop<T> : m_old;
           const float alpha = grow ? __builtin_amdgcn_exp2f(m_old - m_new) : 1.0f;
           nm[qt] = m_new == -INFINITY ? INFINITY : -m_new;
           l_run[qt] *= alpha;

@@ -1,6 +1,7 @@
 """The paged key-value cache on the GPU: every operator against float64 at the sizes,
 lengths, layouts and masks where it can go wrong."""
 
+import math
 import random
 
 import pytest
@@ -669,3 +670,41 @@ def test_refusals(gpu):
                    dict(rotary=table[:0]), dict(rotary=table.cpu()), dict(rotary=table[0]),
                    dict(rotary=table.t().contiguous().t())):
         refused(cg.paged_kv_append, args, **change)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("new", [1, 20])
+def test_many_small_weights_add_up(gpu, dtype, hd, new):
+    """One key far above 2^17 others, in as many sequences as leave each to one block: those
+    keys have a weight below the smallest float16 each and a few parts in a thousand
+    together, which the output keeps."""
+    n, gap, B = 2 ** 17, 25.5, 2048
+    half = torch.finfo(dtype).eps / 2
+    cu = torch.arange(B + 1, dtype=torch.int32, device=gpu) * new
+    pages = n // 64
+    table = torch.arange(pages, dtype=torch.int32, device=gpu)[None].expand(B, pages)  # the same for all
+    lens = torch.full((B,), n, dtype=torch.int32, device=gpu)
+    k = torch.zeros(pages, 1, 64, hd, dtype=dtype, device=gpu)
+    k[0, 0, 0, 0] = 8.0
+    q = torch.zeros(B * new, 1, hd, dtype=dtype, device=gpu)
+    q[:, :, 0] = 1.0
+    # Scores 0 and, of the first key, gap in base 2; token i of the step sees n - new + 1 + i keys.
+    scale = gap * math.log(2.0) / 8.0
+    tail = torch.arange(n - new, n, dtype=torch.float64).repeat(B)[:, None, None] * 2.0 ** -gap
+    for first, rest in ((1.0, 1.0), (0.0, 1.0), (1.0, -1.0)):
+        v = torch.full_like(k, rest)
+        v[0, 0, 0] = first
+        got = cg.paged_attention(q, k, v, table, lens, cu_q=cu, scale=scale)
+        want = ((first + rest * tail) / (1.0 + tail)).expand(B * new, 1, hd)
+        # The score in base 2 is off by three roundings of gap in 32 bits, so a weight by
+        # 4 gap 2^-24; the sums of positive terms by 2^-24 for each addition that a term goes
+        # through, in the numerator and the sum: 16 or fewer within one and at most one for each
+        # 16 keys (float32 products are added key by key); the weight by its rounding, half a
+        # step, or in float16's smallest numbers 2^-25 beside a largest weight of 2^7 at least;
+        # then the result's.
+        share = tail / (1.0 + tail)
+        adds = n if dtype == F32 else n / 16 + 16
+        tol = (share * (half + 4 * gap * 2.0 ** -24) + 2 * adds * 2.0 ** -24 * (want.abs() + share)
+               + (n * 2.0 ** -32 if dtype == F16 else 0.0) + half * want.abs())
+        within(got, want, tol.expand_as(want), f"first {first}, rest {rest}")
