@@ -781,14 +781,18 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     p->bytes += (bytes + 63) / 64 * 64;
     return o;
   };
-  // Short sequences: one launch, as long as the items do not crowd the card.
-  const int64_t items = Hkv * (call.cu_q == nullptr && Hq / Hkv <= 16 ? B : rows / 16 + B);
+  // Short sequences: one launch, as long as the items do not crowd the card.  The plan goes by
+  // what the workspace's question holds, the sizes: as many tokens as sequences count as one
+  // each, with offsets too; only the grid has slots for any spread of them (see slot_seq).
+  const int64_t spread = Hkv * (rows / 16 + B);
+  const int64_t items = n_tokens == B && Hq / Hkv <= 16 ? Hkv * B : spread;
   const int64_t again = prefix_len * Hkv * HD * static_cast<int64_t>(sizeof(T)) * 2 * (B - 1);
   const int64_t most = 2 * items >= cus ? kWholeKeys : 5 * StreamShape<T, HD, 1, whole_waves(HD)>::UK / 2;
   if (rows <= 16 * B && cap <= most && (HD == 128 || 2 * items <= 3 * cus) && again <= kWholeAgain) {
-    if (items > 0x7fffffff) return CGPT_ESHAPE;
+    const int64_t grid = call.cu_q == nullptr ? items : spread;
+    if (grid > 0x7fffffff) return CGPT_ESHAPE;
     p->whole = true;
-    p->grid = static_cast<int>(items);
+    p->grid = static_cast<int>(grid);
     return CGPT_OK;
   }
   // Rows that the tile kernel takes: more than 16 a sequence, or a batch's against a prefix.

@@ -455,8 +455,8 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
  * the same for all sequences and come from the pages prefix_pages (device int32); the
  * rows' own entries for whole pages of it are not read.  workspace: 16-byte aligned
  * device memory of at least the bytes that cgpt_paged_attention_workspace gives for
- * the same sizes (0: none needed), not shared by calls that may overlap; it needs no
- * clearing.
+ * the same sizes, with cu_q or without (0: none needed), not shared by calls that may
+ * overlap; it needs no clearing.
  *
  * No counterpart in the reference, which keeps no cache and runs
  * cutile_causal_attention over the whole prefix for every token

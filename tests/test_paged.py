@@ -90,6 +90,37 @@ def test_workspace_size():
     assert lib.cgpt_paged_attention_workspace(None, ctypes.byref(n)) == EINVAL
 
 
+@pytest.mark.parametrize("dtype", [_lib.CGPT_F32, _lib.CGPT_BF16])
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("group", [1, 4, 17])
+def test_workspace_is_what_the_call_needs(dtype, hd, group):
+    """The workspace's question holds sizes alone: its answer is enough, and no more than
+    enough, for the call with offsets and, at one token a sequence, without.  (Every call is
+    refused before a launch: a workspace off its alignment is, once it is large enough.)"""
+    lib, n = _lib.load(), ctypes.c_int64(-1)
+    seen = set()
+    for Hkv in (1, 3, 12, 25):
+        for B in (1, 10, 16, 20, 32, 33, 64, 300):
+            for tokens in (1, B, B + 1, 2 * B, 4 * B, 9 * B, 16 * B, 17 * B, 70 * B):
+                for cols in (1, 64, 128, 144, 400):
+                    for prefix in (0, 16, 2048):
+                        if prefix > 16 * cols:
+                            continue
+                        size = dict(n_tokens=tokens, B=B, Hq=group * Hkv, Hkv=Hkv, head_dim=hd, page_size=16, max_pages=cols,
+                                    prefix_len=prefix, dtype=dtype)
+                        args = _lib.paged_args(*(size.get(f, 0) for f in _lib.PAGED_FIELDS))
+                        assert lib.cgpt_paged_attention_workspace(args, ctypes.byref(n)) == 0, size
+                        seen.add(n.value > 0)
+                        size.update(q_st=size["Hq"] * hd, q_sh=hd, out_st=size["Hq"] * hd, out_sh=hd)
+                        size.update({f"{c}_{s}": v for c in ("kc", "vc") for s, v in (("sp", Hkv * 16 * hd), ("sh", 16 * hd), ("ss", hd))})
+                        for cu in (P, 0) if tokens == B else (P,):
+                            assert call(FNS[1], **size, cu_q=cu, workspace=P + 8, workspace_bytes=n.value) == EINVAL, (size, cu)
+                            if n.value:
+                                short = dict(workspace=P + 8, workspace_bytes=n.value - 1)
+                                assert call(FNS[1], **size, cu_q=cu, **short) == ESCRATCH, (size, cu)
+    assert seen == {False, True}
+
+
 def test_wrappers_refuse_host_tensors():
     p = Problem(torch.float32, 16, 8, 2, 2, ctx=[3], new=[1])
     with pytest.raises(ValueError):

@@ -708,3 +708,23 @@ def test_many_small_weights_add_up(gpu, dtype, hd, new):
         tol = (share * (half + 4 * gap * 2.0 ** -24) + 2 * adds * 2.0 ** -24 * (want.abs() + share)
                + (n * 2.0 ** -32 if dtype == F16 else 0.0) + half * want.abs())
         within(got, want, tol.expand_as(want), f"first {first}, rest {rest}")
+
+
+@pytest.mark.parametrize("dtype,hd,Hq,Hkv,B,new,cols", [
+    (BF16, 64, 12, 12, 32, 2, 64), (F16, 64, 12, 12, 32, 1, 64), (F32, 64, 12, 12, 32, 4, 64), (BF16, 64, 16, 16, 24, 3, 64),
+    (BF16, 64, 24, 24, 16, 8, 64), (F32, 32, 12, 12, 10, 2, 144), (BF16, 16, 48, 12, 16, 5, 144), (BF16, 64, 24, 12, 31, 1, 128)])
+@pytest.mark.parametrize("prefix", [0, 16])
+def test_guessed_tokens_near_a_full_card(gpu, dtype, hd, Hq, Hkv, B, new, cols, prefix):
+    """Offsets (one token each among them) where heads and sequences come to about one and a
+    half items a CU, with the tables that one launch serves at most."""
+    ctx = [prefix + (b * 29) % 150 for b in range(B)]
+    tokens = [1 + (b % new if b else new - 1) for b in range(B)]
+    p = Problem(dtype, hd, 16, Hq, Hkv, ctx, tokens, prefix=prefix, seed=B + new)
+    p.table = torch.cat([p.table, torch.full((B, cols - p.table.shape[1]), -7, dtype=torch.int32)], 1)
+    want, bound = attention(p)
+    d = p.on(gpu)
+    if prefix:
+        got = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, prefix, cu_q=d.cu)
+    else:
+        got = cg.paged_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, cu_q=d.cu)
+    within(got, want, bound)
