@@ -75,20 +75,27 @@ int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const
 // Offsets within 16 consecutive slots of a page fit 32 bits.
 inline bool short_rows(const PagedAttnArgs& a) { return a.kc.ss <= (1 << 25) && a.vc.ss <= (1 << 25); }
 
+// The sizes that a plan goes by, small enough for its products to stay within 64 bits.
+inline int check_sizes(const cgpt_paged_args& a) {
+  if (a.n_tokens < 0 || a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.page_size <= 0 || a.max_pages < 0 || a.Hq % a.Hkv != 0)
+    return CGPT_EINVAL;
+  if (a.dtype != CGPT_F32 && a.dtype != CGPT_BF16 && a.dtype != CGPT_F16) return CGPT_EDTYPE;
+  if (a.head_dim != 16 && a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 128) return CGPT_ESHAPE;
+  if (a.n_tokens > 0x3fffffff || a.B > 0x3fffffff || a.Hq > 0x7fff || a.page_size > 0x3fffffff ||
+      a.max_pages > 0x3fffffff || a.n_tokens * a.Hq > 0x7fffffff || a.page_size * a.max_pages > 0x3fffffff)
+    return CGPT_ESHAPE;
+  return CGPT_OK;
+}
+
 // The checks that the entry points share: the sizes, then (with tokens to work on) the
 // pointers.  CGPT_OK with *empty when there is nothing to launch.
 inline int check_paged(const cgpt_paged_args* p, bool* empty) {
   if (p == nullptr) return CGPT_EINVAL;
   const cgpt_paged_args& a = *p;
-  if (a.n_tokens < 0 || a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.page_size <= 0 || a.n_pages <= 0 || a.max_pages < 0)
-    return CGPT_EINVAL;
-  if (a.Hq % a.Hkv != 0 || a.bt_stride < 0) return CGPT_EINVAL;
-  if (a.dtype != CGPT_F32 && a.dtype != CGPT_BF16 && a.dtype != CGPT_F16) return CGPT_EDTYPE;
-  if (a.head_dim != 16 && a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 128) return CGPT_ESHAPE;
-  if (a.n_tokens > 0x3fffffff || a.B > 0x3fffffff || a.Hq > 0x7fff || a.page_size > 0x3fffffff ||
-      a.n_pages > 0x7fffffff || a.max_pages > 0x3fffffff || a.n_tokens * a.Hq > 0x7fffffff ||
-      a.page_size * a.max_pages > 0x3fffffff)
-    return CGPT_ESHAPE;
+  if (a.n_pages <= 0 || a.bt_stride < 0) return CGPT_EINVAL;
+  const int rc = check_sizes(a);
+  if (rc != CGPT_OK) return rc;
+  if (a.n_pages > 0x7fffffff) return CGPT_ESHAPE;
   // Rows are read and written as 16-byte vectors; no two of a pool may overlap.
   const int64_t epv = a.dtype == CGPT_F32 ? 4 : 8;
   const int64_t pools[2][3] = {{a.kc_sp, a.kc_sh, a.kc_ss}, {a.vc_sp, a.vc_sh, a.vc_ss}};

@@ -966,10 +966,9 @@ extern "C" int cgpt_paged_attention_workspace(const cgpt_paged_args* args, int64
   if (args == nullptr || workspace_bytes == nullptr) return CGPT_EINVAL;
   *workspace_bytes = 0;
   const cgpt_paged_args& p = *args;
-  if (p.n_tokens < 0 || p.B < 0 || p.Hq <= 0 || p.Hkv <= 0 || p.Hq % p.Hkv != 0 || p.page_size <= 0 ||
-      p.max_pages < 0 || p.prefix_len < 0 || p.prefix_len > p.page_size * p.max_pages)
-    return CGPT_EINVAL;
-  if (p.dtype != CGPT_F32 && p.dtype != CGPT_BF16 && p.dtype != CGPT_F16) return CGPT_EDTYPE;
+  const int rc = check_sizes(p);
+  if (rc != CGPT_OK) return rc;
+  if (p.prefix_len < 0 || p.prefix_len > p.page_size * p.max_pages) return CGPT_EINVAL;
   if (p.n_tokens == 0 || p.B == 0) return CGPT_OK;
   return with_type(p, [&](auto t, auto hd) {
     PagedPlan plan;

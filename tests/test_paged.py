@@ -3,6 +3,9 @@ of the wrappers, the rotation table and the tests' own oracle."""
 
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -158,3 +161,27 @@ def test_oracle_against_dense_softmax():
         want = torch.einsum("htj,jhd->thd", s.softmax(-1), v.repeat_interleave(2, 1))
         assert (out[int(p.cu[b]):int(p.cu[b + 1])] - want).abs().max() < 1e-12
         assert (bound[int(p.cu[b]):int(p.cu[b + 1])] < 1e-3).all()
+
+
+HUGE = [dict(n_tokens=1 << 38, B=1 << 38, Hq=1 << 32, Hkv=1 << 32, prefix_len=16, max_pages=4096),
+        dict(n_tokens=1 << 62), dict(B=1 << 40),
+        dict(Hq=1 << 20, Hkv=1 << 20), dict(page_size=1 << 40, max_pages=1 << 40), dict(max_pages=1 << 40),
+        dict(n_tokens=1 << 29, Hq=16, Hkv=16), dict(page_size=1 << 20, max_pages=1 << 11), dict(head_dim=1 << 40)]
+
+
+def test_workspace_refuses_the_sizes_that_the_call_does():
+    """Sizes whose products leave 64 bits among them.  In a process of its own: a division by
+    one of those, wrapped to zero, ends the process."""
+    code = ("import ctypes, sys; sys.path[:0] = ['.', 'tests']\n"
+            "from test_paged import HUGE, _lib\n"
+            "lib, n = _lib.load(), ctypes.c_int64(-1)\n"
+            "size = dict(n_tokens=4, B=4, Hq=4, Hkv=2, head_dim=64, page_size=16, max_pages=64, dtype=_lib.CGPT_BF16)\n"
+            "for change in HUGE:\n"
+            "    args = _lib.paged_args(*({**size, **change}.get(f, 0) for f in _lib.PAGED_FIELDS))\n"
+            "    status = lib.cgpt_paged_attention_workspace(args, ctypes.byref(n))\n"
+            "    assert (status, n.value) == (-3, 0), (change, status, n.value)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert res.returncode == 0, (res.returncode, res.stderr[-500:])
+    for change in HUGE:
+        assert call(FNS[1], **{**dict(bt_stride=64, max_pages=64, prefix_len=0), **change}) == ESHAPE, change
