@@ -1,6 +1,11 @@
 // Addressing shared by the kernels of the paged key-value cache.
 #pragma once
 
+#include <algorithm>
+#include <array>
+#include <initializer_list>
+#include <utility>
+
 #include "common.h"
 
 namespace cgpt {
@@ -75,6 +80,22 @@ int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const
 // Offsets within 16 consecutive slots of a page fit 32 bits.
 inline bool short_rows(const PagedAttnArgs& a) { return a.kc.ss <= (1 << 25) && a.vc.ss <= (1 << 25); }
 
+// Whether the rows of n values that these extents and strides place are apart: each stride
+// reaches past all that the smaller ones place.
+inline bool rows_apart(std::initializer_list<std::pair<int64_t, int64_t>> dims, int64_t n) {
+  std::array<std::pair<int64_t, int64_t>, 3> by_stride;
+  auto end = by_stride.begin();
+  for (auto [extent, stride] : dims)
+    if (extent > 1) *end++ = {stride, extent};
+  std::sort(by_stride.begin(), end);
+  __int128 span = n;
+  for (auto d = by_stride.begin(); d != end; ++d) {
+    if (d->first < span) return false;
+    span += static_cast<__int128>(d->first) * (d->second - 1);
+  }
+  return true;
+}
+
 // The sizes that a plan goes by, small enough for its products to stay within 64 bits.
 inline int check_sizes(const cgpt_paged_args& a) {
   if (a.n_tokens < 0 || a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.page_size <= 0 || a.max_pages < 0 || a.Hq % a.Hkv != 0)
@@ -88,15 +109,16 @@ inline int check_sizes(const cgpt_paged_args& a) {
 }
 
 // The checks that the entry points share: the sizes, then (with tokens to work on) the
-// pointers.  CGPT_OK with *empty when there is nothing to launch.
-inline int check_paged(const cgpt_paged_args* p, bool* empty) {
+// pointers.  CGPT_OK with *empty when there is nothing to launch.  `writes`: the pools are
+// written too.
+inline int check_paged(const cgpt_paged_args* p, bool writes, bool* empty) {
   if (p == nullptr) return CGPT_EINVAL;
   const cgpt_paged_args& a = *p;
   if (a.n_pages <= 0 || a.bt_stride < 0) return CGPT_EINVAL;
   const int rc = check_sizes(a);
   if (rc != CGPT_OK) return rc;
   if (a.n_pages > 0x7fffffff) return CGPT_ESHAPE;
-  // Rows are read and written as 16-byte vectors; no two of a pool may overlap.
+  // Rows are read and written as 16-byte vectors; no two that are written may overlap.
   const int64_t epv = a.dtype == CGPT_F32 ? 4 : 8;
   const int64_t pools[2][3] = {{a.kc_sp, a.kc_sh, a.kc_ss}, {a.vc_sp, a.vc_sh, a.vc_ss}};
   const void* bases[2] = {a.k_cache, a.v_cache};
@@ -105,6 +127,7 @@ inline int check_paged(const cgpt_paged_args* p, bool* empty) {
     if (bases[i] == nullptr || (reinterpret_cast<uintptr_t>(bases[i]) & 15)) return CGPT_EINVAL;
     if (s[0] % epv != 0 || s[1] % epv != 0 || s[2] % epv != 0) return CGPT_EINVAL;
     if ((a.n_pages > 1 && s[0] < hd) || (a.Hkv > 1 && s[1] < hd) || (a.page_size > 1 && s[2] < hd)) return CGPT_EINVAL;
+    if (writes && !rows_apart({{a.n_pages, s[0]}, {a.Hkv, s[1]}, {a.page_size, s[2]}}, hd)) return CGPT_EINVAL;
   }
   *empty = a.n_tokens == 0 || a.B == 0;
   if (*empty) return CGPT_OK;
@@ -114,8 +137,7 @@ inline int check_paged(const cgpt_paged_args* p, bool* empty) {
     if (st < 0 || st % epv != 0) return CGPT_EINVAL;
   for (const void* r : {a.q, a.k, a.v, static_cast<const void*>(a.out)})
     if (reinterpret_cast<uintptr_t>(r) & 15) return CGPT_EINVAL;
-  if (a.out != nullptr && ((a.Hq > 1 && a.out_sh < a.head_dim) || (a.n_tokens > 1 && a.out_st < a.head_dim)))
-    return CGPT_EINVAL;
+  if (a.out != nullptr && !rows_apart({{a.n_tokens, a.out_st}, {a.Hq, a.out_sh}}, a.head_dim)) return CGPT_EINVAL;
   return CGPT_OK;
 }
 

@@ -180,7 +180,7 @@ static int launch_append(const AppendArgs& a, hipStream_t s) {
 extern "C" int cgpt_paged_kv_append(const cgpt_paged_args* args, void* stream) {
   using namespace cgpt;
   bool empty;
-  const int rc = check_paged(args, &empty);
+  const int rc = check_paged(args, true, &empty);
   if (rc != CGPT_OK) return rc;
   const cgpt_paged_args& p = *args;
   if (p.k_cache == p.v_cache || (p.q == nullptr) != (p.out == nullptr)) return CGPT_EINVAL;

@@ -943,7 +943,7 @@ static int with_type(const cgpt_paged_args& p, F&& f) {
 extern "C" int cgpt_paged_attention(const cgpt_paged_args* args, void* stream) {
   using namespace cgpt;
   bool empty;
-  const int rc = check_paged(args, &empty);
+  const int rc = check_paged(args, false, &empty);
   if (rc != CGPT_OK) return rc;
   const cgpt_paged_args& p = *args;
   const float scale = static_cast<float>(p.scale), scale_log2 = scale * 1.4426950408889634f;

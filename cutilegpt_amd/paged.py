@@ -83,7 +83,12 @@ def _check_out(name: str, out: torch.Tensor, like: torch.Tensor, vec: int) -> No
                          f"on {like.device}")
     s0, s1, s2 = out.stride()
     n, h, hd = out.shape
-    if s2 != 1 or s0 % vec or s1 % vec or out.data_ptr() % 16 or (h > 1 and s1 < hd) or (n > 1 and s0 < hd):
+    # Apart when the larger stride reaches past what the smaller one places.
+    near = hd
+    for stride, extent in sorted(((s0, n), (s1, h))):
+        if extent > 1:
+            near = near + stride * (extent - 1) if stride >= near else math.inf
+    if s2 != 1 or s0 % vec or s1 % vec or out.data_ptr() % 16 or near == math.inf:
         raise ValueError(f"{name}: the output's rows must be separate, contiguous and 16-byte aligned")
 
 

@@ -424,7 +424,8 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
  * The paged key-value cache.  Pools hold pages of page_size rows: element (page,
  * head, slot, d) of k_cache at base + page*kc_sp + head*kc_sh + slot*kc_ss + d,
  * of v_cache with the vc_ strides; rows separate and 16-byte aligned, strides
- * multiples of 16 bytes.  Row b of block_table (max_pages int32, rows bt_stride
+ * multiples of 16 bytes.  Where rows are written (pools by the append, out) each stride
+ * reaches past all that the smaller ones place, else CGPT_EINVAL.  Row b of block_table (max_pages int32, rows bt_stride
  * apart) names sequence b's pages: its key t is in slot t % page_size of page
  * block_table[b][t / page_size].  seq_lens[b] (device int32) counts its keys, those
  * of the step's tokens, its last ones, included.  The tokens are packed rows: token b

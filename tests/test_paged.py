@@ -185,3 +185,33 @@ def test_workspace_refuses_the_sizes_that_the_call_does():
     assert res.returncode == 0, (res.returncode, res.stderr[-500:])
     for change in HUGE:
         assert call(FNS[1], **{**dict(bt_stride=64, max_pages=64, prefix_len=0), **change}) == ESHAPE, change
+
+
+OVERLAPS = [dict(n_tokens=3, out_st=64, out_sh=64), dict(n_tokens=3, out_st=192, out_sh=64), dict(n_tokens=3, out_st=64, out_sh=128),
+            dict(kc_sp=1024, kc_sh=1024), dict(kc_sp=2040), dict(vc_sh=1016), dict(vc_sp=64, vc_sh=504, vc_ss=1024),
+            dict(vc_sp=2048, vc_sh=64, vc_ss=64), dict(kc_sp=1 << 62, kc_sh=1 << 62)]
+APART = [dict(kc_sp=64, kc_sh=512, kc_ss=1024), dict(vc_sp=1024, vc_sh=64 * 128, vc_ss=64), dict(vc_sp=2048, vc_sh=64, vc_ss=128),
+         dict(kc_sp=4096, kc_sh=2048, kc_ss=128), dict(n_pages=1, kc_sp=0), dict(Hq=1, Hkv=1, kc_sh=0, kc_sp=1024),
+         dict(page_size=1, max_pages=64, kc_ss=0, prefix_len=0), dict(kc_sp=1 << 60)]
+
+
+@pytest.mark.parametrize("fn", FNS)
+def test_rows_that_overlap_are_refused(fn):
+    """Pools that are written and outputs two of whose rows share memory: two blocks would
+    write there."""
+    for change in OVERLAPS:
+        if "out_st" in change or fn == FNS[0]:
+            assert call(fn, **{**dict(workspace=P + 8), **change}) == EINVAL, change
+    for change in APART:
+        assert call(fn, **change) == 0, change
+
+
+def test_output_rows_that_overlap_are_refused():
+    from cutilegpt_amd.paged import _check_out
+    like = torch.empty(3, 4, 64)
+    for strides in ((64, 64, 1), (192, 64, 1), (64, 128, 1), (0, 64, 1)):
+        with pytest.raises(ValueError):
+            _check_out("test", torch.empty(2000).as_strided((3, 4, 64), strides), like, 4)
+    for strides in ((256, 64, 1), (64, 192, 1), (320, 80, 1)):
+        _check_out("test", torch.empty(2000).as_strided((3, 4, 64), strides), like, 4)
+    _check_out("test", torch.empty(64).as_strided((1, 1, 64), (0, 0, 1)), like[:1, :1], 4)
