@@ -663,6 +663,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PagedW
     if (b >= a.seq.B) return;
     const SeqUnits su = seq_units<R, UK>(a, b);
     if (t < su.first || t >= su.first + su.count) return;  // in front of the first sequence
+    // A length past a table that names no key past the prefix: no block has units of it.
+    if (su.kt == 0 && su.len > a.seq.cap && a.err != nullptr) *a.err = 1;
     const int U = ws.starts[a.seq.B], start = ws.starts[b];
     const Deal deal(grid, U);
     auto run = [&](int k, int from, int units, int r) {

@@ -728,3 +728,28 @@ def test_guessed_tokens_near_a_full_card(gpu, dtype, hd, Hq, Hkv, B, new, cols, 
     else:
         got = cg.paged_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, cu_q=d.cu)
     within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B", [3, 300])
+@pytest.mark.parametrize("keys,prefix", [(0, 0), (160, 0), (160, 160), (1024, 1024)])
+def test_lengths_past_the_table_set_the_flag(gpu, dtype, B, keys, prefix):
+    """Whatever the table holds: nothing at all, or no key past the prefix."""
+    ctx = [max(0, keys - 1)] * B
+    p = Problem(dtype, 64, 16, 2, 2, ctx, [1] * B, prefix=prefix, seed=B, spare_cols=0)
+    if keys == 0:
+        p.table, want, bound = p.table[:, :0], torch.zeros(B, 2, 64, dtype=torch.float64), torch.zeros(1)
+    else:
+        want, bound = attention(p)
+    d = p.on(gpu)
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    for past in (0, 5, 2 ** 30):
+        d.lens = torch.full_like(d.lens, keys)
+        d.lens[B - 1] += past
+        flag.zero_()
+        if prefix:
+            got = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, prefix, err_flag=flag)
+        else:
+            got = cg.paged_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, err_flag=flag)
+        within(got, want, bound, past)
+        assert int(flag) == (1 if past else 0), past
