@@ -36,7 +36,8 @@ template <typename T, int CPR> __device__ __forceinline__ int vswz(int key) {
 //   * (prefix only) rows are the packed tokens of all sequences, token-major, G
 //     heads each; keys are [0, prefix_len);
 //   * rows are one sequence's; keys are [prefix_len, length).
-// An item's keys are cut into units of UK.  The units of all items, in order (prefix:
+// An item's keys are cut into units of UK << unit_shift keys (a shift of 0, unless the units of
+// the longest sequences that the table allows would pass 32 bits).  The units of all items, in order (prefix:
 // head, row tile, unit; then sequence, head, row tile, unit), are dealt to the blocks in
 // equal contiguous runs, so a batch of any lengths keeps every CU busy to the end: the
 // lengths live on the device, and the host launches one grid for all of them.  A run
@@ -50,8 +51,14 @@ struct SeqUnits {
   int rt, kt;        // row tiles, key units
 };
 
+// ceil(n / (UK << shift)).
+template <int UK> __device__ __forceinline__ int key_units(int n, int shift) {
+  static_assert((UK & (UK - 1)) == 0, "divided by a shift");
+  return (n + (UK << shift) - 1) >> (__builtin_ctz(UK) + shift);
+}
+
 template <int R, int UK>
-__device__ __forceinline__ SeqUnits seq_units(const PagedAttnArgs& a, int b) {
+__device__ __forceinline__ SeqUnits seq_units(const PagedAttnArgs& a, int b, int shift) {
   SeqUnits u;
   seq_tokens(a.seq, b, &u.first, &u.count);
   u.len = max(a.seq.lens[b], 0);
@@ -59,7 +66,7 @@ __device__ __forceinline__ SeqUnits seq_units(const PagedAttnArgs& a, int b) {
   u.kb = a.prefix_len;
   u.base0 = u.kb & ~15;
   u.rt = (u.count * static_cast<int>(a.group.d) + R - 1) / R;
-  u.kt = u.n > u.kb ? (u.n - u.base0 + UK - 1) / UK : 0;
+  u.kt = u.n > u.kb ? key_units<UK>(u.n - u.base0, shift) : 0;
   return u;
 }
 
@@ -89,6 +96,7 @@ struct PagedWs {
   float* whole_o;    // {prefix, own} x n_tokens x Hq x HD
   float* tile_ml;    // the tile kernel's splits x n_tokens x Hq x {m, l}
   float* tile_o;     // splits x n_tokens x Hq x HD
+  int unit_shift;    // units of UK << unit_shift keys
 };
 
 template <typename T, int HD, int QTW, int NW>
@@ -166,7 +174,7 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     c0 = c;
     n_units = 0;
     if (c + lane < end) {
-      mine = seq_units<R, UK>(a, c + lane);
+      mine = seq_units<R, UK>(a, c + lane, ws.unit_shift);
       n_units = mine.rt * mine.kt * a.Hkv;
     }
     incl = scan(n_units);
@@ -236,14 +244,14 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
       const int first_b = lane * per, end_b = min(first_b + per, a.seq.B);
 #pragma unroll 4
       for (int b = first_b; b < end_b; ++b) {
-        const SeqUnits su = seq_units<R, UK>(a, b);
+        const SeqUnits su = seq_units<R, UK>(a, b, ws.unit_shift);
         group_units += su.rt * su.kt * a.Hkv;
       }
       group_incl = scan(group_units);
       if (writes) {
         int at = prefix_units + group_incl - group_units;
         for (int b = first_b; b < end_b; ++b) {
-          const SeqUnits su = seq_units<R, UK>(a, b);
+          const SeqUnits su = seq_units<R, UK>(a, b, ws.unit_shift);
           ws.starts[b] = at;
           at += su.rt * su.kt * a.Hkv;
         }
@@ -257,7 +265,7 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     u_end = deal.start(blockIdx.x + 1);
     if (u < prefix_units) {
       prefix = true;
-      kt_item = (a.prefix_len + UK - 1) / UK;
+      kt_item = key_units<UK>(a.prefix_len, ws.unit_shift);
       rows = a.seq.n_tokens * G;
       rts = (rows + R - 1) / R;
       n_all = a.prefix_len;
@@ -323,8 +331,9 @@ paged_stream_kernel(PagedAttnArgs a, PagedWs ws, int prefix_units) {
     // ---- its keys
     const T* const kh = static_cast<const T*>(a.kc.base) + hk * a.kc.sh;
     const T* const vh = static_cast<const T*>(a.vc.base) + hk * a.vc.sh;
-    const int sub0 = base0 + t0 * UK + wave * KT;  // first subtile; the next is UK further
-    const int cnt = sub0 < n ? min(t1 - t0, (n - sub0 + UK - 1) / UK) : 0;
+    const int shift = WHOLE ? 0 : ws.unit_shift;
+    const int sub0 = base0 + ((t0 * UK) << shift) + wave * KT;  // first subtile; the next is UK further
+    const int cnt = sub0 < n ? min((t1 - t0) << shift, (n - sub0 + UK - 1) / UK) : 0;
     int odd_from = 0x7fffffff;  // first masked key tile of the wave with a value that is not finite
     u32x4_t kf[NT][NKS], vf[NT][NKS];
     // Pages of subtile i: one a 16-key tile, or one a lane's key.
@@ -661,7 +670,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PagedW
   } else {
     const int b = wave_seq_of(a.seq, t, lane);
     if (b >= a.seq.B) return;
-    const SeqUnits su = seq_units<R, UK>(a, b);
+    const SeqUnits su = seq_units<R, UK>(a, b, ws.unit_shift);
     if (t < su.first || t >= su.first + su.count) return;  // in front of the first sequence
     // A length past a table that names no key past the prefix: no block has units of it.
     if (su.kt == 0 && su.len > a.seq.cap && a.err != nullptr) *a.err = 1;
@@ -675,7 +684,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PagedW
       wr[k] = r;
     };
     if (prefix_units > 0) {
-      const int rows = a.seq.n_tokens * G, rts = (rows + R - 1) / R, kt = (a.prefix_len + UK - 1) / UK;
+      const int rows = a.seq.n_tokens * G, rts = (rows + R - 1) / R, kt = key_units<UK>(a.prefix_len, ws.unit_shift);
       const int r = t * G + h - hk * G;
       run(0, (hk * rts + r / R) * kt, kt, r % R);
     }
@@ -748,7 +757,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, PagedW
 struct PagedPlan {
   bool whole = false;               // stream kernel, a block an item
   int tile_qt = 1, flat_split = 0, split = 0, n_tile = 0;  // tile kernel, and its partials a row
-  int stream_qt = 0, grid = 0, prefix_units = 0;  // stream kernel (stream_qt 0: none)
+  int stream_qt = 0, grid = 0, prefix_units = 0, unit_shift = 0;  // stream kernel (stream_qt 0: none)
   int64_t o_starts = 0, o_eml = 0, o_eo = 0, o_wml = 0, o_wo = 0, o_tml = 0, o_to = 0, bytes = 0;
 };
 
@@ -842,9 +851,17 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     p->stream_qt = wide ? (HD == 128 ? 2 : 4) : 1;
     const int64_t R = 16 * p->stream_qt;
     const int64_t UK = wide ? StreamShape<T, HD, 1, 4>::UK : StreamShape<T, HD, 1, stream_waves(HD)>::UK;
-    const int64_t pu = prefix_len > 0 && !flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + UK - 1) / UK) : 0;
-    const int64_t own = Hkv * (rows / R + B) * ((cap - (prefix_len & ~int64_t{15}) + UK - 1) / UK);
-    if (pu + own > 0x7fffffff) return CGPT_ESHAPE;
+    // Units as large as keep their number, had every sequence the length that the table
+    // allows, within 32 bits.
+    if (Hkv * (rows / R + B) > 0x7fffffff) return CGPT_ESHAPE;
+    int64_t pu = 0, own = 0;
+    for (;; ++p->unit_shift) {
+      const int64_t unit = UK << p->unit_shift;
+      if (unit > int64_t{1} << 30) return CGPT_ESHAPE;
+      pu = prefix_len > 0 && !flat ? Hkv * ((rows + R - 1) / R) * ((prefix_len + unit - 1) / unit) : 0;
+      own = Hkv * (rows / R + B) * ((cap - (prefix_len & ~int64_t{15}) + unit - 1) / unit);
+      if (pu + own <= 0x7fffffff) break;
+    }
     // Eight waves a CU; four of the widest, which need more registers than two a SIMD
     // leave (fp32, 8 x 512 tokens: 712 us with spills, 321 without).
     const int64_t per_cu = HD == 128 ? (wide ? 1 : 2) : wide ? 2 : 8;
@@ -895,7 +912,7 @@ static int run_plan(const PagedAttnArgs& a, const cgpt_paged_args& call, hipStre
   if (reinterpret_cast<uintptr_t>(w) & 15) return CGPT_EINVAL;
   auto f32 = [&](int64_t o) { return reinterpret_cast<float*>(w + o); };
   const PagedWs ws{reinterpret_cast<int*>(w + p.o_starts), f32(p.o_eml), f32(p.o_eo), f32(p.o_wml), f32(p.o_wo),
-                   f32(p.o_tml), f32(p.o_to)};
+                   f32(p.o_tml), f32(p.o_to), p.unit_shift};
   if (p.flat_split + p.split > 0) {
     TileJob job{};
     if (p.n_tile > 0) {

@@ -215,3 +215,21 @@ def test_output_rows_that_overlap_are_refused():
     for strides in ((256, 64, 1), (64, 192, 1), (320, 80, 1)):
         _check_out("test", torch.empty(2000).as_strided((3, 4, 64), strides), like, 4)
     _check_out("test", torch.empty(64).as_strided((1, 1, 64), (0, 0, 1)), like[:1, :1], 4)
+
+
+def test_wide_tables_of_many_sequences_are_taken():
+    """Lengths that a table allows and no batch has: the plan's counts go by them."""
+    lib, n = _lib.load(), ctypes.c_int64(-1)
+    for dtype in (_lib.CGPT_F32, _lib.CGPT_BF16):
+        for size in (dict(B=4096, n_tokens=4096, Hq=32, Hkv=32, page_size=256, max_pages=4096),
+                     dict(B=4096, n_tokens=9000, Hq=32, Hkv=32, page_size=256, max_pages=4096),
+                     dict(B=4096, n_tokens=4096, Hq=64, Hkv=8, page_size=16, max_pages=(1 << 26) - 1, prefix_len=4096),
+                     dict(B=300, n_tokens=300, Hq=8, Hkv=8, page_size=1 << 15, max_pages=(1 << 15) - 1)):
+            for hd in (16, 32, 64, 128):
+                size.update(head_dim=hd, dtype=dtype)
+                args = _lib.paged_args(*(size.get(f, 0) for f in _lib.PAGED_FIELDS))
+                assert lib.cgpt_paged_attention_workspace(args, ctypes.byref(n)) == 0 and n.value > 0, size
+                a = dict(prefix_len=0, bt_stride=64, kc_sp=1 << 40, kc_sh=1 << 30, kc_ss=hd, vc_sp=1 << 40, vc_sh=1 << 30, vc_ss=hd,
+                         q_st=64 * hd, q_sh=hd, out_st=64 * hd, out_sh=hd, workspace=P + 8, workspace_bytes=n.value)
+                assert call(FNS[1], **{**a, **size}) == EINVAL, size
+                assert call(FNS[1], **{**a, **size, "workspace_bytes": n.value - 1}) == ESCRATCH, size

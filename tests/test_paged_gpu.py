@@ -753,3 +753,27 @@ def test_lengths_past_the_table_set_the_flag(gpu, dtype, B, keys, prefix):
             got = cg.paged_attention(d.q, d.k_cache, d.v_cache, d.table, d.lens, err_flag=flag)
         within(got, want, bound, past)
         assert int(flag) == (1 if past else 0), past
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("prefix", [0, 160])
+def test_tables_far_wider_than_the_lengths(gpu, dtype, hd, prefix):
+    """270 sequences, 8 heads and columns for 2^28 keys: more units of keys than 32 bits
+    count, had the sequences such lengths."""
+    B, cols = 270, 2 ** 24
+    p = Problem(dtype, hd, 16, 8, 8, ctx=[prefix + (b * 61) % 2900 for b in range(B)], new=[1] * B, prefix=prefix, seed=hd)
+    want, bound = attention(p)
+    d = p.on(gpu)
+    # Rows that run on into the next ones' entries, which no length reaches.
+    stride = p.table.shape[1]
+    flat = torch.full((B * stride + cols,), -7, dtype=torch.int32, device=gpu)
+    flat[:B * stride] = d.table.flatten()
+    table = flat.as_strided((B, cols), (stride, 1))
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    if prefix:
+        got = cg.shared_prefix_attention(d.q, d.k_cache, d.v_cache, table, d.lens, prefix, err_flag=flag)
+    else:
+        got = cg.paged_attention(d.q, d.k_cache, d.v_cache, table, d.lens, err_flag=flag)
+    within(got, want, bound)
+    assert int(flag) == 0
