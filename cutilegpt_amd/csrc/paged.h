@@ -77,6 +77,9 @@ struct TileJob {
 // qt: 16-row sub-tiles of each of a block's four waves, 1 or 2.
 int launch_paged_tile(int64_t dtype, int head_dim, const PagedAttnArgs& a, const TileJob& job, int qt, hipStream_t s);
 
+// Blocks of 256 threads that one launch holds, fewer than 2^32 threads.
+constexpr int64_t kMaxBlocks = 0xffffff;
+
 // Offsets within 16 consecutive slots of a page fit 32 bits.
 inline bool short_rows(const PagedAttnArgs& a) { return a.kc.ss <= (1 << 25) && a.vc.ss <= (1 << 25); }
 

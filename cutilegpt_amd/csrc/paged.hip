@@ -168,6 +168,7 @@ static int launch_append(const AppendArgs& a, hipStream_t s) {
   int tokens_log2 = 0;
   while (tokens_log2 < 8 - unit_log2 && (a.seq.n_tokens >> (tokens_log2 + 1)) >= 8 * num_cus()) ++tokens_log2;
   const unsigned blocks = static_cast<unsigned>((a.seq.n_tokens + (1 << tokens_log2) - 1) >> tokens_log2);
+  if (blocks > kMaxBlocks) return CGPT_ESHAPE;
   if (a.interleaved || (a.rot_dim / 2) % EPV == 0)
     hipLaunchKernelGGL((append_kernel<T, true>), dim3(blocks), dim3(kAppendThreads), 0, s, a, unit_log2, tokens_log2);
   else

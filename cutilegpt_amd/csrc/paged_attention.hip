@@ -799,11 +799,10 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
   const int64_t items = n_tokens == B && Hq / Hkv <= 16 ? Hkv * B : spread;
   const int64_t again = prefix_len * Hkv * HD * static_cast<int64_t>(sizeof(T)) * 2 * (B - 1);
   const int64_t most = 2 * items >= cus ? kWholeKeys : 5 * StreamShape<T, HD, 1, whole_waves(HD)>::UK / 2;
-  if (rows <= 16 * B && cap <= most && (HD == 128 || 2 * items <= 3 * cus) && again <= kWholeAgain) {
-    const int64_t grid = call.cu_q == nullptr ? items : spread;
-    if (grid > 0x7fffffff) return CGPT_ESHAPE;
+  if (rows <= 16 * B && cap <= most && (HD == 128 || 2 * items <= 3 * cus) && again <= kWholeAgain &&
+      spread * whole_waves(HD) <= 4 * kMaxBlocks) {
     p->whole = true;
-    p->grid = static_cast<int>(grid);
+    p->grid = static_cast<int>(call.cu_q == nullptr ? items : spread);
     return CGPT_OK;
   }
   // Rows that the tile kernel takes: more than 16 a sequence, or a batch's against a prefix.
@@ -839,7 +838,8 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     const int64_t n_own = Hkv * (rows / BQ + B);
     if (flat) p->flat_split = parts(blocks(BQ), HD <= 64 ? 4 : 2, prefix_len);
     if (own) p->split = parts(n_own, 6, cap - (flat ? prefix_len : 0));
-    if (blocks(BQ) * p->flat_split + n_own * p->split > 0x7fffffff) return CGPT_ESHAPE;
+    // (head_blocks rounds the heads' blocks up by fewer than 8 a kind.)
+    if ((flat ? blocks(BQ) : 0) * p->flat_split + n_own * p->split > kMaxBlocks - 16) return CGPT_ESHAPE;
     p->n_tile = flat || p->split > 1 ? p->flat_split + p->split : 0;
     p->o_tml = take(p->n_tile * n_tokens * Hq * 8);
     p->o_to = take(p->n_tile * n_tokens * Hq * HD * 4);
@@ -873,6 +873,8 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     p->o_wml = take(prefix_len > 0 ? 2 * n_tokens * Hq * 8 : 0);
     p->o_wo = take(prefix_len > 0 ? 2 * n_tokens * Hq * HD * 4 : 0);
   }
+  // The join: four rows a block.
+  if ((p->split == 0 || p->n_tile > 0) && n_tokens * Hq > 4 * kMaxBlocks) return CGPT_ESHAPE;
   return CGPT_OK;
 }
 

@@ -449,7 +449,7 @@ static int launch_tile(const PagedAttnArgs& a, TileJob job, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.seq.n_tokens) * (a.Hq / a.Hkv);
   const int64_t flat = job.flat_split > 0 ? (rows + BQ - 1) / BQ : 0;
   const int64_t own = job.split == 0 ? 0 : a.seq.cu == nullptr && a.Hq / a.Hkv <= BQ ? a.seq.B : rows / BQ + a.seq.B;
-  if ((flat * job.flat_split + own * job.split) * (a.Hkv + 8) > 0x7fffffff) return CGPT_ESHAPE;
+  if ((flat * job.flat_split + own * job.split) * a.Hkv > kMaxBlocks - 16) return CGPT_ESHAPE;
   job.flat_tiles = static_cast<int>(flat);
   job.tiles = static_cast<int>(own);
   job.flat_blocks = head_blocks(a.Hkv, job.flat_tiles * job.flat_split);

@@ -434,7 +434,8 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
  * Element (token, head, d) of q, k, v and out at base + token*st + head*sh + d,
  * 16-byte aligned.  Hq is a multiple of Hkv; head_dim is 16, 32, 64 or 128; dtype
  * fp32, bf16 or fp16; offsets into the pools may pass 32 bits; page_size * max_pages
- * < 2^30.
+ * < 2^30.  CGPT_ESHAPE, before any launch, also where one would hold 2^32 threads:
+ * some 2^26 (token, head) rows.
  *
  * Device values that are out of range fault nothing and set *err_flag (a device int,
  * may be NULL) to 1: a page id outside [0, n_pages) is not written, and read as

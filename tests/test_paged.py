@@ -233,3 +233,24 @@ def test_wide_tables_of_many_sequences_are_taken():
                          q_st=64 * hd, q_sh=hd, out_st=64 * hd, out_sh=hd, workspace=P + 8, workspace_bytes=n.value)
                 assert call(FNS[1], **{**a, **size}) == EINVAL, size
                 assert call(FNS[1], **{**a, **size, "workspace_bytes": n.value - 1}) == ESCRATCH, size
+
+
+def test_launches_past_32_bits_are_refused():
+    """A launch holds less than 2^32 threads: more is refused before the first one."""
+    lib, n = _lib.load(), ctypes.c_int64(-1)
+    for dtype in (_lib.CGPT_F32, _lib.CGPT_BF16):
+        for size, hds in ((dict(B=1 << 22, n_tokens=1 << 22, Hq=32, Hkv=32, page_size=16, max_pages=4), (16, 64, 128)),
+                          (dict(B=1 << 22, n_tokens=1 << 22, Hq=32, Hkv=32, page_size=16, max_pages=400), (16, 64, 128)),
+                          (dict(B=1 << 17, n_tokens=1 << 26, Hq=31, Hkv=31, page_size=16, max_pages=400), (16, 64, 128)),
+                          (dict(B=1 << 17, n_tokens=1 << 23, Hq=31, Hkv=31, page_size=16, max_pages=400, prefix_len=6400), (16, 64, 128))):
+            for hd in hds:
+                size.update(head_dim=hd, dtype=dtype)
+                args = _lib.paged_args(*(size.get(f, 0) for f in _lib.PAGED_FIELDS))
+                assert lib.cgpt_paged_attention_workspace(args, ctypes.byref(n)) == ESHAPE, size
+                a = dict(prefix_len=0, bt_stride=400, kc_sp=1 << 40, kc_sh=1 << 30, kc_ss=hd, vc_sp=1 << 40, vc_sh=1 << 30, vc_ss=hd,
+                         q_st=64 * hd, q_sh=hd, out_st=64 * hd, out_sh=hd, workspace=P + 8, workspace_bytes=1 << 60)
+                assert call(FNS[1], **{**a, **size}) == ESHAPE, size
+    # 16 tokens a block at most in fp32 of head_dim 128.
+    a = dict(n_tokens=1 << 29, B=1 << 29, Hq=2, Hkv=2, head_dim=128, dtype=_lib.CGPT_F32, kc_sp=4096, kc_sh=2048, kc_ss=128, vc_sp=4096,
+             vc_sh=2048, vc_ss=128, out_st=256, out_sh=128)
+    assert call(FNS[0], **a) == ESHAPE
