@@ -62,12 +62,12 @@ struct PagedAttnArgs {
   int* err;
 };
 
-// What the tile kernel (paged_tile.hip; 16-bit types of head_dim 64 and 128) is to do:
-// all packed rows against the shared prefix in flat_split parts of its keys (0: not at
-// all), and every sequence's rows against its keys from `from` on, those below
-// prefix_len read from the prefix's pages, in `split` parts (0: not at all).  With ml each
-// part leaves (m, l, O) of its (token, head) rows there, the prefix's parts first; else the
-// rows' results are written.  The other fields are launch_paged_tile's.
+// What the tile kernel (paged_tile.hip; every type and head_dim) is to do: all packed rows
+// against the shared prefix in flat_split parts of its keys (0: not at all), and every
+// sequence's rows against its keys from `from` on, those below prefix_len read from the
+// prefix's pages, in `split` parts (0: not at all).  With ml each part leaves (m, l, O) of its
+// (token, head) rows there, the prefix's parts first; else the rows' results are written.  The
+// other fields are launch_paged_tile's.
 struct TileJob {
   float* ml;
   float* o;

@@ -3,9 +3,10 @@
 // append_kernel copies the step's keys and values into their pages and turns keys
 // and queries by their positions on the way: (x, y) -> (x c - y s, y c + x s) in 32 bits.
 // The bound is the bytes (k, v and q of a token read once and written once): 18 thousand
-// tokens, 12 heads of head_dim 64 with queries, bf16, 46 us, 4.1 TB/s where a large copy
-// reaches 4.9; or, for a decode step, the launch and three dependent loads (length, page
-// id, row): 32 tokens x 25 heads 3.9 us.
+// tokens, 12 heads of head_dim 64 with queries, bf16, 44 us, 4.3 TB/s where a large copy
+// reaches 4.9 (33 us when its 190 MB lie in the 256 MB cache from the call before); or,
+// for a decode step, the launch and three dependent loads (length, page id, row): 32 tokens
+// x 25 heads 3.7 us.
 #include "internal.h"
 #include "paged.h"
 

@@ -13,8 +13,9 @@
 // Three kernels: the stream kernel here for few rows (a decode step reads every key once:
 // the bound is HBM), the tile kernel (paged_tile.hip) for many, the join of their
 // partials.  make_plan below chooses.  Measured: 64 sequences of 1 to 8192 keys, 25 heads
-// of head_dim 64, bf16 294 us, 5.7 TB/s; four of 90 to 130 thousand, 8 heads of 128, fp16
-// 308 us, 5.8 TB/s (a large copy reaches 4.9 on the same card); one of 500 keys 8 us.
+// of head_dim 64, bf16 295 us, 5.7 TB/s, fp32 577 us, 5.8 TB/s; four of 90 to 130 thousand, 8
+// heads of 128, fp16 308 us, 5.8 TB/s (a kernel that only reads reaches 6.3 on the same card
+// with this cache policy, 7.2 with nontemporal loads); one of 500 keys 8 us.
 #include <algorithm>
 
 #include "internal.h"
@@ -821,9 +822,12 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     // rows win up to 2048 rows, 61 us against 65; fp32 tiles that sequences leave half empty
     // too: 24 of up to 64 tokens behind 2048 keys, 12 heads 190 us, 174 in tiles of 64), else
     // 64.  The keys are split, 256 a part at least (fp32 from head_dim 64 on 128: 64 tokens
-    // behind 1000 keys, 12 heads of 128 34 -> 23 us), while a CU has fewer than six blocks of own rows (16 prompts of up to 128 tokens, 12 heads of
-    // head_dim 64: 55 us whole, 43 in 3 parts; of up to 512: 67 whole, 86 in 2) or the
-    // resident number of prefix rows, whose partials are many.
+    // behind 1000 keys, 12 heads of 128 34 -> 23 us), while a CU has fewer than six blocks of
+    // own rows (16 prompts of up to 128 tokens, 12 heads of head_dim 64: 55 us whole, 43 in 3
+    // parts; of up to 512: 67 whole, 86 in 2) or the resident number of prefix rows, whose
+    // partials are many.  Keys are those that the table's width allows: a wide table of short
+    // sequences has parts without a key (24 of up to 64 tokens behind 2048 keys, 12 heads: 30
+    // us, 32 with a table eight times as wide as needed).
     p->tile_qt = blocks(128) >= 4 * cus || (flat && HD == 128 && rows > 128 && (!dear || !tall || rows >= 128 * B)) ? 2 : 1;
     const int64_t BQ = 64 * p->tile_qt;
     auto parts = [&](int64_t n, int64_t room, int64_t of) {
@@ -832,8 +836,9 @@ static int make_plan(const cgpt_paged_args& call, PagedPlan* p) {
     // A sequence's own keys behind a prefix go by the same launch, even for a single row
     // (64 sequences, 25 heads, 4096 keys shared: 64 keys of their own 42 -> 36 us, 512 69 ->
     // 60, 2048 159 -> 153), unless its tiles have 128 rows (128 sequences, 8 heads of
-    // head_dim 128, 2048 keys: 226 us, 211 by the stream kernel) or one sequence may have
-    // so many that its few blocks end last.
+    // head_dim 128, 2048 keys: 226 us, 211 by the stream kernel) or one sequence may, by the
+    // table's width, have so many that its few blocks end last (the launch more where it has
+    // not: 64 sequences behind 4096 keys 40 us, 50 with a table twice as wide as needed).
     const bool own = tall || (flat && !dear && p->tile_qt == 1 && cap - prefix_len <= kOwnKeys);
     const int64_t n_own = Hkv * (rows / BQ + B);
     if (flat) p->flat_split = parts(blocks(BQ), HD <= 64 ? 4 : 2, prefix_len);

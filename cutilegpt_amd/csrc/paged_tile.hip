@@ -12,16 +12,19 @@
 // kernel: a lane owns one query row, P goes from the accumulators straight into the second
 // product, V is transposed by the LDS read (fp32: read word by word).
 //
-// Bound: the exponentials.  A P costs an FMA, an exponential (a quarter of the rate), an
-// add and half a conversion, 26 cycles a 64 of them, against 16 on the matrix cores at
-// head_dim 64; 16 chunks of up to 2048 tokens behind up to 4096 keys, 16 heads of
-// head_dim 64, take 300 us: 630 TFLOP/s of what the mask leaves, VALU busy 55 % and
-// matrix cores 26 % of the time.  128 rows a block (two sub-tiles a wave) use a loaded
-// key for twice the rows of 64; blocks of eight waves with 128 or 256 rows were slower
-// (350 and 412 us), and 128 registers, for four waves a SIMD, spill (524 us).  At head_dim
-// 32 the same chunks take 236 us, 561 by the stream kernel, at 16 215 and 548.  fp32 is bound by its products:
-// 1896 us at head_dim 64, 99 TFLOP/s where a large product reaches 153 (2227 by the stream
-// kernel), 3940 at 128 (6570).
+// What bounds it: no unit alone.  16 chunks of up to 2048 tokens behind up to 4096 keys, 16
+// heads of head_dim 64, take 303 us: 619 TFLOP/s of what the mask leaves.  By the counters the
+// VALU is busy 53 % of that, the matrix cores 25 %, a CU has no wave for 19 % (the last
+// tiles), and a SIMD holds two waves where three fit.  64 weights take 6.4 vector
+// instructions, 3.5 of them their own arithmetic (an FMA, an exponential, an add, half a
+// conversion); masks, addresses, moves and the maximum's check are the rest.  128 rows a block
+// (two sub-tiles a wave) use a loaded key for twice the rows of 64; blocks of eight waves with
+// 128 or 256 rows were slower (350 and 412 us), and 128 registers, for four waves a SIMD,
+// spill (524 us).  At head_dim 32 the same chunks take 236 us, 561 by the stream kernel, at 16
+// 215 and 548.  fp32 is bound by its products: 1911 us at head_dim 64 (2227 by the stream
+// kernel), 98 TFLOP/s where a large product reaches 153; the matrix cores are busy 65 %, a CU
+// has no wave for 13 %, and two waves a SIMD, all that the registers leave, do not fill the
+// rest; 3940 us at 128 (6570).
 #include "internal.h"
 #include "paged.h"
 

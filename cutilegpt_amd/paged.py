@@ -21,7 +21,8 @@ with the same pages (samples of one prompt, users behind one document): those ar
 read once for all sequences.
 
 Head counts may differ (n_head a multiple of n_kv_head); head_dim is 16, 32, 64 or
-128; float32, bfloat16 or float16, one dtype a call; any page size.  The reference
+128; float32, bfloat16 or float16, one dtype a call; any page size (a table row names
+fewer than 2^30 keys, a call holds some 2^26 rows of one head).  The reference
 keeps no cache (``cutile_gpt/models/gpt.py:185-229`` runs the whole prefix again for
 every token; its attention is ``cutile_gpt/kernels/attention.py:24-175``).
 
@@ -173,7 +174,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     values of every key, and of the queries ``q`` (n_tokens, n_head, head_dim), by
     their positions on the way: pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) with
     ``interleaved``, in float32, rounded once.  Returns the turned queries (in
-    ``q_out`` when given, which may be ``q``), None without ``q``."""
+    ``q_out`` when given, which may be ``q`` but shares no memory with ``k`` or
+    ``v``), None without ``q``."""
     name = "paged_kv_append"
     dev, code, vec, n_pages, hkv, page, hd, cs, B, cols, ts = _check_cache(
         name, k, k_cache, v_cache, block_table, seq_lens, cu_q, err_flag)

@@ -445,7 +445,7 @@ int cgpt_kv_store(const void* k, const void* v, void* k_cache, void* v_cache, in
  *
  * cgpt_paged_kv_append: k and v (Hkv heads) into their pages; with rot_dim > 0 the
  * first rot_dim values of every key, and of q (Hq heads, written to out, which may
- * be q; both may be NULL), are turned by the token's position p: pairs (i,
+ * be q but shares no memory with k or v; both may be NULL), are turned by the token's position p: pairs (i,
  * i + rot_dim/2), or (2i, 2i+1) when interleaved, (x, y) -> (x c - y s, y c + x s) with
  * c = rotary[p][i], s = rotary[p][rot_dim/2 + i] (fp32, n_pos rows rot_stride apart), in
  * fp32 and rounded once.  Two tokens of a call must not share a slot.
