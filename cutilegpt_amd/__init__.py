@@ -29,6 +29,10 @@ from .paged import (  # noqa: F401
     rotary_table,
     shared_prefix_attention,
 )
+from .paged8 import (  # noqa: F401
+    paged_kv_append_8bit,
+    paged_kv_read_8bit,
+)
 from .model import CutileGPT  # noqa: F401
 from .hf_loader import HFWeightLoader  # noqa: F401
 from . import api  # noqa: F401  (Tile API: cutilegpt_amd.api.tile, configure_tiles, ...)
@@ -53,4 +57,6 @@ __all__ = [
     "paged_attention",
     "shared_prefix_attention",
     "rotary_table",
+    "paged_kv_append_8bit",
+    "paged_kv_read_8bit",
 ]

@@ -22,6 +22,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libcgpt.so"
 CGPT_F32 = 0
 CGPT_BF16 = 1
 CGPT_F16 = 2
+CGPT_E4M3 = 0
+CGPT_INT8 = 1
 EPI_NONE = 0
 EPI_BIAS = 1
 EPI_BIAS_GELU = 2
@@ -76,6 +78,8 @@ SIGNATURES = {
     "cgpt_paged_kv_append": (_I, [ctypes.c_char_p, _P]),
     "cgpt_paged_attention": (_I, [ctypes.c_char_p, _P]),
     "cgpt_paged_attention_workspace": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_paged_kv_append_8bit": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_paged_kv_read_8bit": (_I, [ctypes.c_char_p, _P]),
     "cgpt_partials_bias_act": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I64, _I, _I,
                                     _P]),
 }
@@ -88,6 +92,10 @@ PAGED_FIELDS = ("q", "k", "v", "out", "k_cache", "v_cache", "block_table", "seq_
                 "v_st", "v_sh", "out_st", "out_sh", "kc_sp", "kc_sh", "kc_ss", "vc_sp", "vc_sh", "vc_ss", "rot_dim",
                 "n_pos", "rot_stride", "interleaved", "dtype", "scale")
 paged_args = struct.Struct(f"{len(PAGED_FIELDS) - 1}qd").pack
+# cgpt_paged8_args: the same and what the 8-bit cache has besides.
+PAGED8_FIELDS = PAGED_FIELDS + ("k_scale", "v_scale", "v_out", "ks_sp", "ks_sh", "ks_sb", "vs_sp", "vs_sh", "vs_sb",
+                                "vo_st", "vo_sh", "block", "code")
+paged8_args = struct.Struct(f"{len(PAGED_FIELDS) - 1}qd{len(PAGED8_FIELDS) - len(PAGED_FIELDS)}q").pack
 
 ABI_VERSION = 1
 

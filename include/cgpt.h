@@ -48,6 +48,10 @@ extern "C" {
 #define CGPT_BF16 1
 #define CGPT_F16 2
 
+/* codes of the 8-bit paged cache */
+#define CGPT_E4M3 0            /* OCP e4m3 (finite, largest 448) */
+#define CGPT_INT8 1            /* -127 .. 127 */
+
 /* GEMM epilogues */
 #define CGPT_EPI_NONE 0        /* C = A W^T                                  */
 #define CGPT_EPI_BIAS 1        /* C = A W^T + bias                           */
@@ -483,6 +487,42 @@ typedef struct cgpt_paged_args {
 int cgpt_paged_kv_append(const cgpt_paged_args* args, void* stream);
 int cgpt_paged_attention(const cgpt_paged_args* args, void* stream);
 int cgpt_paged_attention_workspace(const cgpt_paged_args* args, int64_t* workspace_bytes);
+
+/*
+ * The paged cache in 8 bits.  Pools, tables, lengths and tokens as above, with pools of
+ * one byte an element (strides in bytes, multiples of 16): a cached value is code * 2^e,
+ * the code an e4m3 number or an int8 (`code`), e one exponent for each `block` consecutive
+ * slots of a page and key head, held as the byte e + 127 (that of page, head, slot at
+ * k_scale + page*ks_sp + head*ks_sh + slot/block*ks_sb; v_scale alike; page_size is a multiple
+ * of block).  Bytes outside 27 .. 246 (e4m3) or 27 .. 248 (int8) are read as the nearest
+ * of these.  dtype is that of k, v, q and the outputs.  Out-of-range device values do what
+ * they do above.
+ *
+ * cgpt_paged_kv_append_8bit: as cgpt_paged_kv_append.  e is the smallest for which the
+ * step's values in the block fit (|x| <= 448 * 2^e or 127 * 2^e), within -100 .. 119 (e4m3)
+ * or 121 (int8).  Where the step goes on behind rows of the block, e is the larger of that
+ * and the one there, and if it grew the codes in front are rounded again, to nearest even.
+ * A code is the exact turned value over 2^e (computed in 64 bits), rounded once to nearest
+ * even; turned queries are rounded once to dtype.  Values that are not finite take no part
+ * in e: infinities become the largest code, a NaN stays one (int8: 0), and *err_flag is set.
+ * Two sequences of a call must not write to the same block.
+ *
+ * cgpt_paged_kv_read_8bit: rows cu_q[b] .. cu_q[b+1]-1 of out and v_out (Hkv heads, strides
+ * out_ and vo_) receive the last keys and values of sequence b, code * 2^e rounded to
+ * dtype; rows that are not in the cache (positions below 0, or past the table) zeros.
+ *
+ * No counterpart in the reference, which keeps no cache (cutile_gpt/models/gpt.py:185-229).
+ */
+typedef struct cgpt_paged8_args {
+  cgpt_paged_args p;
+  uint8_t *k_scale, *v_scale;
+  void* v_out;
+  int64_t ks_sp, ks_sh, ks_sb, vs_sp, vs_sh, vs_sb;
+  int64_t vo_st, vo_sh;
+  int64_t block, code;
+} cgpt_paged8_args;
+int cgpt_paged_kv_append_8bit(const cgpt_paged8_args* args, void* stream);
+int cgpt_paged_kv_read_8bit(const cgpt_paged8_args* args, void* stream);
 
 /*
  * Greedy token per row: ids[r] = argmax_c x[r * ld + c] (the first maximum;
