@@ -30,6 +30,7 @@ from .paged import (  # noqa: F401
     shared_prefix_attention,
 )
 from .paged8 import (  # noqa: F401
+    paged_attention_8bit,
     paged_kv_append_8bit,
     paged_kv_read_8bit,
 )
@@ -59,4 +60,5 @@ __all__ = [
     "rotary_table",
     "paged_kv_append_8bit",
     "paged_kv_read_8bit",
+    "paged_attention_8bit",
 ]

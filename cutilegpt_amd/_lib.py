@@ -80,6 +80,8 @@ SIGNATURES = {
     "cgpt_paged_attention_workspace": (_I, [ctypes.c_char_p, _P]),
     "cgpt_paged_kv_append_8bit": (_I, [ctypes.c_char_p, _P]),
     "cgpt_paged_kv_read_8bit": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_paged_attention_8bit": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_paged_attention_8bit_workspace": (_I, [ctypes.c_char_p, _P]),
     "cgpt_partials_bias_act": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I64, _I, _I,
                                     _P]),
 }

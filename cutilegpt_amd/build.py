@@ -44,6 +44,7 @@ FILE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

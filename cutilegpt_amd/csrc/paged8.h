@@ -72,6 +72,25 @@ inline Paged8 paged8(const cgpt_paged8_args& a) {
                 FastDiv(a.block)};
 }
 
+// f(T{}, code, head_dim) with the call's types as compile-time values.
+template <typename F> inline int with_types8(const cgpt_paged8_args& a, F&& f) {
+  auto by_dim = [&](auto t, auto code) {
+    switch (a.p.head_dim) {
+      case 16: return f(t, code, std::integral_constant<int, 16>{});
+      case 32: return f(t, code, std::integral_constant<int, 32>{});
+      case 64: return f(t, code, std::integral_constant<int, 64>{});
+      default: return f(t, code, std::integral_constant<int, 128>{});
+    }
+  };
+  auto by_code = [&](auto t) {
+    return a.code == CGPT_E4M3 ? by_dim(t, std::integral_constant<int, CGPT_E4M3>{})
+                               : by_dim(t, std::integral_constant<int, CGPT_INT8>{});
+  };
+  if (a.p.dtype == CGPT_BF16) return by_code(bf16_t{});
+  if (a.p.dtype == CGPT_F16) return by_code(f16_t{});
+  return by_code(float{});
+}
+
 #if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
 
 // 2^e of an exponent byte; bytes that no append writes count as the nearest that one does.
@@ -134,6 +153,10 @@ template <> struct Codec<CGPT_INT8> {
     return w;
   }
   __device__ static void decode4(uint32_t w, float* y) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    // Kept a word up to here: else the compiler carries its four bytes in as many registers.
+    asm("" : "+v"(w));
+#endif
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
   }

@@ -272,25 +272,6 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args a, int tokens_log2
   if (bad && a.err != nullptr) *a.err = 1;
 }
 
-// f(T{}, code, head_dim) with the call's types as compile-time values.
-template <typename F> static int with_types8(const cgpt_paged8_args& a, F&& f) {
-  auto by_dim = [&](auto t, auto code) {
-    switch (a.p.head_dim) {
-      case 16: return f(t, code, std::integral_constant<int, 16>{});
-      case 32: return f(t, code, std::integral_constant<int, 32>{});
-      case 64: return f(t, code, std::integral_constant<int, 64>{});
-      default: return f(t, code, std::integral_constant<int, 128>{});
-    }
-  };
-  auto by_code = [&](auto t) {
-    return a.code == CGPT_E4M3 ? by_dim(t, std::integral_constant<int, CGPT_E4M3>{})
-                               : by_dim(t, std::integral_constant<int, CGPT_INT8>{});
-  };
-  if (a.p.dtype == CGPT_BF16) return by_code(bf16_t{});
-  if (a.p.dtype == CGPT_F16) return by_code(f16_t{});
-  return by_code(float{});
-}
-
 }  // namespace cgpt
 
 extern "C" int cgpt_paged_kv_append_8bit(const cgpt_paged8_args* args, void* stream) {

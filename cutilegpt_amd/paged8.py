@@ -25,6 +25,8 @@ numbers; int8: all such steps together move a value by less than one step).
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -33,7 +35,7 @@ import torch
 from . import _lib
 from .paged import _CODE, _HEAD_DIMS, _check_out, _launch, _ptr, _rows
 
-__all__ = ["paged_kv_append_8bit", "paged_kv_read_8bit"]
+__all__ = ["paged_kv_append_8bit", "paged_kv_read_8bit", "paged_attention_8bit"]
 
 _CODES8 = {torch.float8_e4m3fn: _lib.CGPT_E4M3, torch.int8: _lib.CGPT_INT8}
 
@@ -213,3 +215,59 @@ def paged_kv_read_8bit(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: to
         0, 0, 0, 0, dt, 0.0,
         k_scale.data_ptr(), v_scale.data_ptr(), v_out.data_ptr(), *ss, vos, voh, block, code), dev, name)
     return k_out, v_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes8(n: int, B: int, hq: int, hkv: int, hd: int, page: int, cols: int, dt: int, code: int,
+                      device: int) -> int:
+    """The C ABI's answer for these sizes (it goes by the device's CU count too)."""
+    out = ctypes.c_int64()
+    size = dict(n_tokens=n, B=B, Hq=hq, Hkv=hkv, head_dim=hd, page_size=page, max_pages=cols, dtype=dt, code=code)
+    args = _lib.paged8_args(*(size.get(f, 0) for f in _lib.PAGED8_FIELDS))
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().cgpt_paged_attention_8bit_workspace(args, ctypes.byref(out)),
+                   "paged_attention_8bit_workspace")
+    return out.value
+
+
+def paged_attention_8bit(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         cu_q: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         out: Optional[torch.Tensor] = None, err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attention`` over a cache in 8 bits: causal softmax attention of the step's
+    queries (n_tokens, n_head, head_dim; float32, bfloat16 or float16) over their
+    sequences' pages; returns the same shape and type.
+
+    Cached values are taken exactly as code * 2^e.  Queries and probabilities enter the
+    products with the bits of their type at least, statistics and sums are float32."""
+    name = "paged_attention_8bit"
+    try:
+        dev = q.get_device()
+    except AttributeError:
+        dev = -1
+    code, n_pages, hkv, page, hd, cs, ss, block, B, cols, ts = _check_cache8(
+        name, dev, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_q, err_flag)
+    dt = _check_rows8(name, "q", q, B, hd, cu_q)
+    n, hq, _ = q.shape
+    if hq == 0 or hq % hkv:
+        raise ValueError(f"{name}: n_head {hq} is not a multiple of n_kv_head {hkv}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    elif not 0.0 < scale < math.inf:
+        raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
+    vec = 8 if dt else 4
+    if out is None:
+        out = q.new_empty((n, hq, hd))
+    else:
+        _check_out(name, out, q, vec)
+    qr, qs, qh = _rows(q, vec)
+    os_, oh, _ = out.stride()
+    size = _workspace_bytes8(n, B, hq, hkv, hd, page, cols, dt, code, dev)
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _launch(_lib.load().cgpt_paged_attention_8bit, _lib.paged8_args(
+        qr.data_ptr(), 0, 0, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), _ptr(cu_q), 0, 0, _ptr(ws), _ptr(err_flag), size,
+        n, B, hq, hkv, hd, n_pages, page, cols, ts, 0, qs, qh, 0, 0, 0, 0, os_, oh, *cs,
+        0, 0, 0, 0, dt, scale,
+        k_scale.data_ptr(), v_scale.data_ptr(), 0, *ss, 0, 0, block, code), dev, name)
+    return out

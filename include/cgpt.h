@@ -511,6 +511,11 @@ int cgpt_paged_attention_workspace(const cgpt_paged_args* args, int64_t* workspa
  * out_ and vo_) receive the last keys and values of sequence b, code * 2^e rounded to
  * dtype; rows that are not in the cache (positions below 0, or past the table) zeros.
  *
+ * cgpt_paged_attention_8bit: as cgpt_paged_attention without a prefix (prefix_len and
+ * prefix_pages are not read) on code * 2^e; queries and weights enter the products with the bits
+ * of dtype at least, statistics and sums are fp32.  workspace as there, of the bytes that
+ * cgpt_paged_attention_8bit_workspace gives for the same sizes and code.
+ *
  * No counterpart in the reference, which keeps no cache (cutile_gpt/models/gpt.py:185-229).
  */
 typedef struct cgpt_paged8_args {
@@ -523,6 +528,8 @@ typedef struct cgpt_paged8_args {
 } cgpt_paged8_args;
 int cgpt_paged_kv_append_8bit(const cgpt_paged8_args* args, void* stream);
 int cgpt_paged_kv_read_8bit(const cgpt_paged8_args* args, void* stream);
+int cgpt_paged_attention_8bit(const cgpt_paged8_args* args, void* stream);
+int cgpt_paged_attention_8bit_workspace(const cgpt_paged8_args* args, int64_t* workspace_bytes);
 
 /*
  * Greedy token per row: ids[r] = argmax_c x[r * ld + c] (the first maximum;

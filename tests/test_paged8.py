@@ -13,8 +13,8 @@ from paged8_ref import F8, HI, LO, TOP, Problem8, append, exponent, grid, neares
 
 P = 1 << 20  # a pointer that is never followed
 EINVAL, EDTYPE, ESHAPE, ESCRATCH = -1, -2, -3, -4
-APPEND, READ = "cgpt_paged_kv_append_8bit", "cgpt_paged_kv_read_8bit"
-FNS = [APPEND, READ]
+APPEND, READ, ATTEND = "cgpt_paged_kv_append_8bit", "cgpt_paged_kv_read_8bit", "cgpt_paged_attention_8bit"
+FNS = [APPEND, READ, ATTEND]
 
 
 def fields(**change):
@@ -77,10 +77,44 @@ def test_c_read_refuses():
         assert call(READ, n_tokens=3, **change) == EINVAL, change
 
 
+def workspace(**change):
+    out = ctypes.c_int64(-1)
+    return _lib.load().cgpt_paged_attention_8bit_workspace(fields(**change), ctypes.byref(out)), out.value
+
+
+def test_c_attention_refuses():
+    for change in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e-60),
+                   dict(scale=1e60), dict(scale=3e38)):
+        assert call(ATTEND, **change) == EINVAL, change
+    for change in (dict(q=0), dict(out=0), dict(out_st=64)):
+        assert call(ATTEND, n_tokens=3, **change) == EINVAL, change
+    # A workspace that is missing, too small or unaligned is refused before any launch.
+    long = dict(n_tokens=2, cu_q=0, max_pages=4096, bt_stride=4096)
+    status, size = workspace(**long)
+    assert status == 0 and size > 64
+    assert call(ATTEND, **long) == ESCRATCH
+    assert call(ATTEND, **long, workspace=P, workspace_bytes=size - 1) == ESCRATCH
+    assert call(ATTEND, **long, workspace=P + 8, workspace_bytes=1 << 40) == EINVAL
+    assert call(ATTEND, n_tokens=1 << 20, B=1 << 20, cu_q=0, Hq=1 << 11, Hkv=1) == ESHAPE
+
+
+def test_workspace_size():
+    assert workspace(n_tokens=0) == (0, 0) and workspace(n_tokens=4, B=0) == (0, 0)
+    # Short sequences need none, with offsets or without.
+    for cu in (0, P):
+        assert workspace(n_tokens=8, B=8, cu_q=cu, max_pages=8) == (0, 0)
+    assert _lib.load().cgpt_paged_attention_8bit_workspace(None, None) == EINVAL
+    for change, status in SIZES:
+        if set(change) & {"n_tokens", "B", "Hq", "Hkv", "page_size", "max_pages", "dtype", "head_dim", "code"}:
+            assert workspace(**{"n_tokens": 4, **change})[0] == status, change
+
+
 def test_wrappers_refuse_host_tensors():
     p = Problem8(torch.bfloat16, F8, 64, 16, 16, 2, 2, ctx=[3], new=[1])
     with pytest.raises(ValueError, match="one GPU"):
         cg.paged_kv_append_8bit(p.k, p.v, *p.cache)
+    with pytest.raises(ValueError, match="one GPU"):
+        cg.paged_attention_8bit(p.q, *p.cache)
     with pytest.raises(ValueError, match="one GPU"):
         cg.paged_kv_read_8bit(*p.cache, p.cu_rows, 4)
     with pytest.raises(ValueError, match="n_rows"):

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import cutilegpt_amd as cg
-from paged8_ref import F8, NAN, Problem8, append, values
+from paged8_ref import F8, NAN, Problem8, append, attention, values
 from paged_ref import within
 
 pytestmark = pytest.mark.gpu
@@ -262,3 +262,389 @@ def test_read_bad_device_values(gpu):
     d.table[2, 0] = p.n_pages + 5
     cg.paged_kv_read_8bit(*d.cache, d.cu_rows, 60, BF16, err_flag=flag)
     assert int(flag) == 1
+
+
+# ------------------------------------------------------------------------- attention
+# ``room``: columns of the table past what the lengths need.  A narrow table of short
+# sequences runs in one launch, a wide one in shared-out parts and their join.
+
+ROOM = [1, 400]
+
+
+def run_attention(p, gpu, **kw):
+    d = p.on(gpu)
+    cu = None if p.n == p.B and p.new == [1] * p.B else d.cu
+    return cg.paged_attention_8bit(d.q, *d.cache, cu_q=cu, **kw)
+
+
+def check_attention(p, gpu, scale=None, **kw):
+    want, bound = attention(p, scale)
+    got = run_attention(p, gpu, scale=scale, **kw)
+    assert got.shape == p.q.shape and got.dtype == p.dtype
+    live = int(p.cu[-1])
+    within(got[:live], want[:live], bound[:live], "attention")
+
+
+def problem(dtype, code, hd, page, block, Hq, Hkv, ctx, new, **kw):
+    """Keys that are all numbers."""
+    return Problem8(dtype, code, hd, page, block, Hq, Hkv, ctx, new, size=40, **kw)
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("hd,Hq,Hkv,page,block", [(16, 4, 2, 16, 16), (32, 3, 3, 8, 8), (64, 12, 12, 16, 16), (64, 8, 1, 24, 8),
+                                                  (64, 20, 1, 64, 32), (128, 8, 2, 32, 32), (128, 3, 1, 10, 5), (64, 2, 2, 1, 1)])
+def test_single_tokens(gpu, dtype, code, hd, Hq, Hkv, page, block, room):
+    p = problem(dtype, code, hd, page, block, Hq, Hkv, ctx=[0, 1, 14, 15, 16, 31, 63, 64, 127, 200, 333], new=[1] * 11,
+                seed=hd + page, spare_cols=room)
+    check_attention(p, gpu)
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("hd,Hq,Hkv,page,block,new", [
+    (64, 4, 2, 16, 16, [3, 1, 0, 8, 2]), (64, 4, 4, 16, 8, [70, 1, 129, 0, 33]), (128, 4, 1, 64, 64, [5, 200, 0, 64, 17]),
+    (32, 6, 3, 10, 5, [5, 40, 1, 16, 2]), (16, 2, 1, 16, 16, [90, 3, 65, 1, 0]), (128, 2, 2, 24, 24, [40, 8, 100, 1, 1]),
+    (32, 2, 2, 128, 64, [300, 64, 65, 63, 1]), (64, 8, 1, 7, 7, [20, 9, 0, 3, 1])])
+def test_ragged_tokens(gpu, dtype, code, hd, Hq, Hkv, page, block, new, room):
+    p = problem(dtype, code, hd, page, block, Hq, Hkv, ctx=[0, 17, 40, 100, 250], new=new, seed=sum(new), spare_cols=room,
+                pad_rows=3)
+    check_attention(p, gpu)
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype,new,hd", [(BF16, 1, 64), (F16, 4, 128), (F32, 2, 64), (BF16, 80, 64), (F16, 40, 32)])
+def test_one_long_sequence(gpu, dtype, code, new, hd):
+    p = problem(dtype, code, hd, 64, 64, Hq=4, Hkv=2, ctx=[9000], new=[new], seed=new)
+    check_attention(p, gpu)
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_rows_without_a_key(gpu, new, room):
+    """Sequences shorter than their step: the tokens in front of position 0 give zeros."""
+    p = problem(BF16, F8, 64, 16, 16, 4, 2, ctx=[0, 30, 0, 5], new=[new] * 4, seed=new, spare_cols=room)
+    for b, n in ((0, 0), (2, max(new - 2, 0))):
+        p.lens[b] = n
+        p.total[b] = n
+    check_attention(p, gpu)
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("hd,new,Hkv", [(64, 1, 2), (64, 6, 2), (128, 3, 1), (64, 70, 2), (16, 30, 1), (32, 150, 2), (128, 90, 1)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_masked_nan_codes_do_not_leak(gpu, dtype, new, Hkv, hd, room):
+    """Keys and values that are no numbers count for the rows that see them, and for no
+    other."""
+    p = problem(dtype, F8, hd, 16, 8, 2 * Hkv, Hkv, ctx=[20, 3, 150], new=[new] * 3, seed=new + hd, spare_cols=room)
+    at = {}
+    for b in range(3):
+        # The last key, and one in the middle of the step, of the first head.
+        for pos, which in ((p.total[b] - 1, "k"), (p.total[b] - 1 - new // 2, "v"), (p.total[b] - 1 - new // 3, "v")):
+            page, slot = int(p.table[b, pos // 16]), pos % 16
+            getattr(p, which + "_cache").view(torch.uint8)[page, 0, slot, 3] = 0x7f if which == "k" else 0xff
+            at.setdefault(b, []).append((pos, which))
+    G = 2
+    clean = problem(dtype, F8, hd, 16, 8, 2 * Hkv, Hkv, ctx=[20, 3, 150], new=[new] * 3, seed=new + hd, spare_cols=room)
+    want, bound = attention(clean)
+    got = run_attention(p, gpu).cpu()
+    for b in range(3):
+        for i in range(new):
+            t, pos = int(p.cu[b]) + i, p.total[b] - new + i
+            rows_nan = any(w == "k" and pos >= a for a, w in at[b])
+            d3_nan = rows_nan or any(pos >= a for a, w in at[b])
+            first, others = got[t, :G], got[t, G:]
+            assert bool(first[:, 3].isnan().all()) == d3_nan and bool(first[:, 3].isnan().any()) == d3_nan, (b, i)
+            rest = torch.cat([first[:, :3], first[:, 4:]], 1)
+            assert bool(rest.isnan().all()) == rows_nan and bool(rest.isnan().any()) == rows_nan, (b, i)
+            if not rows_nan:
+                w, e = want[t].clone(), bound[t]
+                if d3_nan:
+                    w[:G, 3] = NAN
+                within(got[t], w, e, f"{b} {i}")
+            within(others, want[t, G:], bound[t, G:])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("new", [1, 30])
+def test_a_query_that_is_not_a_number(gpu, dtype, new):
+    """It spoils its own row only."""
+    p = problem(dtype, F8, 64, 16, 16, 2, 1, ctx=[40, 10], new=[new, new], seed=3)
+    want, bound = attention(p)
+    p.q[new, 1, 5] = NAN
+    got = run_attention(p, gpu)
+    assert bool(got[new, 1].isnan().all())
+    want[new, 1] = NAN
+    within(got, want, bound)
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("B,new,room", [(130, 1, 1), (300, 1, 40), (70, 3, 1), (90, 20, 1)])
+def test_many_sequences(gpu, code, B, new, room):
+    g = torch.Generator().manual_seed(B)
+    ctx = torch.randint(0, 150, (B,), generator=g).tolist()
+    p = problem(BF16, code, 32, 16, 16, 2, 1, ctx=ctx, new=[new] * B, seed=B, spare_cols=room)
+    check_attention(p, gpu)
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("new,room", [(1, 1), (1, 400), (40, 1)])
+def test_exponents_far_apart(gpu, code, dtype, new, room):
+    """Blocks whose values differ by 2^40, and the ends of the exponents' range."""
+    p = problem(dtype, code, 64, 16, 16, 2, 2, ctx=[100, 60], new=[new, new], seed=4, spare_cols=room)
+    p.k_scale.fill_(118)
+    g = torch.Generator().manual_seed(9)
+    p.v_scale.copy_(torch.randint(60, 101, p.v_scale.shape, generator=g, dtype=torch.uint8))
+    if dtype != F16:
+        p.v_scale += 60
+    check_attention(p, gpu)
+    # All values of the smallest exponent there is: 2^-100, read from the bytes below too.
+    p.v_scale.fill_(0)
+    if dtype != F16:
+        want, bound = attention(p)
+        got = run_attention(p, gpu)
+        # (The bound's own floor is of that size: take it without.)
+        within(got, want, bound - 2.0 ** -100 + want.abs().amax() * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("new,room", [(1, 1), (3, 400), (60, 1)])
+def test_large_scores(gpu, dtype, new, room):
+    p = problem(dtype, I8, 64, 16, 16, 4, 2, ctx=[150, 33], new=[new, new], seed=11, spare_cols=room, spread=4)
+    check_attention(p, gpu, scale=2.0)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_out_may_be_q(gpu, new):
+    p = problem(BF16, F8, 64, 16, 16, 4, 2, ctx=[30, 7], new=[new, new], seed=2)
+    d = p.on(gpu)
+    got = cg.paged_attention_8bit(d.q, *d.cache, cu_q=d.cu, out=d.q)
+    assert got is d.q
+    want, bound = attention(p)
+    within(got, want, bound)
+
+
+def test_attention_views(gpu):
+    """q out of a fused projection, pools and exponents views of others, out with gaps."""
+    p = problem(BF16, I8, 64, 16, 4, 4, 2, ctx=[30, 7, 100], new=[1, 9, 40], seed=2)
+    d = p.on(gpu)
+    fused = torch.zeros(p.n, 8, 64, dtype=BF16, device=gpu)
+    fused[:, :4] = d.q
+    pool = torch.stack([d.k_cache, d.v_cache], 2)          # (pages, heads, 2, slots, hd)
+    scale = torch.stack([d.k_scale, d.v_scale], -1)        # (pages, heads, blocks, 2)
+    out = torch.full((p.n, 6, 64), 7.0, dtype=BF16, device=gpu)
+    cg.paged_attention_8bit(fused[:, :4], pool[:, :, 0], pool[:, :, 1], scale[..., 0], scale[..., 1], d.table, d.lens,
+                            cu_q=d.cu, out=out[:, 1:5])
+    want, bound = attention(p)
+    within(out[:, 1:5], want, bound)
+    assert bool((out[:, 0] == 7).all()) and bool((out[:, 5] == 7).all())
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_pool_past_32_bits(gpu, new):
+    """Pages and exponents further than 2^32 bytes from the pool's start."""
+    p = problem(BF16, F8, 64, 16, 16, 2, 2, ctx=[100], new=[new], seed=1)
+    d = p.on(gpu)
+    apart = 1 << 30
+    big = torch.empty(apart * p.n_pages, dtype=torch.uint8, device=gpu)
+    kc = big.as_strided((p.n_pages, 2, 16, 64), (apart, 1024, 64, 1))
+    ks = big[4096:].as_strided((p.n_pages, 2, 1), (apart, 1, 1))
+    kc.copy_(d.k_cache.view(torch.uint8))
+    ks.copy_(d.k_scale)
+    got = cg.paged_attention_8bit(d.q, kc.view(F8), d.v_cache, ks, d.v_scale, d.table, d.lens, cu_q=d.cu)
+    want, bound = attention(p)
+    within(got, want, bound)
+    cg.paged_kv_append_8bit(d.k, d.v, kc.view(F8), d.v_cache, ks, d.v_scale, d.table, d.lens, cu_q=d.cu)
+    after, _ = append(p)
+    same_bytes(kc, after[0], "k_cache")
+    same_bytes(ks, after[2], "k_scale")
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_bad_device_values(gpu, new):
+    """A page outside the pool is read as page 0, a length past the table is cut; each sets the
+    flag, and other sequences' rows stay right."""
+    p = problem(BF16, F8, 64, 16, 16, 2, 2, ctx=[40, 40, 40], new=[new] * 3, seed=6, spare_cols=0)
+    want, bound = attention(p)
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    d = p.on(gpu)
+    within(cg.paged_attention_8bit(d.q, *d.cache, cu_q=d.cu, err_flag=flag), want, bound)
+    assert int(flag) == 0
+    d.table[1, 0] = p.n_pages
+    got = cg.paged_attention_8bit(d.q, *d.cache, cu_q=d.cu, err_flag=flag)
+    assert int(flag) == 1
+    for b in (0, 2):
+        rows = slice(int(p.cu[b]), int(p.cu[b + 1]))
+        within(got[rows], want[rows], bound[rows])
+    flag.zero_()
+    d = p.on(gpu)
+    d.lens[2] = d.table.shape[1] * 16 + 9
+    got = cg.paged_attention_8bit(d.q, *d.cache, cu_q=d.cu, err_flag=flag)
+    assert int(flag) == 1
+    within(got[:2 * new], want[:2 * new], bound[:2 * new])
+
+
+def test_rows_in_front_of_the_first_sequence(gpu):
+    """Offsets that begin past 0: the rows in front are left as they were."""
+    p = problem(BF16, F8, 64, 16, 16, 2, 2, ctx=[30, 20], new=[3, 2], seed=6)
+    d = p.on(gpu)
+    q = torch.cat([d.q[:2], d.q])
+    out = torch.full_like(q, 5.0)
+    cg.paged_attention_8bit(q, *d.cache, cu_q=d.cu + 2, out=out)
+    want, bound = attention(p)
+    within(out[2:], want, bound)
+    assert bool((out[:2] == 5).all())
+
+
+def test_empty_calls(gpu):
+    p = problem(BF16, F8, 64, 16, 16, 2, 2, ctx=[30], new=[1], seed=6)
+    d = p.on(gpu)
+    none = d.q[:0]
+    cu = torch.zeros(1, dtype=torch.int32, device=gpu)
+    assert cg.paged_attention_8bit(none, *d.cache[:4], d.table[:0], d.lens[:0]).shape == (0, 2, 64)
+    assert cg.paged_attention_8bit(none, *d.cache[:4], d.table[:0], d.lens[:0], cu_q=cu).shape == (0, 2, 64)
+    cg.paged_kv_append_8bit(none, none, *d.cache[:4], d.table[:0], d.lens[:0])
+    k, v = cg.paged_kv_read_8bit(*d.cache[:4], d.table[:0], d.lens[:0], cu, 0)
+    assert k.shape == v.shape == (0, 2, 64)
+    # Tables without a page: nothing to see.
+    o = cg.paged_attention_8bit(d.q, *d.cache[:4], d.table[:, :0], torch.zeros_like(d.lens))
+    assert bool((o == 0).all())
+
+
+def test_same_bits_twice_and_on_side_streams(gpu):
+    """One answer, whatever the stream and what runs beside it."""
+    p = problem(BF16, F8, 64, 16, 16, 4, 2, ctx=[3000, 10, 700], new=[1, 20, 3], seed=8)
+    d = p.on(gpu)
+    first = cg.paged_attention_8bit(d.q, *d.cache, cu_q=d.cu)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(cg.paged_attention_8bit(d.q, *d.cache, cu_q=d.cu))
+    torch.cuda.synchronize()
+    for x in got:
+        assert torch.equal(x.view(torch.int16), first.view(torch.int16))
+
+
+def test_captured_steps(gpu):
+    """A captured step (append, attention) of single tokens replays with the lengths of the
+    moment, as the eager one does bit for bit."""
+    B, Hq, Hkv, hd, page = 3, 4, 2, 64, 16
+    base = problem(BF16, F8, hd, page, 16, Hq, Hkv, ctx=[5, 14, 40], new=[20] * 3, seed=12)
+    rotary = cg.rotary_table(100, hd)
+    g = torch.Generator().manual_seed(3)
+    steps = [torch.randn(B, Hq + 2 * Hkv, hd, generator=g).to(BF16).to(gpu) for _ in range(18)]
+
+    def fresh():
+        d = base.on(gpu)
+        d.lens = torch.tensor(base.ctx, dtype=torch.int32, device=gpu)
+        return d
+
+    def step(d, x):
+        q = cg.paged_kv_append_8bit(x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:], *d.cache, q=x[:, :Hq], rotary=rotary)
+        return cg.paged_attention_8bit(q, *d.cache)
+
+    e, want = fresh(), []
+    for x in steps:
+        e.lens += 1
+        want.append(step(e, x))
+    c = fresh()
+    x = steps[0].clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(problem(BF16, F8, hd, page, 16, Hq, Hkv, ctx=[5, 14, 40], new=[20] * 3, seed=12).on(gpu), x)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(c, x)
+    for i, y in enumerate(steps):
+        c.lens += 1
+        x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), want[i].view(torch.int16)), i
+    for a, b in zip(c.cache[:4], e.cache[:4]):
+        same_bytes(a, b.cpu(), "pools")
+
+
+def test_written_cache_against_16_bits(gpu):
+    """Prompts, then tokens, through the 8-bit cache against the 16-bit one: the answers differ by
+    what the codes round.  With one-hot scores (a huge scale) an answer is one cached value."""
+    hd, page = 64, 16
+    g = torch.Generator().manual_seed(21)
+    n, H = 50, 2
+    k, v, q = (torch.randn(n, H, hd, generator=g).to(BF16).to(gpu) for _ in range(3))
+    table = torch.randperm(8, generator=g).to(torch.int32).view(1, 8).to(gpu)
+    lens, cu = torch.tensor([n], dtype=torch.int32, device=gpu), torch.tensor([0, n], dtype=torch.int32, device=gpu)
+    for code in (F8, I8):
+        pools = [torch.zeros(8, H, page, hd, dtype=torch.uint8, device=gpu).view(code) for _ in range(2)]
+        scales = [torch.zeros(8, H, page // 8, dtype=torch.uint8, device=gpu) for _ in range(2)]
+        cg.paged_kv_append_8bit(k, v, *pools, *scales, table, lens, cu_q=cu)
+        kr, vr = cg.paged_kv_read_8bit(*pools, *scales, table, lens, cu, n)
+        # Values within half a step: of 2^-3 relative, or of the block's largest over 64 (a power of
+        # two at or above largest / 127).
+        for got, want in ((kr, k), (vr, v)):
+            want = want.double()
+            big = want.reshape(n, H, hd).abs().amax(-1)
+            blocks = torch.stack([big[i // 8 * 8:i // 8 * 8 + 8].amax(0) for i in range(n)])[..., None]
+            bound = want.abs() / 16 + blocks * 2.0 ** -18 if code == F8 else blocks / 127 + want * 0
+            assert bool(((got.double() - want).abs() <= bound).all())
+        o8 = cg.paged_attention_8bit(q, *pools, *scales, table, lens, cu_q=cu)
+        kc, vc = torch.zeros(8, H, page, hd, dtype=BF16, device=gpu), torch.zeros(8, H, page, hd, dtype=BF16, device=gpu)
+        cg.paged_kv_append(kr, vr, kc, vc, table, lens, cu_q=cu)
+        o16 = cg.paged_attention(q, kc, vc, table, lens, cu_q=cu)
+        # The same values in 16 bits: both round weights and results to bf16.
+        assert float((o8.double() - o16.double()).abs().max()) <= 4 * 2.0 ** -8 * float(vr.double().abs().max())
+
+
+def test_refusals(gpu):
+    p = problem(BF16, F8, 64, 16, 8, 4, 2, ctx=[30, 7], new=[1, 1], seed=2)
+    d = p.on(gpu)
+    kc, vc, ks, vs, table, lens = d.cache
+
+    def refused(match, q=d.q, kc=kc, vc=vc, ks=ks, vs=vs, table=table, lens=lens, **kw):
+        with pytest.raises(ValueError, match=match):
+            cg.paged_attention_8bit(q, kc, vc, ks, vs, table, lens, **kw)
+
+    refused("float8_e4m3fn or int8", kc=kc.view(I8))
+    refused("float8_e4m3fn or int8", kc=kc.to(BF16), vc=vc.to(BF16))
+    refused("unsupported dtype", q=d.q.double())
+    refused("uint8", ks=ks.to(torch.int32))
+    refused("divide a page", ks=ks[..., :1].expand(-1, -1, 3), vs=vs[..., :1].expand(-1, -1, 3))
+    refused("page_size / block", ks=ks[:-1], vs=vs[:-1])
+    refused("page_size / block", vs=vs[..., :1])
+    refused("share a shape", vc=vc[:-1])
+    refused("cache rows", kc=kc.transpose(2, 3).contiguous().transpose(2, 3))
+    refused("not a multiple", q=d.q[:, :3])
+    refused("need cu_q", q=torch.cat([d.q, d.q]))
+    refused("int32", table=table.long())
+    refused("one GPU", lens=lens.cpu())
+    refused("scale must", scale=0.0)
+    refused("scale must", scale=float("nan"))
+    refused("output", out=torch.empty(2, 4, 64, dtype=F16, device=gpu))
+    refused("output's rows", out=torch.empty(2, 1, 64, dtype=BF16, device=gpu).expand(2, 4, 64))
+    refused("err_flag", err_flag=torch.zeros(2, dtype=torch.int32, device=gpu))
+    refused("offsets", cu_q=torch.zeros(2, dtype=torch.int32, device=gpu))
+    with pytest.raises(ValueError, match="invalid argument"):
+        off = torch.zeros(kc.numel() + 16, dtype=torch.uint8, device=gpu)[4:4 + kc.numel()].view(kc.shape)
+        cg.paged_attention_8bit(d.q, off.view(F8), vc, ks, vs, table, lens)
+    with pytest.raises(ValueError, match="same memory"):
+        cg.paged_kv_append_8bit(d.k, d.v, kc, kc, ks, vs, table, lens)
+    with pytest.raises(ValueError, match="same memory"):
+        cg.paged_kv_append_8bit(d.k, d.v, kc, vc, ks, ks, table, lens)
+    with pytest.raises(ValueError, match="k and v"):
+        cg.paged_kv_append_8bit(d.k, d.v.to(F16), *d.cache)
+    with pytest.raises(ValueError, match="invalid argument"):
+        cg.paged_kv_append_8bit(d.k, d.v, kc, vc, ks[..., :1].expand(-1, -1, 2), vs, table, lens)
+    with pytest.raises(ValueError, match="n_rows"):
+        cg.paged_kv_read_8bit(*d.cache, d.cu, 2.0)
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        cg.paged_kv_read_8bit(*d.cache, d.cu, 2, torch.float64)
+    with pytest.raises(ValueError, match="k_out and v_out"):
+        cg.paged_kv_read_8bit(*d.cache, d.cu, 2, BF16, k_out=torch.empty(3, 2, 64, dtype=BF16, device=gpu))
