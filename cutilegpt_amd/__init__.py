@@ -34,6 +34,7 @@ from .paged8 import (  # noqa: F401
     paged_kv_append_8bit,
     paged_kv_read_8bit,
 )
+from .sampling import sample_tokens  # noqa: F401
 from .model import CutileGPT  # noqa: F401
 from .hf_loader import HFWeightLoader  # noqa: F401
 from . import api  # noqa: F401  (Tile API: cutilegpt_amd.api.tile, configure_tiles, ...)
@@ -61,4 +62,5 @@ __all__ = [
     "paged_kv_append_8bit",
     "paged_kv_read_8bit",
     "paged_attention_8bit",
+    "sample_tokens",
 ]

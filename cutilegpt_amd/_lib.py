@@ -35,6 +35,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/cgpt.h.
 SIGNATURES = {
@@ -82,6 +83,7 @@ SIGNATURES = {
     "cgpt_paged_kv_read_8bit": (_I, [ctypes.c_char_p, _P]),
     "cgpt_paged_attention_8bit": (_I, [ctypes.c_char_p, _P]),
     "cgpt_paged_attention_8bit_workspace": (_I, [ctypes.c_char_p, _P]),
+    "cgpt_sample": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _D, _I64, _D, _D, _P, _P]),
     "cgpt_partials_bias_act": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I64, _I, _I,
                                     _P]),
 }

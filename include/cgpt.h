@@ -541,6 +541,29 @@ int cgpt_argmax(const void* x, int64_t rows, int64_t cols, int64_t ld, int dtype
                 int64_t* ids, int64_t* hist, int64_t hist_ld, const int* step_dev,
                 void* stream);
 
+/*
+ * The next token of each row, drawn with a given random number: ids[r] from the cols
+ * logits at x + r * ld (fp32, bf16 or fp16; at most 2^20) and u[r] (fp32, of [0, 1)).
+ * temperature, top_k, top_p and min_p point to a value a row (device memory), or are NULL for
+ * the one of all rows in the `_all` argument.
+ *
+ * Weights are exp((x - max x) / temperature), held to 2^-44 of the largest, sums exact.  In
+ * the order of the logits, largest first and equal ones by index, the first top_k are kept
+ * (0: all), of these the shortest run with top_p of their weight or more, one at least (1: all),
+ * and of it weights of at least min_p of the largest (0: all).  The token is the first index
+ * at which the running sum of the kept weights, in the order of the vocabulary, exceeds u times
+ * their sum.  A temperature of 0 takes the largest logit, the first of equals.  NaN entries
+ * are skipped, -inf is never chosen; -1 where nothing is left.  Settings in device memory that
+ * make no sense count as the nearest that do (temperature below 0 as 0, top_k below 0 and a NaN
+ * top_p or min_p as none, min_p above 1 as 1, u as within [0, 1)).
+ *
+ * Replaces the sampling of generate, cutile_gpt/models/gpt.py:207-226.
+ */
+int cgpt_sample(const void* x, int64_t rows, int64_t cols, int64_t ld, int dtype, const float* u,
+                const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all,
+                int64_t* ids, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
