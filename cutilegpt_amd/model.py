@@ -269,7 +269,8 @@ class CutileGPT:
     @torch.inference_mode()
     def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature: float = 1.0,
                  top_k: Optional[int] = None, use_cache: bool = True,
-                 use_graph: bool = True) -> torch.Tensor:
+                 use_graph: bool = True, top_p: Optional[float] = None, min_p: Optional[float] = None,
+                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
         """Autoregressive continuation with the semantics of
         ``cutile_gpt/models/gpt.py:185-229``: temperature, top-k masking, then
         sampling; ``top_k=1`` is greedy decoding.
@@ -279,11 +280,26 @@ class CutileGPT:
         KV-cache step (``decode.DecodeSession``); greedy steps run entirely on
         the device and are replayed from one captured HIP graph when
         ``use_graph``.  Otherwise every token re-runs the full forward on the
-        last block_size tokens, as the reference does."""
+        last block_size tokens, as the reference does.
+
+        With ``top_p``, ``min_p`` or a ``generator`` (of the model's device) tokens are drawn
+        by ``sample_tokens``: the shortest run of tokens with ``top_p`` of the probability,
+        those of at least ``min_p`` of the likeliest's, exactly ``top_k`` of equal logits,
+        ``temperature`` 0 the likeliest; the random numbers are the generator's."""
         idx = self._prepare_idx(idx)
         B, T0 = idx.shape
         if max_new_tokens <= 0:
             return idx
+        if top_p is not None or min_p is not None or generator is not None:
+            from .sampling import sample_tokens
+
+            u = torch.rand(max_new_tokens, B, device=self.device, generator=generator)
+
+            def sample(logits, t):
+                return sample_tokens(logits, u[t], temperature, top_k, top_p, min_p).view(B, 1)
+        else:
+            def sample(logits, t):
+                return self._sample(logits, temperature, top_k)
         if use_cache and T0 + max_new_tokens <= self.config.block_size and B <= 64:
             from .decode import DecodeSession
 
@@ -296,7 +312,7 @@ class CutileGPT:
                 sess = DecodeSession(self, B, T0, max_new_tokens)
                 self._decode_session = sess
             sess.prefill(idx)
-            if top_k == 1:
+            if top_k == 1:  # no draw to make
                 new = sess.run_greedy(use_graph=use_graph)
                 return torch.cat([idx, new], dim=1)
             sess.step.zero_()
@@ -305,16 +321,16 @@ class CutileGPT:
             for t in range(max_new_tokens):
                 if t > 0:
                     sess.next_logits(use_graph=use_graph and max_new_tokens >= 4)
-                nxt = self._sample(sess.logits, temperature, top_k)
+                nxt = sample(sess.logits, t)
                 out.append(nxt)
                 sess.ids.copy_(nxt.view(-1))
                 if t > 0:
                     sess.step.add_(1)
             return torch.cat([idx] + out, dim=1)
-        for _ in range(max_new_tokens):
+        for t in range(max_new_tokens):
             cond = idx if idx.shape[1] <= self.config.block_size else idx[:, -self.config.block_size:]
             logits = self._forward(cond)
-            nxt = self._sample(logits[:, -1, :], temperature, top_k)
+            nxt = sample(logits[:, -1, :], t)
             idx = torch.cat([idx, nxt], dim=1)
         return idx
 
