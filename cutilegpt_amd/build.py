@@ -45,6 +45,7 @@ FILE_FLAGS = {
     "attention_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged8_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

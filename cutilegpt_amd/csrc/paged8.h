@@ -72,6 +72,12 @@ inline Paged8 paged8(const cgpt_paged8_args& a) {
                 FastDiv(a.block)};
 }
 
+// The tile kernel (paged8_tile.hip): every sequence's rows against its keys in job.split parts;
+// with job.ml each part leaves (m, l, O) of its rows there, else the results are written.  qt:
+// 16-row sub-tiles of each of a block's four waves, 1 or 2.
+int launch_paged8_tile(const cgpt_paged8_args& call, const PagedAttnArgs& a, const Paged8& quant, const TileJob& job, int qt,
+                       hipStream_t s);
+
 // f(T{}, code, head_dim) with the call's types as compile-time values.
 template <typename F> inline int with_types8(const cgpt_paged8_args& a, F&& f) {
   auto by_dim = [&](auto t, auto code) {
@@ -177,6 +183,30 @@ template <int CODE> __device__ __forceinline__ u32x2_t bf16x4_of(uint32_t w, flo
   return u32x2_t{0, 0};
 #endif
 }
+
+// The queries' values as sums of bf16 parts.
+template <typename T> constexpr int kParts = std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, f16_t>::value ? 2 : 3;
+
+// Eight values as NP bf16 fragments.
+template <int NP> __device__ __forceinline__ void split_parts(const float* x, u32x4_t (&f)[NP]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      f[p][i] = w;
+      if (p + 1 < NP) {
+        r[2 * i] -= __uint_as_float(w << 16);
+        r[2 * i + 1] -= __uint_as_float(w & 0xffff0000u);
+      }
+    }
+}
+
+// e4m3 has one code of either sign that is no number, all ones: the sign bits of such bytes.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 #endif
 

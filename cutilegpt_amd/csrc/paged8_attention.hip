@@ -19,30 +19,6 @@
 
 namespace cgpt {
 
-// The queries' values as sums of bf16 parts.
-template <typename T> constexpr int kParts = std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, f16_t>::value ? 2 : 3;
-
-// Eight values as NP bf16 fragments.
-template <int NP> __device__ __forceinline__ void split_parts(const float* x, u32x4_t (&f)[NP]) {
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = x[i];
-#pragma unroll
-  for (int p = 0; p < NP; ++p)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = pack_bf16x2(r[2 * i], r[2 * i + 1]);
-      f[p][i] = w;
-      if (p + 1 < NP) {
-        r[2 * i] -= __uint_as_float(w << 16);
-        r[2 * i + 1] -= __uint_as_float(w & 0xffff0000u);
-      }
-    }
-}
-
-// e4m3 has one code of either sign that is no number, all ones: the sign bits of such bytes.
-__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
 template <int HD, int NW>
 struct Shape8 {
   static constexpr int LB = HD >= 64 ? 16 : 8;                 // bytes of a lane's load
@@ -516,10 +492,12 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
 
 // ------------------------------------------------------------------------- host
 
-// What a call runs.  Workspace offsets in bytes.
+// What a call runs: the tile kernel, or the stream kernel, and the join.  Workspace offsets in
+// bytes.
 struct Plan8 {
-  bool whole = false;  // a block an item, no workspace
-  int grid = 0, unit_shift = 0;
+  bool whole = false;             // stream kernel, a block an item, no workspace
+  int tile_qt = 0, split = 0;     // tile kernel (0: not at all), parts of the keys
+  int grid = 0, unit_shift = 0;   // stream kernel
   int64_t o_starts = 0, o_ml = 0, o_o = 0, bytes = 0;
 };
 
@@ -543,6 +521,19 @@ template <int HD> static int make_plan8(const cgpt_paged_args& call, Plan8* p) {
     p->grid = static_cast<int>(call.cu_q == nullptr ? items : spread);
     return CGPT_OK;
   }
+  // The join: four rows a block.
+  if (n_tokens * Hq > 4 * kMaxBlocks) return CGPT_ESHAPE;
+  if (rows > 16 * B) {
+    p->tile_qt = Hkv * (rows / 128 + B) >= 4 * cus ? 2 : 1;
+    const int64_t tiles = Hkv * (rows / (64 * p->tile_qt) + B);
+    p->split = static_cast<int>(std::max<int64_t>(1, std::min(6 * cus / tiles, cap / 256)));
+    if (tiles * p->split > kMaxBlocks - 16) return CGPT_ESHAPE;
+    if (p->split > 1) {
+      p->o_ml = take(p->split * n_tokens * Hq * 8);
+      p->o_o = take(p->split * n_tokens * Hq * HD * 4);
+    }
+    return CGPT_OK;
+  }
   constexpr int64_t R = 16, UK = Shape8<HD, stream_waves8(HD)>::UK;
   // Units as large as keep their number, had every sequence the length that the table
   // allows, within 32 bits.
@@ -559,8 +550,6 @@ template <int HD> static int make_plan8(const cgpt_paged_args& call, Plan8* p) {
   p->o_starts = take((B + 1) * 4);
   p->o_ml = take(int64_t{p->grid} * 2 * R * 8);
   p->o_o = take(int64_t{p->grid} * 2 * R * HD * 4);
-  // The join: four rows a block.
-  if (n_tokens * Hq > 4 * kMaxBlocks) return CGPT_ESHAPE;
   return CGPT_OK;
 }
 
@@ -574,30 +563,43 @@ static void launch_stream8(const PagedAttnArgs& a, const Paged8& quant, const Pa
 }
 
 template <typename T, int CODE, int HD>
-static int run_plan8(const PagedAttnArgs& a, const Paged8& quant, const cgpt_paged_args& call, hipStream_t s) {
+static int run_plan8(const PagedAttnArgs& a, const Paged8& quant, const cgpt_paged8_args& args, hipStream_t s) {
+  const cgpt_paged_args& call = args.p;
   Plan8 p;
-  const int rc = make_plan8<HD>(call, &p);
+  int rc = make_plan8<HD>(call, &p);
   if (rc != CGPT_OK) return rc;
   char* w = static_cast<char*>(call.workspace);
   if (p.bytes > 0 && (call.workspace_bytes < p.bytes || w == nullptr)) return CGPT_ESCRATCH;
   if (reinterpret_cast<uintptr_t>(w) & 15) return CGPT_EINVAL;
   PagedWs ws{};
   ws.starts = reinterpret_cast<int*>(w + p.o_starts);
-  ws.edge_ml = reinterpret_cast<float*>(w + p.o_ml);
-  ws.edge_o = reinterpret_cast<float*>(w + p.o_o);
+  ws.edge_ml = ws.tile_ml = reinterpret_cast<float*>(w + p.o_ml);
+  ws.edge_o = ws.tile_o = reinterpret_cast<float*>(w + p.o_o);
   ws.unit_shift = p.unit_shift;
   if (p.whole) {
     launch_stream8<T, CODE, HD, whole_waves8(HD), true>(a, quant, ws, p, s);
     return hip_status(hipGetLastError());
   }
   constexpr int NW = stream_waves8(HD), UK = Shape8<HD, NW>::UK;
-  launch_stream8<T, CODE, HD, NW, false>(a, quant, ws, p, s);
+  if (p.split > 0) {
+    TileJob job{};
+    if (p.split > 1) {
+      job.ml = ws.tile_ml;
+      job.o = ws.tile_o;
+    }
+    job.split = p.split;
+    rc = launch_paged8_tile(args, a, quant, job, p.tile_qt, s);
+    if (rc != CGPT_OK || p.split == 1) return rc;
+  } else {
+    launch_stream8<T, CODE, HD, NW, false>(a, quant, ws, p, s);
+  }
+  const int n_tile = p.split;
   const int rows = a.seq.n_tokens * a.Hq;
   // Few rows have many partials each; many rows want many of them on a CU.
   if (rows < 4 * num_cus())
-    hipLaunchKernelGGL((paged_join_kernel<T, HD, 16, UK, 4>), dim3(rows), dim3(256), 0, s, a, ws, 0, p.grid, 0);
+    hipLaunchKernelGGL((paged_join_kernel<T, HD, 16, UK, 4>), dim3(rows), dim3(256), 0, s, a, ws, 0, p.grid, n_tile);
   else
-    hipLaunchKernelGGL((paged_join_kernel<T, HD, 16, UK, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a, ws, 0, p.grid, 0);
+    hipLaunchKernelGGL((paged_join_kernel<T, HD, 16, UK, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a, ws, 0, p.grid, n_tile);
   return hip_status(hipGetLastError());
 }
 
@@ -620,7 +622,7 @@ extern "C" int cgpt_paged_attention_8bit(const cgpt_paged8_args* args, void* str
                         scale_log2, p.err_flag};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_types8(*args, [&](auto t, auto code, auto hd) {
-    return run_plan8<decltype(t), decltype(code)::value, decltype(hd)::value>(a, paged8(*args), p, s);
+    return run_plan8<decltype(t), decltype(code)::value, decltype(hd)::value>(a, paged8(*args), *args, s);
   });
 }
 

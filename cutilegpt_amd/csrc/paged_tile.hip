@@ -26,7 +26,7 @@
 // has no wave for 13 %, and two waves a SIMD, all that the registers leave, do not fill the
 // rest; 3940 us at 128 (6570).
 #include "internal.h"
-#include "paged.h"
+#include "paged_units.h"
 
 namespace cgpt {
 
@@ -43,44 +43,8 @@ __device__ __forceinline__ void dma_lds16_at(const void* p, uint32_t lds) {
 #pragma clang diagnostic pop
 #endif
 
-// Block i -> (key head, unit of that head), units 0 .. T - 1.  Blocks go to the eight XCDs
-// in turn, each with an L2 of its own: eight heads at a time take one XCD each, the
-// last Hkv % 8 (1, 2 or 4) share the XCDs evenly, so an L2 holds the keys of few heads.
-// Against heads in turn: 2048 tokens behind 20000 keys, 25 heads 274 -> 198 us, 12 heads
-// 116 -> 112; 16 prompts, 4 heads 322 -> 302, 25 heads 521 -> 499, 16 heads 392 -> 396.
-__host__ __device__ inline int head_blocks(int Hkv, int T) {
-  const int r = Hkv & 7;
-  return (Hkv - r) * T + (r == 0 ? 0 : 8 % r == 0 ? (T + 8 / r - 1) / (8 / r) * 8 : r * T);
-}
-__device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* unit) {
-  const int r = Hkv & 7, whole = Hkv - r;
-  if (i < whole * T) {
-    const int group = i / (8 * T), rem = i - group * 8 * T;
-    *hk = 8 * group + (rem & 7);
-    *unit = rem >> 3;
-    return true;
-  }
-  i -= whole * T;
-  if (8 % r == 0) {
-    const int per = 8 / r, x = i & 7;
-    *hk = whole + x / per;
-    *unit = (i >> 3) * per + x % per;
-  } else {
-    *hk = whole + i % r;
-    *unit = i / r;
-  }
-  return *unit < T;
-}
-
-// Chunk swizzle of a key's row in LDS.  Rows of 64 bytes lie four to the banks' 256: a
-// K read's 16 rows then take each chunk four times, and neighbouring groups of four
-// rows, which a transposing V read takes two chunks of, the other two.  Of 32-byte rows the
-// first eight and the next take the other chunk.
-template <int KROW> __device__ __forceinline__ int tile_swz(int row) {
-  if (KROW == 32) return (row >> 3) & 1;
-  return KROW == 64 ? ((row >> 1) & 2) | ((row >> 3) & 1) : row & (KROW >= 256 ? 15 : 7);
-}
-// And of V's: fp32 columns are read by four lane groups, four rows apart and 64 bytes wide each.
+// Chunk swizzle of a value's row in LDS: as a key's (tile_swz), but fp32 columns are read by four
+// lane groups, four rows apart and 64 bytes wide each.
 template <typename T, int KROW> __device__ __forceinline__ int tile_vswz(int row) {
   return sizeof(T) == 2 ? tile_swz<KROW>(row) : row & 12 & (KROW / 16 - 1);
 }

@@ -1,5 +1,5 @@
-// How the stream kernels of the paged caches share out their work, and the kernel that joins
-// their partials.
+// How the kernels of the paged caches share out their work, and the kernel that joins their
+// partials.
 #pragma once
 
 #include "paged.h"
@@ -75,6 +75,48 @@ struct PagedWs {
   float* tile_o;     // splits x n_tokens x Hq x HD
   int unit_shift;    // units of UK << unit_shift keys
 };
+
+// ------------------------------------------------------------------ row tiles
+
+// Block i -> (key head, unit of that head), units 0 .. T - 1.  Blocks go to the eight XCDs
+// in turn, each with an L2 of its own: eight heads at a time take one XCD each, the
+// last Hkv % 8 (1, 2 or 4) share the XCDs evenly, so an L2 holds the keys of few heads.
+// Against heads in turn: 2048 tokens behind 20000 keys, 25 heads 274 -> 198 us, 12 heads
+// 116 -> 112; 16 prompts, 4 heads 322 -> 302, 25 heads 521 -> 499, 16 heads 392 -> 396.
+__host__ __device__ inline int head_blocks(int Hkv, int T) {
+  const int r = Hkv & 7;
+  return (Hkv - r) * T + (r == 0 ? 0 : 8 % r == 0 ? (T + 8 / r - 1) / (8 / r) * 8 : r * T);
+}
+__device__ __forceinline__ bool head_unit(int i, int Hkv, int T, int* hk, int* unit) {
+  const int r = Hkv & 7, whole = Hkv - r;
+  if (i < whole * T) {
+    const int group = i / (8 * T), rem = i - group * 8 * T;
+    *hk = 8 * group + (rem & 7);
+    *unit = rem >> 3;
+    return true;
+  }
+  i -= whole * T;
+  if (8 % r == 0) {
+    const int per = 8 / r, x = i & 7;
+    *hk = whole + x / per;
+    *unit = (i >> 3) * per + x % per;
+  } else {
+    *hk = whole + i % r;
+    *unit = i / r;
+  }
+  return *unit < T;
+}
+
+// Chunk swizzle of a key's row in LDS.  Rows of 64 bytes lie four to the banks' 256: a
+// K read's 16 rows then take each chunk four times, and neighbouring groups of four
+// rows, which a transposing V read takes two chunks of, the other two.  Of 32-byte rows the
+// first eight and the next take the other chunk.
+template <int KROW> __device__ __forceinline__ int tile_swz(int row) {
+  if (KROW == 32) return (row >> 3) & 1;
+  return KROW == 64 ? ((row >> 1) & 2) | ((row >> 3) & 1) : row & (KROW >= 256 ? 15 : 7);
+}
+
+// ------------------------------------------------------------------ the join
 
 // One wave, or with WAVES = 4 one block, a (token, head) row: its partials, each read by
 // HD / 4 lanes, added group of lanes by group and then across the groups, always in the
