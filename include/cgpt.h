@@ -504,7 +504,8 @@ int cgpt_paged_attention_workspace(const cgpt_paged_args* args, int64_t* workspa
  * and the one there, and if it grew the codes in front are rounded again, to nearest even.
  * A code is the exact turned value over 2^e (computed in 64 bits), rounded once to nearest
  * even; turned queries are rounded once to dtype.  Values that are not finite take no part
- * in e: infinities become the largest code, a NaN stays one (int8: 0), and *err_flag is set.
+ * in e: infinities (and turned values past fp32) become the largest code, a NaN stays one
+ * (int8: 0), and *err_flag is set.
  * Two sequences of a call must not write to the same block.
  *
  * cgpt_paged_kv_read_8bit: rows cu_q[b] .. cu_q[b+1]-1 of out and v_out (Hkv heads, strides
