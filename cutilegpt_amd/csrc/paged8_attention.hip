@@ -43,8 +43,9 @@ constexpr int stream_waves8(int hd) { return hd == 128 ? 4 : 1; }
 // from their pages into registers one subtile of KT keys ahead of the one in use, S^T = K Q^T
 // from registers, V through the wave's own LDS tile (as bf16) for its transpose.  WHOLE: a
 // block is one item with all its keys.  A16: 16 keys from a multiple of 16 on lie in one page and
-// block of the exponents: page ids and exponents come by scalar loads; else every lane looks
-// its own key up.
+// block of the exponents: page ids come by scalar loads; else every lane looks its own key up.
+// (Exponents by scalar loads would make every LDS read wait for them: 64 sequences of up to 8192
+// keys, 25 heads of 64, e4m3 188 us so, 172 now.)
 // The exponents: e4m3's go into the conversion to bf16; int8's would cost a product a value
 // there, so with one exponent a tile (A16) they go to the scores and the weights instead.
 template <typename T, int CODE, int HD, bool A16, int NW, bool WHOLE>
@@ -229,11 +230,11 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
         }
       }
     };
-    // The byte at a uniform address, out of the word around it.
-    auto byte_at = [&](const uint8_t* p) __attribute__((always_inline)) {
-      const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-      const uint32_t w = *(const __attribute__((address_space(4))) uint32_t*)(at & ~uintptr_t{3});
-      return static_cast<int>((w >> (8 * (at & 3))) & 0xff);
+    // Past the caches, which have no use for a key that is read once: 64 sequences of up to 8192 keys,
+    // 25 heads of 64, int8 182 -> 169 us; but not rows of two loads, which share their lines (four of
+    // 90 to 130 thousand keys, 8 heads of 128, 164 us, 174 so).
+    auto read_once = [&](const chunk_t* p) __attribute__((always_inline)) {
+      return HD == 128 ? *p : __builtin_nontemporal_load(p);
     };
     const uint32_t k_row = static_cast<uint32_t>(a.kc.ss), v_row = static_cast<uint32_t>(a.vc.ss);
     auto load = [&](int i, const int (&pg)[NT], chunk_t (&kd)[NT][NL], chunk_t (&vd)[NT][NL], int (&kxd)[NT], int (&vxd)[NT])
@@ -253,16 +254,16 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
         const int block = quant.block.div(A16 ? __builtin_amdgcn_readfirstlane(slot) : slot);
         const uint8_t* const ke = ksh + p * quant.ks.sp + block * quant.ks.sb;
         const uint8_t* const ve = vsh + p * quant.vs.sp + block * quant.vs.sb;
-        kxd[kt] = A16 ? byte_at(ke) : *ke;
-        vxd[kt] = A16 ? byte_at(ve) : *ve;
+        kxd[kt] = *ke;
+        vxd[kt] = *ve;
         uint32_t row = 0;
         if (A16) row = tile + 16 <= n ? frow : min(tile + frow, n - 1) - key;
         const uint32_t ko = row * k_row, vo = row * v_row;
         const int c = C::LB * (HD > 16 ? g : g & 1);
 #pragma unroll
         for (int l = 0; l < NL; ++l) {
-          kd[kt][l] = *reinterpret_cast<const chunk_t*>(kp + (ko + c + 64 * l));
-          vd[kt][l] = *reinterpret_cast<const chunk_t*>(vp + (vo + c + 64 * l));
+          kd[kt][l] = read_once(reinterpret_cast<const chunk_t*>(kp + (ko + c + 64 * l)));
+          vd[kt][l] = read_once(reinterpret_cast<const chunk_t*>(vp + (vo + c + 64 * l)));
         }
         // Lanes past a short row's chunks: 0 x NaN would be NaN.
         if (HD == 16 && g >= 2) kd[kt][0] = chunk_t{};
