@@ -1,8 +1,17 @@
 // Writing the 8-bit paged cache, and reading it back as values.
 //
-// append8_kernel: the step's keys and values into codes, a power of two for each block of
-// tokens and head (see paged8.h), keys and queries turned by their positions on the way.
-// read8_kernel: code * 2^e as rows of a wider type.
+// append8_kernel and, for single tokens, append8_step_kernel: the step's keys and values into
+// codes, a power of two for each block of tokens and head (see paged8.h), keys and queries turned
+// by their positions on the way.  read8_kernel: code * 2^e as rows of a wider type.
+//
+// 20 thousand tokens, 12 heads of 64 with turned queries, bf16 into int8: 71 us where the 153 MB
+// alone would take 30 at a copy's 5.18 TB/s.  The VALU is busy 50 % of it (some 36 instructions
+// a value: turning in 64 bits 9, rounding to odd 5, maximum 2, code 2, addresses and unpacking),
+// and the 155 registers leave three waves a SIMD to hide three barriers a head; 128 registers
+// spill (77 us).  With a wave for an item and eight values a lane it took 204.  Eight tokens:
+// 3.9 us (launch and dependent loads).  Reading the 20 thousand tokens back: 23 us, 4.0 TB/s.
+#include <algorithm>
+
 #include "internal.h"
 #include "paged8.h"
 

@@ -7,6 +7,11 @@
 // straight to LDS would have to be turned by every wave for itself.)  S^T = K Q^T and
 // O^T = V^T P^T as there; queries and weights of more bits than bf16 go in as parts (see
 // paged8_attention.hip).
+//
+// 16 chunks of up to 2048 tokens behind up to 4096 keys, 16 heads of 64, e4m3: bf16 331 us, 566
+// TFLOP/s of what the mask leaves (16-bit cache: 303; the stream kernel: 1387), fp16 485, fp32 628
+// (16-bit cache: 1911 in fp32).  As there the VALU's work on the weights bounds it, with the
+// turning of the keys on top.
 #include "internal.h"
 #include "paged8.h"
 #include "paged_units.h"

@@ -13,9 +13,19 @@
 // entry.  (In fp32 a sum of 50 thousand flat weights is off by some 1e-7 of it, and one draw in
 // a hundred would take a neighbour.)
 //
-// A block takes a row.  It needs the maximum, then a histogram of the logits below it (counts
-// and weights), the cut bins' entries, and the sums of the kept weights by segments of the
-// vocabulary.
+// A block takes a row and passes over it: for the maximum; then, where top_k, min_p or the row
+// itself leave few entries that can be kept, for those alone, which are put in order; else for a
+// histogram of the weights by their logits (for a long top_k first one of the counts), and for
+// the sums of the weights in front of the bin that the cut falls into, whose own entries are put
+// in order.  Bins of too many entries are cut again by their keys.  The draw finds the wave's
+// run, the step and the entry.
+//
+// One row of 50257 fp32 logits, top_k 40: 19 us, mostly latencies (of a block's some forty barriers,
+// the passes 4 and 2 us).  64 rows in bf16, top_p among them: 67 us, 256 rows of 128000 in fp32, top_p
+// 0.95: 166 us, 256 in turn on the card's CUs; there the weights of all entries bound it, twice
+// some 45 instructions each.  33 rows of 32001, 97 % masked: 23 us.  (Rows shared out over blocks,
+// a launch for each pass, were slower where rows are few: 37 us for the one, 33 for the 33, 58
+// for the 64.)
 #include "internal.h"
 #include "common.h"
 
