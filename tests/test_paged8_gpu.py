@@ -69,6 +69,40 @@ def test_append_step(gpu, code):
 
 
 @pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype,hd,rot,interleaved", [(BF16, 64, 64, True), (F16, 64, 32, False), (F32, 128, 6, False),
+                                                      (BF16, 16, 16, False), (F32, 32, 20, True), (F16, 128, 128, False)])
+def test_append_step_turned(gpu, code, dtype, hd, rot, interleaved):
+    """Single tokens with every way of turning, more heads than a block's threads have rows."""
+    p = Problem8(dtype, code, hd, 12, 4, Hq=30, Hkv=15, ctx=[0, 3, 11, 12, 50], new=[1] * 5, seed=rot, spread=4)
+    check_append(p, gpu, cg.rotary_table(64, rot, device="cpu"), interleaved)
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("new", [1, 5])
+def test_append_turned_past_the_floats(gpu, code, new):
+    """A key that the turning takes past float32 counts as infinite: the largest code, the flag, and
+    an exponent that goes by the others."""
+    p = Problem8(BF16, code, 64, 16, 1, 1, 1, ctx=[0, 0], new=[new, new], seed=3)
+    rotary = torch.full((new, 64), 0.70710678)
+    p.k[new - 1, 0, 5], p.k[new - 1, 0, 37] = 3e38, -3e38    # to 4.2e38 and 0
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    d, _ = run_append(p, gpu, rotary, err_flag=flag)
+    assert int(flag) == 1
+    want, _ = append(p, rotary)
+    page, slot = int(p.table[0, 0]), new - 1
+    got, top = d.k_cache[page, 0, slot].cpu().double(), 448.0 if code == F8 else 127.0
+    assert float(got[5]) == top
+    # The rest of the row is there on a scale of its own size.
+    e = int(d.k_scale[page, 0, slot]) - 127
+    clean = p.k[new - 1, 0].clone()
+    clean[5], clean[37] = 0, 0
+    assert top * 2.0 ** e >= float(clean.abs().max()) / 2 and top * 2.0 ** e < 1e6
+    # Another sequence's rows are as they would be.
+    other = int(p.table[1, 0])
+    same_bytes(d.k_cache[other], want[0][other], "k")
+
+
+@pytest.mark.parametrize("code", [F8, I8])
 def test_append_long_blocks(gpu, code):
     """Blocks of more rows than a wave takes at once, prompts of many blocks."""
     p = Problem8(F16, code, 128, 256, 256, Hq=2, Hkv=2, ctx=[0, 300], new=[700, 213], seed=4)
@@ -386,6 +420,18 @@ def test_many_sequences(gpu, code, B, new, room):
     g = torch.Generator().manual_seed(B)
     ctx = torch.randint(0, 150, (B,), generator=g).tolist()
     p = problem(BF16, code, 32, 16, 16, 2, 1, ctx=ctx, new=[new] * B, seed=B, spare_cols=room)
+    check_attention(p, gpu)
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype,hd,page,block", [(BF16, 64, 16, 16), (F16, 128, 10, 5), (F32, 64, 24, 8), (F32, 128, 16, 16),
+                                                 (BF16, 16, 8, 8), (F16, 32, 64, 64)])
+def test_tiles_of_128_rows(gpu, code, dtype, hd, page, block):
+    """Batches that fill the card with large tiles, most of them not full."""
+    g = torch.Generator().manual_seed(hd)
+    new = torch.randint(12, 30, (64,), generator=g).tolist()
+    new[5], new[9] = 150, 0
+    p = problem(dtype, code, hd, page, block, 16, 16, ctx=torch.randint(0, 70, (64,), generator=g).tolist(), new=new, seed=hd)
     check_attention(p, gpu)
 
 
