@@ -134,11 +134,14 @@ struct RowScale {
   bool odd;          // infinite logits, or a temperature next to 0: the largest weigh 1, others 0
 };
 
-// The weight of an entry from `lightest` on (others give anything): 2^(z / 256) by a table of 256
-// roots and a polynomial in the rest of z, whose relative error is 2^-54 in exact arithmetic.
+// An entry's weight: 2^(z / 256) by a table of 256 roots and a polynomial in the rest of z, whose
+// relative error is 2^-54 in exact arithmetic.  2^-46 and less round to 0 all alike: z ends there,
+// as what follows adds z >> 8 to an exponent, which must not wrap (-inf, and the NaN of -inf
+// times a rate of 0, end there too).  So every entry can be weighed, kept or not.
 __device__ __forceinline__ u64_t weight(const SampleShared& sh, const RowScale& r, float v) {
   double z = (static_cast<double>(v) - r.max) * r.rate;
-  if (r.odd) z = v == r.fmax ? 0.0 : -1e5;  // (inf - inf, or 0 / 0)
+  if (r.odd) z = v == r.fmax ? 0.0 : -INFINITY;  // (inf - inf, or 0 / 0)
+  z = __builtin_fmax(z, -46.0 * 256.0);
   // The nearest whole number, and as an integer, from the sum's last bits.
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
   const double big = z + kMagic;
@@ -154,8 +157,7 @@ __device__ __forceinline__ u64_t weight(const SampleShared& sh, const RowScale& 
   // (The table holds 2^43 as well.)  Times 2^(i >> 8) in its exponent, then rounded to a whole
   // number by the sum with 2^52.
   const u64_t scaled = __double_as_longlong(e) + (static_cast<u64_t>((i & ~255u) << 12) << 32);
-  const u64_t w = __double_as_longlong(__longlong_as_double(scaled) + 4503599627370496.0) & 0xfffffffffffffull;
-  return r.odd && v != r.fmax ? 0 : w;
+  return __double_as_longlong(__longlong_as_double(scaled) + 4503599627370496.0) & 0xfffffffffffffull;
 }
 
 __device__ __forceinline__ int bin_of(const RowScale& r, float v) {

@@ -267,3 +267,61 @@ def test_refusals(gpu):
     refused("min_p", min_p=torch.zeros(3, dtype=torch.float64, device=gpu))
     refused("out must", out=torch.zeros(3, dtype=torch.int32, device=gpu))
     refused("shape outside", x=torch.zeros(1, (1 << 20) + 1, device=gpu), u=u[:1])
+
+
+def draws(row, u, T=1.0, k=0, p=1.0, m=0.0):
+    """``draw`` of one row for many numbers: (tokens, margins), (tokens that can come)."""
+    idx, w = kept(row, T, k, p, m)
+    order = sorted((i, a) for i, a in zip(idx, w) if a > 0)
+    at, w = torch.tensor([i for i, _ in order]), torch.tensor([a for _, a in order], dtype=torch.float64)
+    ends = w.cumsum(0)
+    goal = u.double() * ends[-1]
+    j = torch.searchsorted(ends, goal, right=True).clamp(max=len(at) - 1)
+    return at[j], torch.minimum(goal - (ends[j] - w[j]), ends[j] - goal) / ends[-1], at
+
+
+def check_row(row, n, gpu, seed, **s):
+    """n draws from one row, each the float64 one."""
+    u = torch.rand(n, generator=torch.Generator().manual_seed(seed))
+    u[0], u[1] = 0.0, 1 - 2.0 ** -24
+    want, margin, can = draws(row, u, **s)
+    T, rest = s.get("T", 1.0), dict(top_k=s.get("k"), top_p=s.get("p"), min_p=s.get("m"))
+    got = cg.sample_tokens(row.repeat(n, 1).to(gpu), u.to(gpu), temperature=T, **rest).cpu()
+    assert bool(torch.isin(got, can).all()), (s, "tokens without a weight", got[~torch.isin(got, can)][:5].tolist())
+    bad = (got != want) & (margin >= (len(row) + 64) * 2.0 ** -44)
+    assert not bad.any(), (s, int(bad.sum()), got[bad][:5].tolist(), want[bad][:5].tolist())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", [5000, 50257])
+@pytest.mark.parametrize("low", [-1e3, -1e4, -65504.0, -1e9, None])
+def test_finite_masks(gpu, dtype, V, low):
+    """Masked entries are finite (None: the type's lowest value) among thousands that can be drawn,
+    with nothing cut, min_p alone, and a top_k that reaches into the masked ones."""
+    if dtype == F16 and low == -1e9:
+        low = -3e4
+    low = torch.finfo(dtype).min if low is None else low
+    g = torch.Generator().manual_seed(V)
+    for n_masked in (1, 20, V // 2):
+        row = torch.randn(V, generator=g) * 2.5
+        row[torch.randperm(V, generator=g)[:n_masked]] = low
+        row = row.to(dtype)
+        for T in (0.1, 0.3, 0.7, 0.8, 1.0, 1.2):
+            check_row(row, 48, gpu, n_masked, T=T)
+        check_row(row, 48, gpu, 1, T=1.2, m=1e-6)
+        check_row(row, 48, gpu, 2, T=0.8, m=1e-12)
+        check_row(row, 48, gpu, 3, T=0.8, k=V - n_masked // 2)
+        check_row(row, 48, gpu, 4, T=0.7, k=V - n_masked // 2, m=1e-9)
+        check_row(row, 48, gpu, 5, T=0.8, p=0.999999)
+
+
+@pytest.mark.parametrize("T", [1e-7, 1e-8, 1e-9, 1e-10, 1e-20, 1e-38])
+@pytest.mark.parametrize("V", [1500, 9000])
+def test_temperatures_below_the_logits_steps(gpu, T, V):
+    """Thousands of logits a few steps of fp32 apart, at temperatures that make one step the whole
+    distribution or more."""
+    g = torch.Generator().manual_seed(V)
+    row = 10.0 + torch.randint(-30, 1, (V,), generator=g).float() * 2.0 ** -20
+    row[::7] = 10.0
+    for s in (dict(), dict(k=1000), dict(k=V - 3), dict(p=0.5), dict(p=0.99), dict(m=0.5), dict(m=1e-9), dict(k=1200, p=0.7, m=0.01)):
+        check_row(row, 32, gpu, 1, T=T, **s)
