@@ -319,9 +319,9 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args a, int units) 
   // (Queries past the table are still turned.)
   const int q1 = static_cast<int>(min(static_cast<int64_t>(len), base64 + W)), p1 = min(q1, hi);
   const int r = tid / LPR;
-  // Thread i: block i's place.
+  // Thread i: block i's place, of those that rows are written to (a sequence without tokens has none).
   const int first_p = base + tid * blk, col = a.seq.page.div(max(min(first_p, hi - 1), 0));
-  const bool mine = tid < a.per_item && first_p < p1 && first_p + blk > p0;
+  const bool mine = p0 < p1 && tid < a.per_item && first_p < p1 && first_p + blk > p0;
   const int page = mine ? a.seq.table[b * a.seq.stride + col] : -1;
   const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.seq.n_pages);
   flag |= mine && !there;

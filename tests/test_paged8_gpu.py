@@ -694,3 +694,18 @@ def test_refusals(gpu):
         cg.paged_kv_read_8bit(*d.cache, d.cu, 2, torch.float64)
     with pytest.raises(ValueError, match="k_out and v_out"):
         cg.paged_kv_read_8bit(*d.cache, d.cu, 2, BF16, k_out=torch.empty(3, 2, 64, dtype=BF16, device=gpu))
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("hd,block", [(64, 16), (64, 8), (128, 8), (16, 16)])
+def test_append_sequences_without_tokens(gpu, code, hd, block):
+    """A sequence that has no token in the step has nothing read: an unused table entry where its
+    last keys would be sets no flag, and nothing is written."""
+    p = Problem8(BF16, code, hd, 16, block, 4, 2, ctx=[5, 21, 30, 0, 16], new=[3, 0, 2, 0, 0], seed=hd + block)
+    p.table[1], p.table[4] = -7, p.n_pages
+    want, _ = append(p)
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    d, _ = run_append(p, gpu, err_flag=flag)
+    assert int(flag) == 0
+    for x, w, what in zip(d.cache, want, ("k_cache", "v_cache", "k_scale", "v_scale")):
+        same_bytes(x, w, what)
