@@ -128,7 +128,7 @@ def paged_kv_append_8bit(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor
     code, n_pages, hkv, page, hd, cs, ss, block, B, cols, ts = _check_cache8(
         name, dev, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_q, err_flag)
     dt = _check_rows8(name, "k", k, B, hd, cu_q)
-    if not all(t is None or isinstance(t, torch.Tensor) for t in (v, q, rotary)):
+    if not isinstance(v, torch.Tensor) or not all(t is None or isinstance(t, torch.Tensor) for t in (q, rotary)):
         raise ValueError(f"{name}: k, v, q and rotary must be torch tensors")
     n, vec = k.shape[0], 8 if dt else 4
     if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != dev or k.shape[1] != hkv:

@@ -709,3 +709,10 @@ def test_append_sequences_without_tokens(gpu, code, hd, block):
     assert int(flag) == 0
     for x, w, what in zip(d.cache, want, ("k_cache", "v_cache", "k_scale", "v_scale")):
         same_bytes(x, w, what)
+
+
+def test_append_refuses_missing_values(gpu):
+    d = Problem8(BF16, F8, 64, 16, 8, 4, 2, ctx=[30], new=[1], seed=2).on(gpu)
+    for v in (None, 3):
+        with pytest.raises(ValueError, match="torch tensors"):
+            cg.paged_kv_append_8bit(d.k, v, *d.cache)
