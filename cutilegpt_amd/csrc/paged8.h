@@ -7,8 +7,8 @@
 // matrix cores take cached values as they are; and where a block's exponent grows as tokens
 // are added, its codes are shifted, not rounded to another grid (e4m3: exact above its
 // subnormals; int8: the half steps of all shifts add up to less than one step).
-// Exponents lie in [kMinExp, kMaxExp]: from there up every code's value is a normal
-// bf16 number, and a weight times 2^e too; up to there the largest is finite.
+// Exponents lie between kMinExp and 119 (e4m3) or 121 (int8): from there up every code's value is
+// a normal bf16 number, 2^-kValueDrop of it too; up to there the largest code's value is finite.
 #pragma once
 
 #include "paged.h"
@@ -106,6 +106,18 @@ template <int CODE> __device__ __forceinline__ int clamp_exp(int byte) {
 }
 template <int CODE> __device__ __forceinline__ float scale_of(int byte) {
   return __uint_as_float(static_cast<uint32_t>(clamp_exp<CODE>(byte)) << 23);
+}
+
+// Values enter the attention's second product 2^kValueDrop smaller, and the weights' sum is made as
+// much smaller before it divides.  A weight reaches 2^8 where its score comes up to 8 above the
+// running shift, so without that the largest exponents' products would be infinite where the
+// result is not (and with the exponent in the weight, int8, inf x 0 a NaN for codes of 0).
+// So much holds for one key; a sum of weights times values may still pass fp32 where values
+// above 2^120 meet hundreds of keys as heavy as the heaviest.
+constexpr int kValueDrop = 8;
+constexpr float kSumDrop = 1.f / (1 << kValueDrop);
+template <int CODE> __device__ __forceinline__ float value_scale_of(int byte) {
+  return __uint_as_float(static_cast<uint32_t>(clamp_exp<CODE>(byte) - kValueDrop) << 23);
 }
 
 // The codes.  kTop: the largest code's value.

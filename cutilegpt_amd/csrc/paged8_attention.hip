@@ -286,7 +286,7 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) {
         const int key = 16 * kt + frow;
-        const float f = FOLD ? 1.f : scale_of<CODE>(vxd[kt]);
+        const float f = FOLD ? 1.f : value_scale_of<CODE>(vxd[kt]);
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
           uint32_t w0 = vd[kt][s >> 1][2 * (s & 1)], w1 = vd[kt][s >> 1][2 * (s & 1) + 1];
@@ -351,7 +351,7 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
       float sum = 0.f;
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) {
-        const float fv = FOLD ? scale_of<CODE>(vxd[kt]) : 1.f;
+        const float fv = FOLD ? value_scale_of<CODE>(vxd[kt]) : 1.f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], fk[kt], shift));
@@ -432,7 +432,7 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
     const bool whole = t0 == 0 && t1 == kt_item;
     const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
     {
-      const float l = column_sum(l_run);
+      const float l = column_sum(l_run) * kSumDrop;
       if (g == 0) {
         wave_m[wave][frow] = m_run;
         wave_l[wave][frow] = l;

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kTile8Threads) void paged8_tile_kernel(PagedAttnArg
   // The loaded codes as bf16 into a buffer.  Values that are no numbers become 0 there (0 x NaN
   // would spoil rows that do not see them) and are added at the end.
   auto stage = [&](uint8_t* buf) __attribute__((always_inline)) {
-    const float fk = scale_of<CODE>(kx), fv = scale_of<CODE>(vx);
+    const float fk = scale_of<CODE>(kx), fv = value_scale_of<CODE>(vx);
     uint8_t* const kd = buf + krow * KROW;
     uint8_t* const vd = kd + XB;
     const int swz = tile_swz<KROW>(krow);
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(kTile8Threads) void paged8_tile_kernel(PagedAttnArg
   // ---- out: lane holds O[row][16 dt + 4 g .. +3]
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    const float l = column_sum(l_run[qt]);
+    const float l = column_sum(l_run[qt]) * kSumDrop;
     const int r = wr0 + 16 * qt + frow;
     if (r >= rows) continue;
     const int i = a.group.div(r), h = hk * G + r - i * G, t = first + i;

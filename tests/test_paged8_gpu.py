@@ -716,3 +716,40 @@ def test_append_refuses_missing_values(gpu):
     for v in (None, 3):
         with pytest.raises(ValueError, match="torch tensors"):
             cg.paged_kv_append_8bit(d.k, v, *d.cache)
+
+
+def one_key(dtype, code, score, ctx, new, hd=64, page=16, block=16, B=1, spare_cols=1):
+    """Scores 0 but for each sequence's key at ctx - 1, which every token sees: ``score`` in base 2
+    with scale score ln 2.  Values 0 but for that key's block, whose exponents are the largest: the key
+    itself has the largest code in every other place."""
+    p = problem(dtype, code, hd, page, block, 4, 2, ctx=[ctx] * B, new=[new] * B, seed=1, spare_cols=spare_cols)
+    p.q.zero_()
+    p.q[..., 0] = 1.0
+    owned = p.table[:, :-(-p.total[0] // page)].flatten().long()
+    for cache in (p.k_cache, p.v_cache):
+        cache.view(torch.uint8)[owned] = 0
+    p.k_scale.fill_(127)
+    p.v_scale.fill_(127)
+    at, slot = p.table[:, (ctx - 1) // page].long(), (ctx - 1) % page
+    p.k_cache.view(torch.uint8)[at, :, slot, 0] = 0x38 if code == F8 else 1          # 1.0
+    p.v_cache.view(torch.uint8)[at, :, slot, ::2] = 0x7e if code == F8 else 127      # 448, 127
+    p.v_scale[at, :, slot // block] = 255
+    return p, score * 0.6931471805599453
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,new,room,block,hd", [(1, 1, 1, 16, 64), (1, 1, 1, 8, 64), (1, 1, 1, 16, 32), (300, 1, 400, 16, 64),
+                                                 (300, 1, 400, 8, 64), (300, 3, 400, 16, 128), (1, 40, 1, 16, 64), (1, 40, 1, 8, 16)])
+def test_values_next_to_the_end_of_the_floats(gpu, dtype, code, B, new, room, block, hd):
+    """A key whose score comes up to 8 (in base 2) above those in front of it, and values of the
+    largest exponent: results next to the largest number of float32, and 0 beside them."""
+    for score in (7.9, 1.0, 30.0):
+        p, scale = one_key(dtype, code, score, 1220, new, hd, block=block, B=B, spare_cols=room)
+        want, bound = attention(p, scale)
+        got = run_attention(p, gpu, scale=scale).cpu()
+        assert bool((got[..., 1::2] == 0).all()), score
+        if dtype == F16:
+            assert bool((got[..., ::2] == torch.inf).all()) and float(want[..., ::2].min()) > 1e6, score
+        else:
+            within(got, want, bound, f"score {score}")
