@@ -54,7 +54,7 @@ constexpr int stream_waves8(int hd) { return hd == 128 ? 4 : 1; }
 // (Exponents by scalar loads would make every LDS read wait for them: 64 sequences of up to 8192
 // keys, 25 heads of 64, e4m3 188 us so, 172 now.)
 // The exponents: e4m3's go into the conversion to bf16; int8's would cost a product a value
-// there, so with one exponent a tile (A16) they go to the scores and the weights instead.
+// there, so with one exponent a tile (A16) they go to the scores' scale and the weights instead.
 template <typename T, int CODE, int HD, bool A16, int NW, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void
 paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
@@ -563,8 +563,11 @@ template <int HD> static int make_plan8(const cgpt_paged_args& call, Plan8* p) {
 
 template <typename T, int CODE, int HD, int NW, bool WHOLE>
 static void launch_stream8(const PagedAttnArgs& a, const Paged8& quant, const PagedWs& ws, const Plan8& p, hipStream_t s) {
-  // (Offsets of 16 slots fit 32 bits.)
-  if (quant.block.d % 16 == 0 && short_rows(a))
+  // Offsets of 16 slots fit 32 bits; and where a tile's exponent and the scale become one factor
+  // (int8), it is a normal float whatever the exponent, -100 to 121: else a masked key's
+  // -inf x 0 or a zero key's 0 x inf would be a NaN.
+  const bool one_factor = CODE != CGPT_INT8 || (a.scale_log2 >= 0x1p-26f && a.scale_log2 <= 0x1p6f);
+  if (quant.block.d % 16 == 0 && short_rows(a) && one_factor)
     hipLaunchKernelGGL((paged8_stream_kernel<T, CODE, HD, true, NW, WHOLE>), dim3(p.grid), dim3(64 * NW), 0, s, a, quant, ws);
   else
     hipLaunchKernelGGL((paged8_stream_kernel<T, CODE, HD, false, NW, WHOLE>), dim3(p.grid), dim3(64 * NW), 0, s, a, quant, ws);

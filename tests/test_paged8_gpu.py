@@ -753,3 +753,26 @@ def test_values_next_to_the_end_of_the_floats(gpu, dtype, code, B, new, room, bl
             assert bool((got[..., ::2] == torch.inf).all()) and float(want[..., ::2].min()) > 1e6, score
         else:
             within(got, want, bound, f"score {score}")
+
+
+@pytest.mark.parametrize("code", [F8, I8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new,room", [(1, 1), (1, 400), (5, 400), (40, 1)])
+def test_scales_far_from_1(gpu, dtype, code, new, room):
+    """Scales at which a block's exponent and the scale together leave the floats: blocks of zero keys,
+    of the smallest exponent under a tiny scale, of the largest under a large one."""
+    p = problem(dtype, code, 64, 16, 16, 4, 2, ctx=[150, 33], new=[new, new], seed=11, spare_cols=room)
+    p.k_scale.fill_(27)
+    for scale in (1e-16, 1e-30, 1e-43):
+        want, bound = attention(p, scale)
+        within(run_attention(p, gpu, scale=scale), want, bound, str(scale))
+    p.k_scale.fill_(100)
+    for b, total in enumerate(p.total):
+        for col in range(0, total // 16, 3):
+            page = int(p.table[b, col])
+            p.k_cache.view(torch.uint8)[page] = 0
+            p.k_scale[page] = 255
+    for scale in (100.0, 1e4):
+        p.q.mul_(0.01)
+        want, bound = attention(p, scale)
+        within(run_attention(p, gpu, scale=scale), want, bound, str(scale))
