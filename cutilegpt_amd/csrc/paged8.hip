@@ -284,12 +284,12 @@ __global__ __launch_bounds__(256) void append8_step_kernel(Append8Args a) {
 // Any numbers of tokens.  A block takes an item, per_item neighbouring blocks of one sequence, for
 // `units` of the heads, one after the other; the sequence's items are those that its step
 // touches.  Its waves take rows in turn, lanes 16 values each of a row.  First the largest value of
-// every block (in LDS), then its exponent, then the codes.  kKeep steps of rows stay in registers for
+// every block (in LDS), then its exponent, then the codes.  One step of rows stays in registers for
 // that; longer items are read twice, the second time from the cache.
 constexpr int kItemBlocks = 64;
 template <typename T, int CODE, int HD>
 __global__ __launch_bounds__(256) void append8_kernel(Append8Args a, int units) {
-  constexpr int LPR = HD / 16, RPI = 256 / LPR, kKeep = 1;
+  constexpr int LPR = HD / 16, RPI = 256 / LPR;
   __shared__ uint32_t top[2][kItemBlocks], past[2][kItemBlocks];
   __shared__ int exps[2][kItemBlocks], page_of_block[kItemBlocks], grown_by[2];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -336,32 +336,26 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args a, int units) 
     if (p0 >= p1) continue;
     // ---- the blocks' largest values (of two units in turn: no wait before the next begins)
     const int turn = (unit - unit0) & 1;
-    float y[kKeep][16];
-    uint32_t tops[kKeep];
-    bool odd[kKeep];
-    auto load_run = [&](int from) __attribute__((always_inline)) {
-#pragma unroll
-      for (int it = 0; it < kKeep; ++it) {
-        const int p = from + it * RPI + r;
-        if (p < p1) tops[it] = u.template row<LPR>(a, first + (p - pos0), p, &flag, &odd[it], y[it]);
-      }
+    float y[16];
+    uint32_t row_max = 0;
+    bool odd = false;
+    auto load_rows = [&](int from) __attribute__((always_inline)) {
+      const int p = from + r;
+      if (p < p1) row_max = u.template row<LPR>(a, first + (p - pos0), p, &flag, &odd, y);
     };
-    load_run(p0);
+    load_rows(p0);
     __syncthreads();
     if (tid < kItemBlocks) top[turn ^ 1][tid] = past[turn ^ 1][tid] = 0;
     if (tid == 0) grown_by[turn] = 0;
-    for (int from = p0; from < p1; from += kKeep * RPI) {
-      if (from != p0) load_run(from);
-#pragma unroll
-      for (int it = 0; it < kKeep; ++it) {
-        const int p = from + it * RPI + r;
-        if (p < p1) {
-          const int i = a.quant.block.div(p - base);
-          if (tid % LPR == 0) atomicMax(&top[turn][i], tops[it]);
-          if (odd[it]) {
-            flag = true;
-            past[turn][i] = 1;
-          }
+    for (int from = p0; from < p1; from += RPI) {
+      if (from != p0) load_rows(from);
+      const int p = from + r;
+      if (p < p1) {
+        const int i = a.quant.block.div(p - base);
+        if (tid % LPR == 0) atomicMax(&top[turn][i], row_max);
+        if (odd) {
+          flag = true;
+          past[turn][i] = 1;
         }
       }
     }
@@ -392,16 +386,13 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args a, int units) 
       for (int p = base + i * blk + r; p < p0; p += RPI) shift16<CODE>(row_of(p, i) + 16 * (tid % LPR), grown_by[turn]);
     }
     // ---- the codes
-    const bool again = p1 - p0 > kKeep * RPI;
-    for (int from = p0; from < p1; from += kKeep * RPI) {
-      if (again) load_run(from);
-#pragma unroll
-      for (int it = 0; it < kKeep; ++it) {
-        const int p = from + it * RPI + r;
-        if (p >= p1) continue;
-        const int i = a.quant.block.div(p - base), e = exps[turn][i];
-        if (e >= 0) put16<CODE>(row_of(p, i), u.c, y[it], e);
-      }
+    const bool again = p1 - p0 > RPI;
+    for (int from = p0; from < p1; from += RPI) {
+      if (again) load_rows(from);
+      const int p = from + r;
+      if (p >= p1) continue;
+      const int i = a.quant.block.div(p - base), e = exps[turn][i];
+      if (e >= 0) put16<CODE>(row_of(p, i), u.c, y, e);
     }
   }
   if (flag && a.err != nullptr) *a.err = 1;
