@@ -5,11 +5,13 @@
 // by their positions on the way.  read8_kernel: code * 2^e as rows of a wider type.
 //
 // 20 thousand tokens, 12 heads of 64 with turned queries, bf16 into int8: 71 us where the 153 MB
-// alone would take 30 at a copy's 5.18 TB/s.  The VALU is busy 50 % of it (some 36 instructions
-// a value: turning in 64 bits 9, rounding to odd 5, maximum 2, code 2, addresses and unpacking),
-// and the 155 registers leave three waves a SIMD to hide three barriers a head; 128 registers
-// spill (77 us).  With a wave for an item and eight values a lane it took 204.  Eight tokens:
-// 3.9 us (launch and dependent loads).  Reading the 20 thousand tokens back: 23 us, 4.0 TB/s.
+// alone would take 30 at a copy's 5.18 TB/s.  No unit is busy throughout: the VALU 53 % (some 35
+// instructions a value: turning in 64 bits 9, rounding to odd 5, maximum 2, code 2, addresses and
+// unpacking), the memory 2.2 TB/s, and 2.3 waves a SIMD (153 registers, which every way of turning
+// shares; 128 spill, 77 us) wait at three barriers a head, with none of the next head's rows on
+// their way meanwhile.  With a wave for an item and eight values a lane it took 204.  Eight
+// tokens: 3.9 us (launch and dependent loads).  Reading the 20 thousand tokens back: 23 us, 4.0
+// TB/s.
 #include <algorithm>
 
 #include "internal.h"
@@ -238,7 +240,10 @@ template <typename T> struct Unit8 {
 };
 
 // One token a sequence: a row's lanes take one head.  Bound by the launch and dependent loads
-// (length, page, exponent).
+// (length, page, exponent): 64 sequences, 25 heads of 64, 2 to 3 us within a graph, whatever the
+// block.  But where a head's exponent grows, its row's lanes shift the block's earlier rows one
+// after another, a load and a store each: a last token in blocks of 16 / 64 / 256 slots, two heads
+// growing, e4m3 9 / 34 / 127 us, int8 17 / 63 / 248.
 template <typename T, int CODE, int HD>
 __global__ __launch_bounds__(256) void append8_step_kernel(Append8Args a) {
   constexpr int LPR = HD / 16;

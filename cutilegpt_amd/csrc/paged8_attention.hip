@@ -8,16 +8,24 @@
 // whatever the queries' type, and a query or a weight of more bits goes in as the sum of its
 // bf16 parts: one for bf16, two for fp16 (8 + 8 bits hold its 11), three for fp32 (24).  All
 // types so have bf16's range on the way, and fp32 costs three products, not the sixteen times
-// that the fp32 matrix instruction takes.  A weight is rounded to its parts (2^-9, 2^-17 or
-// 2^-25 relative) for the second product, where the result is rounded to the queries' type
-// as coarsely; sums, maxima and the shift are fp32.
+// that the fp32 matrix instruction takes.  A weight is rounded to its parts (2^-8, 2^-17 or
+// 2^-26 relative) for the second product, where the result is rounded to the queries' type
+// as coarsely (bf16: results are 0.0019 off in all, 0.0017 with exact weights; a second part
+// would be a second product and five instructions a pair of weights more); sums, maxima and the
+// shift are fp32.
 //
 // Two kernels, the stream kernel here for few rows (a decode step reads every key once: the
 // bound is HBM) and the tile kernel (paged8_tile.hip) for more than 16 a sequence and head; make_plan8
-// chooses.  64 sequences of 1 to 8192 keys, 25 heads of 64: int8 159 to 164 us, 5.1 to 5.3 TB/s, e4m3
-// 172, where the 16-bit cache takes 295; four of 90 to 130 thousand, 8 heads of 128, e4m3, fp16
-// 173 us, 5.2 TB/s (308 in 16 bits).  At head_dim 32 a key's 64 bytes leave too few for the some 5
-// instructions that it costs: 3.2 TB/s.  One sequence of 500 keys: 7.3 us.
+// chooses, by the whole call's rows a sequence: where one long chunk comes with many single tokens
+// its keys are read once for every 16 of its rows (63 single tokens behind 500 to 4000 keys 65 to
+// 70 us, 500 tokens behind 3000 keys 35, both in one call 113).
+//
+// 64 sequences of 1 to 8192 keys, 25 heads of 64: int8 158 to 163 us, 5.1 to 5.3 TB/s, e4m3
+// 153 to 155, where the 16-bit cache takes 295 (queries in fp32: 192 and 176); four of 90 to 130
+// thousand, 8 heads of 128, e4m3, fp16 173 us, 5.2 TB/s (308 in 16 bits).  With heads of 32, half
+// the bytes, int8 142 us and e4m3 134 (3.0 and 3.1 TB/s), of 16 147 and 133: the instructions a key
+// costs hardly shrink with it (vector ones 5.4 of a wave, 6.5 at 64; scalar 6.2 and 6.2), and no
+// unit is busy throughout (VALU 42 %, 1.5 waves a SIMD).  One sequence of 500 keys: 7.4 us.
 #include <algorithm>
 
 #include "internal.h"
@@ -237,7 +245,8 @@ paged8_stream_kernel(PagedAttnArgs a, Paged8 quant, PagedWs ws) {
         }
       }
     };
-    // Past the caches, which have no use for a key that is read once: 64 sequences of up to 8192 keys,
+    // Past the caches, which have no use for a key that is read once (as all are but those of
+    // sequences of more than 16 rows beside many short ones): 64 sequences of up to 8192 keys,
     // 25 heads of 64, int8 182 -> 169 us; but not rows of two loads, which share their lines (four of
     // 90 to 130 thousand keys, 8 heads of 128, 164 us, 174 so).
     auto read_once = [&](const chunk_t* p) __attribute__((always_inline)) {

@@ -21,9 +21,10 @@
 // run, the step and the entry.
 //
 // One row of 50257 fp32 logits, top_k 40: 19 us, mostly latencies (of a block's some forty barriers,
-// the passes 4 and 2 us).  64 rows in bf16, top_p among them: 67 us, 256 rows of 128000 in fp32, top_p
-// 0.95: 166 us, 256 in turn on the card's CUs; there the weights of all entries bound it, twice
-// some 45 instructions each.  33 rows of 32001, 97 % masked: 23 us.  (Rows shared out over blocks,
+// the passes 4 and 2 us; temperature 0, two passes alone, 10).  64 rows in bf16, top_p among them: 68
+// us, on 64 of 256 CUs (a wave on 9 % of them, the mean over the call).  256 rows of 128000 in fp32,
+// top_p 0.95: 164 us, a row a CU; 126 vector instructions an entry (two weights of some 24, 14 of
+// those in 64 bits, beside bins, cuts and atomics) keep the VALU busy 60 %.  33 rows of 32001, 97 % masked: 22 us.  (Rows shared out over blocks,
 // a launch for each pass, were slower where rows are few: 37 us for the one, 33 for the 33, 58
 // for the 64.)
 #include "internal.h"

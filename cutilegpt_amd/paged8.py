@@ -239,7 +239,9 @@ def paged_attention_8bit(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     sequences' pages; returns the same shape and type.
 
     Cached values are taken exactly as code * 2^e.  Queries and probabilities enter the
-    products with the bits of their type at least, statistics and sums are float32."""
+    products with the bits of the queries' type at least, statistics and sums are float32:
+    under bfloat16 queries the probabilities are rounded to bfloat16, as in
+    ``paged_attention``; float16 and float32 queries keep 16 and 24 bits of them."""
     name = "paged_attention_8bit"
     try:
         dev = q.get_device()

@@ -37,7 +37,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     at least ``top_p`` of their weight; of it those of at least ``min_p`` of the largest
     weight.  The draw is the first index, in the order of the vocabulary, at which the
     running sum of the kept weights exceeds u times their sum.  Weights are exact to 2^-44
-    of the largest and their sums exact, so a draw does not depend on how they are added.
+    of the largest (smaller ones are 0: a mask may be -inf or any number far enough down) and
+    their sums exact, so a draw does not depend on how they are added.
 
     Each setting is a number for all rows or a tensor (B,), float32 (``top_k`` int32), read
     on the device.  None, a ``top_k`` of 0, a ``top_p`` of 1 or a ``min_p`` of 0 cut nothing.
